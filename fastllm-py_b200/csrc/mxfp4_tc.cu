@@ -1,0 +1,542 @@
+// Products of bfloat16 rows with a matrix in microscaled 4-bit floating point on the tensor cores (mxfp4.cu says what the
+// packed form is): out[t, f] = sum_k x[t, k] W[f, k], and the gated unit act(gate) * up of two such products.
+//
+// The weights are turned into bfloat16 on their way (exactly: a magnitude of two bits of significand times a power of two) and
+// go to tensor memory as the MMA's A operand; the tokens come to shared memory by TMA as its B operand.  So the 16-bit form of
+// the weights touches neither global nor shared memory, whose bandwidth the MMA needs for the tokens.
+//
+// A CTA takes two tiles of 128 rows of W (of a gated unit: a gate tile and the up tile of the same features) and up to 128
+// tokens.  Warps 0-7: each thread reads one row's codes from global memory, two chunks ahead, and writes 64 elements of K a
+// time to tensor memory, a ring of MXT_A stages; then the epilogue.  Warp 8: the tokens' TMA.  Warp 9: the MMAs.  Where there
+// are fewer tiles than SMs a cluster of up to 8 CTAs shares K; its partial sums stay in shared memory, and each CTA adds up
+// its share of the tokens from all of them, in rank order.
+#include "tcgen05.cuh"
+
+#define MX_ROWS 128
+#define MX_CODES 8192
+#define MX_CHUNK 8704
+#define MXT_BN 128                          // most tokens of a tile
+#define MXT_A 4                             // stages of 2 x 32 columns in tensor memory
+#define MXT_RING (144 * 1024)               // the tokens' ring; the epilogue's sums take its place
+#define MXT_MAX_STAGES 16
+#define MXT_PITCH 256                       // floats between the tokens of the sums
+// (No other kernel that takes tensor memory fits an SM beside this much shared memory: an allocation never waits for a CTA that
+// waits for its predecessor in the stream.)
+#define MXT_SMEM (MXT_RING + 1024 + 1024)
+#define MXT_THREADS 320
+enum { MXT_ERR_WAIT = 121 };
+
+__device__ __forceinline__ int mx_scale_at(int r) { return MX_CODES + (r & 31) * 16 + (r >> 5) * 4; }
+
+// A word of 8 codes as 4 pairs of bfloat16, element 2 i in the low half of w[i]: sign and magnitude of nibbles i and 4 + i where
+// a bfloat16 of exponent 2^-126 has them (the magnitudes 0 and 0.5 are subnormal), times 2^126 times the block's scale, exactly.
+// m1 = 2^(s - 1); where that has no bfloat16 (s > 128) m1 = 2^127 and m2 the rest.
+__device__ __forceinline__ uint32_t mx_mul(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ void mx_pairs(uint32_t q, uint32_t m1, uint32_t* w) {
+    w[0] = mx_mul(((q << 12) & 0x80008000u) | ((q << 6) & 0x01C001C0u), m1);
+    w[1] = mx_mul(((q << 8) & 0x80008000u) | ((q << 2) & 0x01C001C0u), m1);
+    w[2] = mx_mul(((q << 4) & 0x80008000u) | ((q >> 2) & 0x01C001C0u), m1);
+    w[3] = mx_mul((q & 0x80008000u) | ((q >> 6) & 0x01C001C0u), m1);
+}
+__device__ __forceinline__ uint32_t mx_both(uint32_t h) { return h | h << 16; }
+// 16 bytes of codes, one block of a row with scale byte s, as 16 pairs
+__device__ __forceinline__ void mx_block(const uint4 q, int s, uint32_t* w) {
+    const uint32_t m1 = mx_both(s == 255 ? 0x7FC0u : (uint32_t)(min(s, 128) + 126) << 7);
+    mx_pairs(q.x, m1, w);
+    mx_pairs(q.y, m1, w + 4);
+    mx_pairs(q.z, m1, w + 8);
+    mx_pairs(q.w, m1, w + 12);
+    if (s > 128) {
+        const uint32_t m2 = mx_both(s == 255 ? 0x3F80u : (uint32_t)(s - 1) << 7);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = mx_mul(w[i], m2);
+    }
+}
+
+__device__ __forceinline__ void mxt_tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void mxt_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mxt_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// lane 0 waits for its warp
+__device__ __forceinline__ bool mxt_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    uint32_t ok = 1;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag) ? 1u : 0u;
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+__device__ __forceinline__ uint32_t mxt_at_rank(uint32_t saddr, uint32_t rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float4 mxt_ld_cluster(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+// 8 features of one token on their way out
+template <typename TO>
+__device__ __forceinline__ void mxt_store8(TO* dst, const float (&v)[8], int n, bool vec) {
+    TO o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = from_f32<TO>(v[i]);
+    if (vec && n >= 8) {
+#pragma unroll
+        for (int i = 0; i < (int)(8 * sizeof(TO) / 16); ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(o)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) dst[i] = o[i];
+    }
+}
+
+__device__ __forceinline__ void mxt_give_up(volatile int* abort_flag, int* status) {
+    if (!*abort_flag) {
+        *abort_flag = 1;
+        atomicCAS(status, 0, MXT_ERR_WAIT);
+    }
+}
+
+// What both kernels end with, by the whole CTA: the accumulators (valid where `any`, else zero) as float sums [token][2 x 128
+// rows] in shared memory, where the ring was (every copy has been read by an MMA that is done), and this CTA's share of the tokens from all of the cluster's.
+// `ok`: of warps 0-7, whether the accumulators may be waited for.  Leaves with the cluster's sums no longer needed.
+template <typename TO, bool GATED>
+__device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, uint64_t* acc_bar, volatile int* abort_flag, int* status, bool ok,
+                                           bool any, int rows, int ranks, int rank, TO* __restrict__ out, long ldo, int f0, int n,
+                                           const FlGate act) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp < 8) {
+        if (ok && !mxt_wait(acc_bar, 0, abort_flag)) {
+            if (lane == 0) mxt_give_up(abort_flag, status);
+            ok = false;
+        }
+        if (ok) {
+            tc_fence_after();
+            const int tile = warp >> 2, f = tile * 128 + (threadIdx.x & 127);
+            const uint32_t src = tmem_d + (uint32_t)(tile * 128) + ((uint32_t)((warp & 3) * 32) << 16);
+            for (int c = 0; c < rows; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(src + (uint32_t)c, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sums[(c + j) * MXT_PITCH + f] = any ? __uint_as_float(v[j]) : 0.0f;
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    if (ranks > 1) cluster_sync_all();
+    else __syncthreads();
+    tc_fence_after();
+    // (a CTA of the cluster that gave up leaves its sums as they are: the status word tells that the results are not valid)
+    if (warp < 8 && !*abort_flag) {
+        const int share = (rows + ranks - 1) / ranks, first = rank * share, last = min(rows, first + share);
+        constexpr int PER = (GATED ? 128 : 256) / 8;                  // threads of a token
+        const int f = (threadIdx.x % PER) * 8;
+        const bool vec = (((uintptr_t)out | (uintptr_t)(ldo * (long)sizeof(TO))) & 15) == 0;
+        for (int t = first + threadIdx.x / PER; t < last && f0 + f < n; t += 256 / PER) {
+            float g[8] = {}, u[8] = {};
+            for (int q = 0; q < ranks; ++q) {
+                const uint32_t at = smem_u32(sums + t * MXT_PITCH + f);
+                const uint32_t a = ranks > 1 ? mxt_at_rank(at, (uint32_t)q) : at;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float4 v = mxt_ld_cluster(a + (uint32_t)(h * 16));
+                    g[4 * h] += v.x, g[4 * h + 1] += v.y, g[4 * h + 2] += v.z, g[4 * h + 3] += v.w;
+                    if (GATED) {
+                        const float4 x = mxt_ld_cluster(a + 512u + (uint32_t)(h * 16));
+                        u[4 * h] += x.x, u[4 * h + 1] += x.y, u[4 * h + 2] += x.z, u[4 * h + 3] += x.w;
+                    }
+                }
+            }
+            if (act.act != FL_ACT_NONE) {
+                if (!GATED)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) u[i] = 1.0f;
+                gated_act(g, u, act);
+            }
+            mxt_store8(out + (long)t * ldo + f0 + f, g, n - f0 - f, vec);
+        }
+    }
+    __syncwarp();
+    if (ranks > 1) cluster_sync_all();                                // the others may still read this CTA's sums
+    else __syncthreads();
+}
+
+// grid: ranks of a cluster x token tiles x row tiles (pairs of them).  bn: tokens of a tile, a multiple of 16.  stages: of
+// bn x 64 elements in the ring.
+template <typename TO, bool GATED>
+__global__ void __launch_bounds__(MXT_THREADS, 1)
+mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ w, TO* __restrict__ out, long ldo, int m, int n,
+           int k, int bn, int stages, int ranks, int per_rank, FlGate act, int* __restrict__ status) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* ring = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* full_bar = (uint64_t*)(ring + MXT_RING);
+    uint64_t* empty_bar = full_bar + MXT_MAX_STAGES;
+    uint64_t* a_full = empty_bar + MXT_MAX_STAGES;
+    uint64_t* a_empty = a_full + MXT_A;
+    uint64_t* acc_bar = a_empty + MXT_A;
+    uint32_t* tmem_slot = (uint32_t*)(acc_bar + 1);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x;
+    const int t0 = blockIdx.y * bn;
+    const int f0 = blockIdx.z * (GATED ? 128 : 256);
+    const int chunks = (k + 127) / 128;
+    const int c_begin = rank * per_rank, c_end = min(chunks, c_begin + per_rank);
+    const int blocks = 2 * max(0, c_end - c_begin);              // of 64 elements along K
+    const int stage_bytes = bn * 128;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+        }
+        for (int s = 0; s < MXT_A; ++s) {
+            mbar_init(&a_full[s], 8);
+            mbar_init(&a_empty[s], 1);
+        }
+        mbar_init(acc_bar, 1);
+        *abort_flag = (*(volatile int*)status != 0) ? 1 : 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 9) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_d = *tmem_slot, tmem_a = tmem_d + 256;   // accumulators of 128 columns each, then the ring of A
+    auto give_up = [&]() { mxt_give_up(abort_flag, status); };
+    pdl_trigger();
+    pdl_wait();
+    int issued = 0;
+    bool ok = !*abort_flag;
+    if (warp < 8) {
+        // ---- a thread's row of W: codes two chunks ahead in registers, 64 elements a time to tensor memory
+        const int tile = warp >> 2;
+        const long row = (GATED ? (long)tile * n : (long)tile * 128) + f0 + (threadIdx.x & 127);
+        const bool real = GATED ? f0 + (threadIdx.x & 127) < n : row < n;
+        const int r = (int)(row & (MX_ROWS - 1));
+        const uint8_t* src = w + row / MX_ROWS * chunks * (long)MX_CHUNK;
+        const uint32_t dst = tmem_a + (uint32_t)(tile * 32) + ((uint32_t)((warp & 3) * 32) << 16);
+        uint4 q[2][4];
+        uint32_t sc[2];
+        auto fetch = [&](int buf, int c) {
+            const uint8_t* p = src + (long)c * MX_CHUNK;
+            const bool there = real && c < c_end;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) q[buf][b] = there ? __ldg(reinterpret_cast<const uint4*>(p + b * 2048 + r * 16)) : make_uint4(0, 0, 0, 0);
+            sc[buf] = there ? __ldg(reinterpret_cast<const uint32_t*>(p + mx_scale_at(r))) : 0;
+        };
+        fetch(0, c_begin);
+        fetch(1, c_begin + 1);
+        int sa = 0;
+        uint32_t pa = 0;
+        auto convert = [&](int buf, int c) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (!ok) return;
+                uint32_t v[32];
+                mx_block(q[buf][2 * h], (int)(sc[buf] >> (16 * h)) & 255, v);
+                mx_block(q[buf][2 * h + 1], (int)(sc[buf] >> (16 * h + 8)) & 255, v + 16);
+                if (!mxt_wait(&a_empty[sa], pa ^ 1u, abort_flag)) {
+                    if (lane == 0) give_up();
+                    ok = false;
+                    return;
+                }
+                tc_fence_after();
+                mxt_tmem_st16(dst + (uint32_t)(sa * 64), v);
+                mxt_tmem_st16(dst + (uint32_t)(sa * 64 + 16), v + 16);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mxt_arrive(&a_full[sa]);
+                if (++sa == MXT_A) { sa = 0; pa ^= 1u; }
+            }
+            fetch(buf, c + 2);
+        };
+        for (int c = c_begin; c < c_end && ok; c += 2) {
+            convert(0, c);
+            if (c + 1 < c_end && ok) convert(1, c + 1);
+        }
+    } else if (warp == 8) {
+        if (lane == 0) {
+            // ---- producer of the tokens' tiles
+            int s = 0;
+            uint32_t ph = 0;
+            for (int i = 0; i < blocks && ok; ++i) {
+                if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag)) {
+                    give_up();
+                    break;
+                }
+                mbar_expect_tx(&full_bar[s], (uint32_t)stage_bytes);
+                tma_load_2d(ring + s * stage_bytes, &map_x, &full_bar[s], (2 * c_begin + i) * 64, t0);
+                ++issued;
+                if (++s == stages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (lane == 0) {
+        // ---- MMA issuer
+        const uint32_t idesc = instr_desc_bf16(128, bn);
+        int s = 0, sa = 0;
+        uint32_t ph = 0, pa = 0;
+        for (int i = 0; i < blocks && ok; ++i) {
+            if (!mbar_wait(&full_bar[s], ph, abort_flag) || !mbar_wait(&a_full[sa], pa, abort_flag)) {
+                give_up();
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint64_t bdesc = smem_desc_sw128(smem_u32(ring + s * stage_bytes));
+#pragma unroll
+            for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                    mxt_umma_ts(tmem_d + (uint32_t)(tile * 128), tmem_a + (uint32_t)(sa * 64 + tile * 32 + kk * 8), bdesc + (uint64_t)(2 * kk),
+                                idesc, (i > 0 || kk > 0) ? 1u : 0u);
+            umma_commit(&empty_bar[s]);
+            umma_commit(&a_empty[sa]);
+            if (++s == stages) { s = 0; ph ^= 1u; }
+            if (++sa == MXT_A) { sa = 0; pa ^= 1u; }
+        }
+        if (ok) umma_commit(acc_bar);
+    }
+    mxt_finish<TO, GATED>(reinterpret_cast<float*>(ring), tmem_d, acc_bar, abort_flag, status, ok, blocks > 0, min(bn, m - t0), ranks, rank,
+                          out + (long)t0 * ldo, ldo, f0, n, act);
+    if (warp == 8 && lane == 0 && *abort_flag) tma_drain(full_bar, stages, issued);
+    __syncthreads();
+    if (warp == 9) tmem_dealloc(tmem_d, 512);
+}
+
+// A cluster of CTAs along the grid's x.
+template <typename... KArgs, typename... Args>
+static int mxt_launch_cluster(void (*kernel)(KArgs...), bool& configured, int smem, dim3 grid, cudaStream_t stream, Args... args) {
+    if (!configured) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return (int)e;
+        configured = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(MXT_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = grid.x;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = fl_pdl_enabled() ? 2 : 1;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+// CTAs of a cluster that share K: as many as there are SMs for, and chunks
+static int mxt_ranks(long tiles, int chunks, int num_sms) {
+    int ranks = 1;
+    while (ranks < 8 && tiles * ranks * 2 <= num_sms && ranks * 2 <= chunks) ranks *= 2;
+    return ranks;
+}
+
+template <typename TO, bool GATED>
+static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ldo, int m, int n, int k, FlGate act, int num_sms,
+                      int* status, cudaStream_t stream) {
+    const int token_tiles = (m + MXT_BN - 1) / MXT_BN;
+    const int bn = ((m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
+    const int row_tiles = (n + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
+    const int tokens_y = (m + bn - 1) / bn;
+    if (tokens_y > 65535 || row_tiles > 65535) return -1;
+    const int chunks = (k + 127) / 128;
+    const int ranks = mxt_ranks((long)tokens_y * row_tiles, chunks, num_sms);
+    const int per_rank = (chunks + ranks - 1) / ranks;
+    int stages = MXT_RING / (bn * 128);
+    if (stages > MXT_MAX_STAGES) stages = MXT_MAX_STAGES;
+    CUtensorMap map;
+    int rc = make_map(&map, x, m, k, ldx, bn);
+    if (rc) return rc;
+    static bool configured = false;
+    return mxt_launch_cluster(mxt_kernel<TO, GATED>, configured, MXT_SMEM, dim3(ranks, tokens_y, row_tiles), stream, map, (const uint8_t*)w,
+                              (TO*)out, ldo, m, n, k, bn, stages, ranks, per_rank, act, status);
+}
+
+// x: bfloat16 rows, 16-byte aligned, `ldx` elements apart (a multiple of 8).  n: output features (gated: half of w's rows).
+// -1: not for this kernel.
+FL_API int fl_mxt_product(const void* x, long ldx, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int gated,
+                          int act, float p0, float p1, int num_sms, int* status, cudaStream_t stream) {
+    const FlGate gate = {act, p0, p1};
+    FL_DISPATCH(out_code, TO, {
+        return gated ? mxt_launch<TO, true>(x, ldx, w, out, ldo, m, n, k, gate, num_sms, status, stream)
+                     : mxt_launch<TO, false>(x, ldx, w, out, ldo, m, n, k, gate, num_sms, status, stream);
+    })
+    return (int)cudaErrorInvalidValue;
+}
+
+// ---------------------------------------------------------------- both operands in 4 bits
+// out[t, f] = sum_k A[t, k] W[f, k] on the block-scaled matrix instruction: codes in shared memory as they lie in the packed form (a
+// row's 16 bytes of a block are a line of an 8 x 16-byte core matrix; core matrices 128 bytes apart along the rows, 2048 along
+// K), the scales copied from there to tensor memory, 4 columns for 128 rows x 4 blocks.  A stage is a chunk of 128 along K of two
+// tiles of W's rows and of one of A's: three copies.
+#define MXQ_STAGE (3 * MX_CHUNK)
+#define MXQ_STAGES 8
+#define MXQ_SF 12                                              // columns of a stage's scales
+#define MXQ_SMEM (MXQ_STAGES * MXQ_STAGE + 1024)
+
+__device__ __forceinline__ void mxq_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+                 "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+// no swizzle: `lead` bytes between core matrices along K, 128 between those of neighbouring groups of 8 rows
+__device__ __forceinline__ uint64_t mxq_desc(uint32_t saddr, uint32_t lead) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+__device__ __forceinline__ void mxq_copy_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// float accumulator; A and B e2m1 with a scale 2^(s - 127) for 32 elements, which of the four bytes of a scale column `id` (0 or 2) and
+// the next one are
+__device__ __forceinline__ uint32_t mxq_idesc(int n, int id) {
+    return (uint32_t)id << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | 1u << 23 | (uint32_t)(128 >> 4) << 24 | (uint32_t)id << 29;
+}
+__device__ __forceinline__ void mxq_umma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+
+template <typename TO>
+__global__ void __launch_bounds__(MXT_THREADS, 1)
+mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __restrict__ out, long ldo, int m, int n, int chunks,
+           int ranks, int per_rank, int* __restrict__ status) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* ring = (unsigned char*)(((uintptr_t)smem_raw + 127) & ~(uintptr_t)127);
+    uint64_t* full_bar = (uint64_t*)(ring + MXQ_STAGES * MXQ_STAGE);
+    uint64_t* empty_bar = full_bar + MXQ_STAGES;
+    uint64_t* acc_bar = empty_bar + MXQ_STAGES;
+    uint32_t* tmem_slot = (uint32_t*)(acc_bar + 1);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x;
+    const int t0 = blockIdx.y * 128, f0 = blockIdx.z * 256;
+    const int rows = min(128, m - t0), tiles = n - f0 > 128 ? 2 : 1;
+    const int c_begin = rank * per_rank, c_end = min(chunks, c_begin + per_rank);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < MXQ_STAGES; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+        }
+        mbar_init(acc_bar, 1);
+        *abort_flag = (*(volatile int*)status != 0) ? 1 : 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 9) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_d = *tmem_slot, tmem_sf = tmem_d + 256;
+    pdl_trigger();
+    pdl_wait();
+    int issued = 0;
+    const bool ok = !*abort_flag;
+    if (warp == 8) {
+        if (lane == 0) {
+            const uint8_t* src_a = a + (long)blockIdx.y * chunks * MX_CHUNK;
+            const uint8_t* src_w = w + (long)blockIdx.z * 2 * chunks * MX_CHUNK;
+            int s = 0;
+            uint32_t ph = 0;
+            for (int c = c_begin; c < c_end && ok; ++c) {
+                if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag)) {
+                    mxt_give_up(abort_flag, status);
+                    break;
+                }
+                unsigned char* dst = ring + s * MXQ_STAGE;
+                mbar_expect_tx(&full_bar[s], (uint32_t)((tiles + 1) * MX_CHUNK));
+                mxq_copy(dst, src_a + (long)c * MX_CHUNK, MX_CHUNK, &full_bar[s]);
+                for (int t = 0; t < tiles; ++t)
+                    mxq_copy(dst + (1 + t) * MX_CHUNK, src_w + ((long)t * chunks + c) * MX_CHUNK, MX_CHUNK, &full_bar[s]);
+                ++issued;
+                if (++s == MXQ_STAGES) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 9) {
+        if (lane == 0) {
+            const int bn = (rows + 15) / 16 * 16;
+            const uint32_t idesc[2] = {mxq_idesc(bn, 0), mxq_idesc(bn, 2)};
+            int s = 0;
+            uint32_t ph = 0;
+            bool going = ok;
+            for (int c = c_begin; c < c_end && going; ++c) {
+                if (!mbar_wait(&full_bar[s], ph, abort_flag)) {
+                    mxt_give_up(abort_flag, status);
+                    going = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t at = smem_u32(ring + s * MXQ_STAGE), sf = tmem_sf + (uint32_t)(s * MXQ_SF);
+                // (the stage's columns: its last use's MMAs were done before its copies were sent for)
+                for (int t = 0; t <= tiles; ++t)
+                    mxq_copy_scales(sf + (uint32_t)(4 * t), mxq_desc(at + (uint32_t)(t * MX_CHUNK + MX_CODES), 128));
+                for (int t = 0; t < tiles; ++t)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        mxq_umma(tmem_d + (uint32_t)(t * 128), mxq_desc(at + (uint32_t)((1 + t) * MX_CHUNK + h * 4096), 2048),
+                                 mxq_desc(at + (uint32_t)(h * 4096), 2048), idesc[h], sf + (uint32_t)(4 + 4 * t), sf,
+                                 (c > c_begin || h > 0) ? 1u : 0u);
+                umma_commit(&empty_bar[s]);
+                if (++s == MXQ_STAGES) { s = 0; ph ^= 1u; }
+            }
+            if (going) umma_commit(acc_bar);
+        }
+    }
+    mxt_finish<TO, false>(reinterpret_cast<float*>(ring), tmem_d, acc_bar, abort_flag, status, ok, c_end > c_begin, rows, ranks, rank,
+                          out + (long)t0 * ldo, ldo, f0, n, FlGate{FL_ACT_NONE, 0.0f, 0.0f});
+    if (warp == 8 && lane == 0 && *abort_flag) tma_drain(full_bar, MXQ_STAGES, issued);
+    __syncthreads();
+    if (warp == 9) tmem_dealloc(tmem_d, 512);
+}
+
+// a [m, k] and w [n, k] packed.  -1: not for this kernel.
+FL_API int fl_mxq_product(const void* a, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int num_sms, int* status,
+                          cudaStream_t stream) {
+    const int chunks = (k + 127) / 128, token_tiles = (m + 127) / 128, row_tiles = (n + 255) / 256;
+    if (token_tiles > 65535 || row_tiles > 65535) return -1;
+    const int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, num_sms), per_rank = (chunks + ranks - 1) / ranks;
+    FL_DISPATCH(out_code, TO, {
+        static bool configured = false;
+        return mxt_launch_cluster(mxq_kernel<TO>, configured, MXQ_SMEM, dim3(ranks, token_tiles, row_tiles), stream, (const uint8_t*)a,
+                                  (const uint8_t*)w, (TO*)out, ldo, m, n, chunks, ranks, per_rank, status);
+    })
+    return (int)cudaErrorInvalidValue;
+}

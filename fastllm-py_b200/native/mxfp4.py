@@ -122,6 +122,23 @@ def _product(name, x, x_ptr, ldx, m, k, w: Matrix, out, gated, activation, param
                                             c_float, c_float, c_void_p])
     if m == 0:
         return
+    if ldx:
+        fn = ops._fn("mxfp4_tc", "fl_mxt_product", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int,
+                                                    c_float, c_float, c_int, c_void_p, c_void_p])
+        from . import gemm_tc
+        rc = fn(x_ptr, ldx, w.data.data_ptr(), out.data_ptr(), code, ldo, m, n, k, int(gated), act, params[0], params[1],
+                ops.sm_count(out.device), gemm_tc.status_word(out.device).data_ptr(), stream)
+        if rc != -1:
+            ops._check(rc, f"mxfp4.{name}")
+            return
+    else:
+        fn2 = ops._fn("mxfp4_tc", "fl_mxq_product", [c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_void_p, c_void_p])
+        from . import gemm_tc
+        rc = fn2(x_ptr, w.data.data_ptr(), out.data_ptr(), code, ldo, m, n, k, ops.sm_count(out.device),
+                 gemm_tc.status_word(out.device).data_ptr(), stream)
+        if rc != -1:
+            ops._check(rc, f"mxfp4.{name}")
+            return
     ops._check(fn(x_ptr, ldx, w.data.data_ptr(), out.data_ptr(), code, ldo, m, n, k, int(gated), act,
                   float(params[0]), float(params[1]), stream), f"mxfp4.{name}")
 
