@@ -162,82 +162,172 @@ FL_API int fl_mx_dequantize(const void* data, void* out, int code, long ld, int 
     return (int)cudaErrorInvalidValue;
 }
 
-// ---------------------------------------------------------------- products
-// out[t, f] = sum_k x[t, k] W[f, k], or of a gated unit act(gate, up) of features f and n + f.  A warp sums one feature for 8
-// tokens: 16 lanes share a chunk, 8 elements each.  x comes in bfloat16 or packed as W is.
-template <typename TO, bool PACKED, bool GATED>
-__global__ void __launch_bounds__(256) mx_product_kernel(const void* __restrict__ x, long ldx, const uint8_t* __restrict__ w,
-                                                         TO* __restrict__ out, long ldo, int m, int n, int k, FlGate act) {
-    pdl_wait();
+// ---------------------------------------------------------------- products of few rows
+// out[t, f] = sum_k x[t, k] W[f, k] for up to 16 tokens, or of a gated unit act(gate, up) of features f and n + f: reading W
+// is the time.  A warp takes 16 (MT = 2: 2 x 16) rows of W and every WARPS-th chunk of K; the rows are the 16 of m16n8k16 and the
+// tokens its 8 columns.  Lane 4 g + q reads the 16 bytes of rows g and g + 8 of block q, so a lane has one scale for 32 codes;
+// which elements of K meet in one instruction does not matter as long as both operands agree, and a lane's 8 consecutive elements
+// of a token are the partners of one word of codes.  The warps' sums meet in shared memory and are added in order.
+__device__ __forceinline__ uint32_t mx_mul(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// A word of 8 codes as 4 pairs of bfloat16, element 2 i in the low half of w[i]: sign and magnitude of nibbles i and 4 + i where
+// a bfloat16 of exponent 2^-126 has them (the magnitudes 0 and 0.5 are subnormal), times m1.  A product with two powers of two puts
+// a nibble in both places at once.
+__device__ __forceinline__ void mx_pairs(uint32_t q, uint32_t m1, uint32_t* w) {
+    constexpr uint32_t PLACES = 0x81C081C0u, NIBBLE = 0x000F000Fu;
+    w[0] = mx_mul(((q & NIBBLE) * 0x1040u) & PLACES, m1);
+    w[1] = mx_mul(((q & (NIBBLE << 4)) * 0x104u) & PLACES, m1);
+    w[2] = mx_mul((((q >> 8) & NIBBLE) * 0x1040u) & PLACES, m1);
+    w[3] = mx_mul((q & 0x80008000u) | ((q >> 6) & 0x01C001C0u), m1);
+}
+__device__ __forceinline__ uint32_t mx_both(uint32_t h) { return h | h << 16; }
+__device__ __forceinline__ void mx_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 8 elements of a token from element c on, zeros behind k
+__device__ __forceinline__ uint4 mx_tokens8(const bf16* row, int c, int k) {
+    if (c + 8 <= k) return *reinterpret_cast<const uint4*>(row + c);
+    uint32_t v[4] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (c + i < k) v[i >> 1] |= (uint32_t)__bfloat16_as_ushort(row[c + i]) << (16 * (i & 1));
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+#define MXF_WARPS 8
+template <typename TO, int MT, int NT, bool GATED>
+__global__ void __launch_bounds__(MXF_WARPS * 32) mx_few_kernel(const bf16* __restrict__ x, long ldx, const uint8_t* __restrict__ w,
+                                                                TO* __restrict__ out, long ldo, int m, int n, int k, bool constant_w,
+                                                                FlGate act) {
+    static_assert(!GATED || MT == 2, "a gated unit's two rows are a warp's two tiles");
+    constexpr int ROWS = GATED ? 16 : 16 * MT;                       // output features of a block
+    __shared__ float red[MXF_WARPS][NT * 8][MT * 16 + 1];
     pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int chunks = (k + 127) / 128;
-    const int lane = threadIdx.x & 31;
-    const int groups = (n + 7) / 8;
-    const int f = blockIdx.x % groups * 8 + (threadIdx.x >> 5);
-    const int t0 = blockIdx.x / groups * 8;
-    if (f >= n) return;                                               // (whole warps)
-    float acc[GATED ? 2 : 1][8] = {};
-    for (int chunk = lane >> 4; chunk < chunks; chunk += 2) {
-        const int b = (lane >> 2) & 3, word = lane & 3;
-        float v[GATED ? 2 : 1][8];
+    const int f0 = blockIdx.x * ROWS;
+    const uint8_t* src[MT][2];                                       // codes of block q of a row, of chunk 0
+    int sc_at[MT][2];                                                // from there to the block's scale
+    bool real[MT][2];
 #pragma unroll
-        for (int g = 0; g < (GATED ? 2 : 1); ++g) {
-            const long row = (long)g * n + f;
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int f = f0 + (GATED ? 0 : 16 * t) + 8 * h + g;
+            const long row = (GATED ? (long)t * n : 0) + f;
             const int r = (int)(row & (MX_ROWS - 1));
-            const uint8_t* src = w + (row / MX_ROWS * chunks + chunk) * MX_CHUNK;
-            const uint32_t codes = *reinterpret_cast<const uint32_t*>(src + b * 2048 + r * 16 + word * 4);
-            const float scale = mx_scale(src[mx_scale_at(r) + b]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[g][i] = mx_value(codes, i) * scale;
+            src[t][h] = w + row / MX_ROWS * chunks * (long)MX_CHUNK + q * 2048 + r * 16;
+            sc_at[t][h] = (int)mx_scale_at(r) + q - (q * 2048 + r * 16);
+            real[t][h] = f < n;
         }
-        const int c = chunk * 128 + b * 32 + word * 8;
+    uint4 codes[MT][2];
+    uint32_t scale[MT][2];
+    auto fetch = [&](int c) {
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            if (t0 + t >= m) break;
-            float a[8];
-            if (PACKED) {
-                const int r = (t0 + t) & (MX_ROWS - 1);
-                const uint8_t* src = (const uint8_t*)x + ((long)((t0 + t) / MX_ROWS) * chunks + chunk) * MX_CHUNK;
-                const uint32_t codes = *reinterpret_cast<const uint32_t*>(src + b * 2048 + r * 16 + word * 4);
-                const float scale = mx_scale(src[mx_scale_at(r) + b]);
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) a[i] = mx_value(codes, i) * scale;
-            } else {
-                mx_load8((const bf16*)x + (long)(t0 + t) * ldx + c, k - c, true, a);
+            for (int h = 0; h < 2; ++h) {
+                const uint8_t* p = src[t][h] + (long)c * MX_CHUNK;
+                const bool there = real[t][h] && c < chunks;
+                codes[t][h] = there ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+                scale[t][h] = there ? p[sc_at[t][h]] : 0;
             }
+    };
+    if (!constant_w) pdl_wait();
+    fetch(warp);
+    if (constant_w) pdl_wait();
+    float acc[MT][NT][4] = {};
+    for (int c = warp; c < chunks; c += MXF_WARPS) {
+        uint4 now[MT][2];
+        uint32_t m1[MT][2], m2[MT][2];
+        bool large = false;
 #pragma unroll
-            for (int g = 0; g < (GATED ? 2 : 1); ++g)
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (c + i < k) acc[g][t] = fmaf(a[i], v[g][i], acc[g][t]);
+            for (int h = 0; h < 2; ++h) {
+                now[t][h] = codes[t][h];
+                const uint32_t s = scale[t][h];
+                m1[t][h] = mx_both(s == 255 ? 0x7FC0u : (min(s, 128u) + 126u) << 7);
+                m2[t][h] = mx_both(s == 255 || s <= 128 ? 0x3F80u : (s - 1) << 7);       // (what 2^(s - 1) has beyond 2^127)
+                large |= s > 128;
+            }
+        uint4 xs[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int token = j * 8 + g;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                xs[j][i] = token < m ? mx_tokens8(x + (long)token * ldx, c * 128 + q * 32 + i * 8, k) : make_uint4(0, 0, 0, 0);
         }
+        fetch(c + MXF_WARPS);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                uint32_t v[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint4 z = now[t][h];
+                    mx_pairs(i == 0 ? z.x : i == 1 ? z.y : i == 2 ? z.z : z.w, m1[t][h], v[h]);
+                    if (large)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[h][e] = mx_mul(v[h][e], m2[t][h]);
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    mx_mma(acc[t][j], v[0][0], v[1][0], v[0][1], v[1][1], xs[j][i].x, xs[j][i].y);
+                    mx_mma(acc[t][j], v[0][2], v[1][2], v[0][3], v[1][3], xs[j][i].z, xs[j][i].w);
+                }
+            }
     }
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-        const float g = warp_sum(acc[0][t]);
-        const float u = GATED ? warp_sum(acc[GATED ? 1 : 0][t]) : 1.0f;
-        if (lane == 0 && t0 + t < m) out[(long)(t0 + t) * ldo + f] = from_f32<TO>(act.act == FL_ACT_NONE ? g : fl_gated(g, u, act));
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) red[warp][j * 8 + 2 * q + (e & 1)][t * 16 + g + 8 * (e >> 1)] = acc[t][j][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < ROWS * m; i += MXF_WARPS * 32) {
+        const int t = i / ROWS, f = i % ROWS;
+        if (f0 + f >= n) continue;
+        float v = 0.0f, u = 1.0f;
+#pragma unroll
+        for (int s = 0; s < MXF_WARPS; ++s) v += red[s][t][f];
+        if (GATED) {
+            u = 0.0f;
+#pragma unroll
+            for (int s = 0; s < MXF_WARPS; ++s) u += red[s][t][(MT - 1) * 16 + f];
+        }
+        out[(long)t * ldo + f0 + f] = from_f32<TO>(act.act == FL_ACT_NONE ? v : fl_gated(v, u, act));
     }
 }
 
-template <typename TO, bool PACKED, bool GATED>
-static int mx_launch_product(const void* x, long ldx, const void* w, void* out, long ldo, int m, int n, int k, FlGate act,
-                             cudaStream_t stream) {
-    const long blocks = (long)((n + 7) / 8) * ((m + 7) / 8);
-    if (blocks > 0x7FFFFFFFl) return (int)cudaErrorInvalidValue;
-    return fl_launch(mx_product_kernel<TO, PACKED, GATED>, dim3((unsigned)blocks), dim3(256), 0, stream, x, ldx,
-                     (const uint8_t*)w, (TO*)out, ldo, m, n, k, act);
+template <typename TO, int NT>
+static int mx_launch_few(const bf16* x, long ldx, const uint8_t* w, TO* out, long ldo, int m, int n, int k, bool gated, bool constant_w,
+                         FlGate act, cudaStream_t stream) {
+    const dim3 block(MXF_WARPS * 32);
+    if (gated)
+        return fl_launch(mx_few_kernel<TO, 2, NT, true>, dim3((n + 15) / 16), block, 0, stream, x, ldx, w, out, ldo, m, n, k, constant_w, act);
+    if (n >= 8192)
+        return fl_launch(mx_few_kernel<TO, 2, NT, false>, dim3((n + 31) / 32), block, 0, stream, x, ldx, w, out, ldo, m, n, k, constant_w, act);
+    return fl_launch(mx_few_kernel<TO, 1, NT, false>, dim3((n + 15) / 16), block, 0, stream, x, ldx, w, out, ldo, m, n, k, constant_w, act);
 }
 
-// x: bfloat16 rows with `ldx` elements between them (a multiple of 8, from 16 bytes on), or, ldx 0, packed.  n: output features
-// (gated: half of w's rows).  act: an FlAct or FL_ACT_NONE; a product that is not gated has f(v, 1).
-FL_API int fl_mx_product(const void* x, long ldx, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int gated,
-                         int act, float p0, float p1, cudaStream_t stream) {
+// x: up to 16 bfloat16 rows with `ldx` elements between them (a multiple of 8, from 16 bytes on).  n: output features (gated: half
+// of w's rows).  act: an FlAct or FL_ACT_NONE; a product that is not gated has f(v, 1).  constant_w: no kernel before this one
+// in the stream writes w, so its first bytes may be read while that one still runs.
+FL_API int fl_mx_few(const void* x, long ldx, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int gated,
+                     int act, float p0, float p1, int constant_w, cudaStream_t stream) {
     const FlGate gate = {act, p0, p1};
+    if (m > 16) return (int)cudaErrorInvalidValue;
     FL_DISPATCH(out_code, TO, {
-        if (gated) return mx_launch_product<TO, false, true>(x, ldx, w, out, ldo, m, n, k, gate, stream);
-        if (ldx == 0) return mx_launch_product<TO, true, false>(x, ldx, w, out, ldo, m, n, k, gate, stream);
-        return mx_launch_product<TO, false, false>(x, ldx, w, out, ldo, m, n, k, gate, stream);
+        if (m <= 8) return mx_launch_few<TO, 1>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, gated != 0, constant_w != 0, gate, stream);
+        return mx_launch_few<TO, 2>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, gated != 0, constant_w != 0, gate, stream);
     })
     return (int)cudaErrorInvalidValue;
 }

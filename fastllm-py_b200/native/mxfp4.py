@@ -25,14 +25,14 @@ from . import ops
 from .ops import KernelError
 
 ROWS, CHUNK_K, CHUNK_BYTES = 128, 128, 8704      # a tile's rows, a chunk's elements along K and its bytes (csrc/mxfp4.cu)
-LIBRARIES = ["mxfp4"]
+LIBRARIES = ["mxfp4", "mxfp4_tc", "gemm_tcgen05"]
 
 
 class Matrix:
     """A matrix [rows, k] in the packed form: uint8 [ceil(rows / 128), ceil(k / 128), 8704] (csrc/mxfp4.cu says how a chunk
     lies).  Codes behind k are zero; rows behind the last are not read for any result."""
 
-    __slots__ = ("data", "rows", "k")
+    __slots__ = ("data", "rows", "k", "shape")
 
     def __init__(self, data: torch.Tensor, rows: int, k: int):
         if rows < 1 or k < 1:
@@ -42,7 +42,7 @@ class Matrix:
                               f"{(-(-rows // ROWS), -(-k // CHUNK_K), CHUNK_BYTES)}, got {data.dtype} {tuple(data.shape)}")
         if data.data_ptr() % 16:
             raise KernelError("mxfp4: a packed matrix begins on 16 bytes")
-        self.data, self.rows, self.k = data, rows, k
+        self.data, self.rows, self.k, self.shape = data, rows, k, (rows, k)
 
     @classmethod
     def empty(cls, rows: int, k: int, device) -> "Matrix":
@@ -56,25 +56,23 @@ class Matrix:
         return q
 
     @property
-    def shape(self):
-        return (self.rows, self.k)
-
-    @property
     def device(self):
         return self.data.device
 
 
-def _launch_stream(*tensors) -> int:
-    """The current stream of the device that all tensors are on, which has to be the current one."""
-    device = tensors[0].device
-    if device.type != "cuda":
+_device = torch._C._cuda_getDevice               # the current device's index
+
+
+def _stream_of(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor) -> int:
+    """The current stream of the device that all three are on, which has to be the current one."""
+    index = a.get_device()
+    if index < 0 or b.get_device() != index or c.get_device() != index:
+        if all(t.is_cuda for t in (a, b, c)):
+            raise KernelError(f"mxfp4: operands on {a.device}, {b.device} and {c.device}")
         raise KernelError("the engine's kernels run on a CUDA device only; got a CPU tensor")
-    for t in tensors[1:]:
-        if t.device != device:
-            raise KernelError(f"mxfp4: operands on {device} and {t.device}")
-    if device.index != torch.cuda.current_device():
-        raise KernelError(f"mxfp4: operands on {device}, the current device is cuda:{torch.cuda.current_device()}")
-    return ops._raw_stream(device.index)
+    if index != _device():
+        raise KernelError(f"mxfp4: operands on {a.device}, the current device is cuda:{_device()}")
+    return ops._raw_stream(index)
 
 
 def _rows_of(t: torch.Tensor, what: str) -> int:
@@ -82,92 +80,120 @@ def _rows_of(t: torch.Tensor, what: str) -> int:
     if t.dim() != 2:
         raise KernelError(f"mxfp4: {what} is a matrix, got shape {tuple(t.shape)}")
     rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    pitch, step = t.stride()
+    if step != 1 and cols > 1:
         raise KernelError(f"mxfp4: the rows of {what} must be contiguous")
-    if rows > 1 and t.stride(0) < cols:
-        raise KernelError(f"mxfp4: the rows of {what} overlap")
-    return t.stride(0) if rows > 1 else max(t.stride(0), cols)
+    if pitch < cols:
+        if rows > 1:
+            raise KernelError(f"mxfp4: the rows of {what} overlap")
+        return cols
+    return pitch
+
+
+def _activations(x: torch.Tensor) -> int:
+    pitch = _rows_of(x, "x")
+    if x.dtype is not torch.bfloat16:
+        raise KernelError(f"mxfp4: activations are bfloat16, got {x.dtype}")
+    if x.shape[0] == 1:
+        pitch = -(-pitch // 8) * 8                               # (a single row has no pitch)
+    if pitch % 8 or x.data_ptr() % 16:
+        raise KernelError("mxfp4: activations must be 16-byte aligned with a row pitch that is a multiple of 8 elements")
+    return pitch
+
+
+_fns: dict = {}                                  # launchers, and status words by device: looked up once
+_QUANTIZE = ("mxfp4", "fl_mx_quantize", [c_void_p, c_int, c_long, c_void_p, c_int, c_int, c_void_p])
+_DEQUANTIZE = ("mxfp4", "fl_mx_dequantize", [c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_void_p])
+_FEW = ("mxfp4", "fl_mx_few", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_float, c_float,
+                               c_int, c_void_p])
+_MANY = ("mxfp4_tc", "fl_mxt_product", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_float,
+                                        c_float, c_int, c_void_p, c_void_p])
+_BOTH = ("mxfp4_tc", "fl_mxq_product", [c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_void_p, c_void_p])
+
+
+def _fn(which):
+    fn = _fns.get(which[1])
+    if fn is None:
+        fn = _fns[which[1]] = ops._fn(*which)
+    return fn
+
+
+def _status(t: torch.Tensor):
+    """(address of the device's status word, its number of SMs)."""
+    found = _fns.get(t.get_device())
+    if found is None:
+        from . import gemm_tc
+        found = _fns[t.get_device()] = (gemm_tc.status_word(t.device).data_ptr(), ops.sm_count(t.device))
+    return found
 
 
 def quantize(x: torch.Tensor, out: Matrix) -> None:
     """out = x [rows, k] (float32 or bfloat16) rounded to nearest, ties to even codes; a block's scale is the power of two that
     puts its largest magnitude into [4, 8) (the codes end at 6), a block that holds a NaN or an infinity becomes NaN."""
-    ld = _rows_of(x, "x")
-    if tuple(x.shape) != out.shape:
+    pitch = _rows_of(x, "x")
+    if x.shape != out.shape:
         raise KernelError(f"mxfp4.quantize: {tuple(x.shape)} into {out.shape}")
-    code, stream = ops.dtype_code(x), _launch_stream(x, out.data)
-    fn = ops._fn("mxfp4", "fl_mx_quantize", [c_void_p, c_int, c_long, c_void_p, c_int, c_int, c_void_p])
-    ops._check(fn(x.data_ptr(), code, ld, out.data.data_ptr(), out.rows, out.k, stream), "mxfp4.quantize")
+    code, data = ops.dtype_code(x), out.data
+    stream = _stream_of(x, data, data)
+    ops._check(_fn(_QUANTIZE)(x.data_ptr(), code, pitch, data.data_ptr(), out.rows, out.k, stream), "mxfp4.quantize")
 
 
 def dequantize(q: Matrix, out: torch.Tensor) -> None:
     """out [rows, k] (float32 or bfloat16) = the values that q stands for, exact in both types."""
-    ld = _rows_of(out, "out")
-    if tuple(out.shape) != q.shape:
+    pitch = _rows_of(out, "out")
+    if out.shape != q.shape:
         raise KernelError(f"mxfp4.dequantize: {q.shape} into {tuple(out.shape)}")
-    code, stream = ops.dtype_code(out), _launch_stream(q.data, out)
-    fn = ops._fn("mxfp4", "fl_mx_dequantize", [c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_void_p])
-    ops._check(fn(q.data.data_ptr(), out.data_ptr(), code, ld, q.rows, q.k, stream), "mxfp4.dequantize")
+    code, data = ops.dtype_code(out), q.data
+    stream = _stream_of(data, out, out)
+    ops._check(_fn(_DEQUANTIZE)(data.data_ptr(), out.data_ptr(), code, pitch, q.rows, q.k, stream), "mxfp4.dequantize")
 
 
-def _product(name, x, x_ptr, ldx, m, k, w: Matrix, out, gated, activation, params) -> None:
-    n = w.rows // 2 if gated else w.rows
-    ldo = _rows_of(out, "out")
-    if w.k != k or tuple(out.shape) != (m, n) or (gated and w.rows % 2):
-        raise KernelError(f"mxfp4.{name}: [{m}, {k}] x {w.shape}^T -> {tuple(out.shape)}")
+FEW_ROWS = 16                                    # most rows that the kernel for few of them takes
+
+
+def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, constant_w) -> None:
+    pitch, out_pitch = _activations(x), _rows_of(out, "out")
+    m, k = x.shape
+    if w.k != k or out.shape != (m, n) or (gated and w.rows % 2):
+        raise KernelError(f"mxfp4.{name}: {tuple(x.shape)} x {w.shape}^T -> {tuple(out.shape)}")
     act = -1 if activation is None else ops.activation_code(activation)
-    code = ops.dtype_code(out)
-    stream = _launch_stream(out, x, w.data)
-    fn = ops._fn("mxfp4", "fl_mx_product", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int,
-                                            c_float, c_float, c_void_p])
+    code, data = ops.dtype_code(out), w.data
+    stream = _stream_of(x, data, out)
     if m == 0:
         return
-    if ldx:
-        fn = ops._fn("mxfp4_tc", "fl_mxt_product", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int,
-                                                    c_float, c_float, c_int, c_void_p, c_void_p])
-        from . import gemm_tc
-        rc = fn(x_ptr, ldx, w.data.data_ptr(), out.data_ptr(), code, ldo, m, n, k, int(gated), act, params[0], params[1],
-                ops.sm_count(out.device), gemm_tc.status_word(out.device).data_ptr(), stream)
-        if rc != -1:
-            ops._check(rc, f"mxfp4.{name}")
-            return
+    if m <= FEW_ROWS:
+        rc = _fn(_FEW)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
+                       constant_w, stream)
     else:
-        fn2 = ops._fn("mxfp4_tc", "fl_mxq_product", [c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_void_p, c_void_p])
-        from . import gemm_tc
-        rc = fn2(x_ptr, w.data.data_ptr(), out.data_ptr(), code, ldo, m, n, k, ops.sm_count(out.device),
-                 gemm_tc.status_word(out.device).data_ptr(), stream)
-        if rc != -1:
-            ops._check(rc, f"mxfp4.{name}")
-            return
-    ops._check(fn(x_ptr, ldx, w.data.data_ptr(), out.data_ptr(), code, ldo, m, n, k, int(gated), act,
-                  float(params[0]), float(params[1]), stream), f"mxfp4.{name}")
+        status, sms = _status(x)
+        rc = _fn(_MANY)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
+                        sms, status, stream)
+    ops._check(rc, name)
 
 
-def _activations(x: torch.Tensor) -> int:
-    ld = _rows_of(x, "x")
-    if x.dtype is not torch.bfloat16:
-        raise KernelError(f"mxfp4: activations are bfloat16, got {x.dtype}")
-    if x.shape[0] == 1:
-        ld = -(-ld // 8) * 8                                     # (a single row has no pitch)
-    if ld % 8 or x.data_ptr() % 16:
-        raise KernelError("mxfp4: activations must be 16-byte aligned with a row pitch that is a multiple of 8 elements")
-    return ld
-
-
-def linear(x: torch.Tensor, w: Matrix, out: torch.Tensor, activation: str | None = None, params=(0.0, 0.0)) -> None:
+def linear(x: torch.Tensor, w: Matrix, out: torch.Tensor, activation: str | None = None, params=(0.0, 0.0),
+           constant_w: bool = False) -> None:
     """out[m, n] (bfloat16 or float32) = x[m, k] @ w[n, k]^T; x bfloat16 (16-byte aligned, its row pitch a multiple of 8
-    elements), products and sums in float.  `activation` (`ops.ACTIVATIONS`, f(v, 1)) is applied on the way out."""
-    ld = _activations(x)
-    _product("linear", x, x.data_ptr(), ld, x.shape[0], x.shape[1], w, out, False, activation, params)
+    elements), products and sums in float.  `activation` (`ops.ACTIVATIONS`, f(v, 1)) is applied on the way out.  `constant_w`
+    says that the kernels just before this one in the stream do not write w (a model's matrix), so that its first bytes may be
+    read while they run."""
+    _times_weights("linear", x, w, out, 0, w.rows, activation, params, constant_w)
 
 
-def linear_gated(x: torch.Tensor, w: Matrix, out: torch.Tensor, activation: str = "silu", params=(0.0, 0.0)) -> None:
+def linear_gated(x: torch.Tensor, w: Matrix, out: torch.Tensor, activation: str = "silu", params=(0.0, 0.0),
+                 constant_w: bool = False) -> None:
     """out[m, i] = act(x @ gate^T) * (x @ up^T) for w = [gate; up] stacked as [2 i, k] (any i: the halves' border may lie
-    inside a row tile); both products stay in float until the unit (`ops.ACTIVATIONS`, with its `params`) has been applied."""
-    ld = _activations(x)
-    _product("linear_gated", x, x.data_ptr(), ld, x.shape[0], x.shape[1], w, out, True, activation, params)
+    inside a row tile); both products stay in float until the unit (`ops.ACTIVATIONS`, with its `params`) has been applied.
+    `constant_w` as in `linear`."""
+    _times_weights("linear_gated", x, w, out, 1, w.rows // 2, activation, params, constant_w)
 
 
 def product(a: Matrix, b: Matrix, out: torch.Tensor) -> None:
     """out[m, n] (bfloat16 or float32) = a[m, k] @ b[n, k]^T, both in 4 bits; sums in float."""
-    _product("product", a.data, a.data.data_ptr(), 0, a.rows, a.k, b, out, False, None, (0.0, 0.0))
+    out_pitch = _rows_of(out, "out")
+    if b.k != a.k or out.shape != (a.rows, b.rows):
+        raise KernelError(f"mxfp4.product: {a.shape} x {b.shape}^T -> {tuple(out.shape)}")
+    code, x, w = ops.dtype_code(out), a.data, b.data
+    stream = _stream_of(x, w, out)
+    status, sms = _status(x)
+    ops._check(_fn(_BOTH)(x.data_ptr(), w.data_ptr(), out.data_ptr(), code, out_pitch, a.rows, b.rows, a.k, sms, status, stream), "mxfp4.product")
