@@ -199,91 +199,121 @@ __device__ __forceinline__ uint4 mx_tokens8(const bf16* row, int c, int k) {
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-#define MXF_WARPS 8
-template <typename TO, int MT, int NT, bool GATED>
-__global__ void __launch_bounds__(MXF_WARPS * 32) mx_few_kernel(const bf16* __restrict__ x, long ldx, const uint8_t* __restrict__ w,
-                                                                TO* __restrict__ out, long ldo, int m, int n, int k, bool constant_w,
-                                                                FlGate act) {
+template <typename TO, int WARPS, int MT, int NT, bool GATED>
+__global__ void __launch_bounds__(WARPS * 32, (NT == 1 ? 24 : 16) / WARPS)
+mx_few_kernel(const bf16* __restrict__ x, long ldx, const uint8_t* __restrict__ w, TO* __restrict__ out, long ldo, int m, int n, int k,
+              bool constant_w, FlGate act) {
     static_assert(!GATED || MT == 2, "a gated unit's two rows are a warp's two tiles");
     constexpr int ROWS = GATED ? 16 : 16 * MT;                       // output features of a block
-    __shared__ float red[MXF_WARPS][NT * 8][MT * 16 + 1];
+    __shared__ float red[WARPS][NT * 8][MT * 16 + 1];
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int chunks = (k + 127) / 128;
     const int f0 = blockIdx.x * ROWS;
-    const uint8_t* src[MT][2];                                       // codes of block q of a row, of chunk 0
+    // codes of block q of a row, from the warp's first chunk on (a row that does not exist: of the last one; not stored)
+    const uint8_t* src[MT][2];
     int sc_at[MT][2];                                                // from there to the block's scale
-    bool real[MT][2];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int f = f0 + (GATED ? 0 : 16 * t) + 8 * h + g;
+            const int f = min(f0 + (GATED ? 0 : 16 * t) + 8 * h + g, n - 1);
             const long row = (GATED ? (long)t * n : 0) + f;
             const int r = (int)(row & (MX_ROWS - 1));
-            src[t][h] = w + row / MX_ROWS * chunks * (long)MX_CHUNK + q * 2048 + r * 16;
+            src[t][h] = w + (row / MX_ROWS * chunks + min(warp, chunks - 1)) * (long)MX_CHUNK + q * 2048 + r * 16;
             sc_at[t][h] = (int)mx_scale_at(r) + q - (q * 2048 + r * 16);
-            real[t][h] = f < n;
         }
+    const bf16* token[NT];                                           // (likewise)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) token[j] = x + (long)min(j * 8 + g, m - 1) * ldx + q * 32;
     uint4 codes[MT][2];
     uint32_t scale[MT][2];
-    auto fetch = [&](int c) {
+    auto fetch = [&]() {
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint8_t* p = src[t][h] + (long)c * MX_CHUNK;
-                const bool there = real[t][h] && c < chunks;
-                codes[t][h] = there ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
-                scale[t][h] = there ? p[sc_at[t][h]] : 0;
+                codes[t][h] = *reinterpret_cast<const uint4*>(src[t][h]);
+                scale[t][h] = src[t][h][sc_at[t][h]];
             }
     };
     if (!constant_w) pdl_wait();
-    fetch(warp);
+    fetch();
     if (constant_w) pdl_wait();
     float acc[MT][NT][4] = {};
-    for (int c = warp; c < chunks; c += MXF_WARPS) {
+#pragma unroll 1
+    for (int c = warp; c < chunks; c += WARPS) {
         uint4 now[MT][2];
-        uint32_t m1[MT][2], m2[MT][2];
-        bool large = false;
+        uint32_t m1[MT][2], most = 0;
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 now[t][h] = codes[t][h];
-                const uint32_t s = scale[t][h];
-                m1[t][h] = mx_both(s == 255 ? 0x7FC0u : (min(s, 128u) + 126u) << 7);
-                m2[t][h] = mx_both(s == 255 || s <= 128 ? 0x3F80u : (s - 1) << 7);       // (what 2^(s - 1) has beyond 2^127)
-                large |= s > 128;
+                m1[t][h] = scale[t][h];
+                most = max(most, m1[t][h]);
             }
         uint4 xs[NT][4];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int token = j * 8 + g;
+            if (c * 128 + 128 <= k) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                xs[j][i] = token < m ? mx_tokens8(x + (long)token * ldx, c * 128 + q * 32 + i * 8, k) : make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < 4; ++i) xs[j][i] = *reinterpret_cast<const uint4*>(token[j] + c * 128 + i * 8);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) xs[j][i] = mx_tokens8(token[j] - q * 32, c * 128 + q * 32 + i * 8, k);
+            }
         }
-        fetch(c + MXF_WARPS);
+        if (c + WARPS < chunks) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int t = 0; t < MT; ++t) src[t][0] += WARPS * MX_CHUNK, src[t][1] += WARPS * MX_CHUNK;
+            fetch();
+        }
+        // Multiplied by 2^(s - 1); where that has no bfloat16 (s > 128: a block whose largest magnitude is 4 or more) by 2^127 and
+        // by the rest.
+        if (!__any_sync(0xffffffffu, most > 128u)) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                uint32_t v[2][4];
+                m1[t][0] = (m1[t][0] + 126u) * 0x00800080u, m1[t][1] = (m1[t][1] + 126u) * 0x00800080u;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint4 z = now[t][h];
-                    mx_pairs(i == 0 ? z.x : i == 1 ? z.y : i == 2 ? z.z : z.w, m1[t][h], v[h]);
-                    if (large)
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t v[2][4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[h][e] = mx_mul(v[h][e], m2[t][h]);
-                }
+                    for (int h = 0; h < 2; ++h) mx_pairs(i == 0 ? now[t][h].x : i == 1 ? now[t][h].y : i == 2 ? now[t][h].z : now[t][h].w, m1[t][h], v[h]);
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    mx_mma(acc[t][j], v[0][0], v[1][0], v[0][1], v[1][1], xs[j][i].x, xs[j][i].y);
-                    mx_mma(acc[t][j], v[0][2], v[1][2], v[0][3], v[1][3], xs[j][i].z, xs[j][i].w);
+                    for (int j = 0; j < NT; ++j) {
+                        mx_mma(acc[t][j], v[0][0], v[1][0], v[0][1], v[1][1], xs[j][i].x, xs[j][i].y);
+                        mx_mma(acc[t][j], v[0][2], v[1][2], v[0][3], v[1][3], xs[j][i].z, xs[j][i].w);
+                    }
                 }
             }
+        } else {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                uint32_t m2[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t s = m1[t][h];
+                    m1[t][h] = mx_both(s == 255 ? 0x7FC0u : (min(s, 128u) + 126u) << 7);
+                    m2[h] = mx_both(s == 255 || s <= 128 ? 0x3F80u : (s - 1) << 7);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t v[2][4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        mx_pairs(i == 0 ? now[t][h].x : i == 1 ? now[t][h].y : i == 2 ? now[t][h].z : now[t][h].w, m1[t][h], v[h]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[h][e] = mx_mul(v[h][e], m2[h]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        mx_mma(acc[t][j], v[0][0], v[1][0], v[0][1], v[1][1], xs[j][i].x, xs[j][i].y);
+                        mx_mma(acc[t][j], v[0][2], v[1][2], v[0][3], v[1][3], xs[j][i].z, xs[j][i].w);
+                    }
+                }
+            }
+        }
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t)
@@ -292,30 +322,30 @@ __global__ void __launch_bounds__(MXF_WARPS * 32) mx_few_kernel(const bf16* __re
 #pragma unroll
             for (int e = 0; e < 4; ++e) red[warp][j * 8 + 2 * q + (e & 1)][t * 16 + g + 8 * (e >> 1)] = acc[t][j][e];
     __syncthreads();
-    for (int i = threadIdx.x; i < ROWS * m; i += MXF_WARPS * 32) {
+    for (int i = threadIdx.x; i < ROWS * m; i += WARPS * 32) {
         const int t = i / ROWS, f = i % ROWS;
         if (f0 + f >= n) continue;
         float v = 0.0f, u = 1.0f;
 #pragma unroll
-        for (int s = 0; s < MXF_WARPS; ++s) v += red[s][t][f];
+        for (int s = 0; s < WARPS; ++s) v += red[s][t][f];
         if (GATED) {
             u = 0.0f;
 #pragma unroll
-            for (int s = 0; s < MXF_WARPS; ++s) u += red[s][t][(MT - 1) * 16 + f];
+            for (int s = 0; s < WARPS; ++s) u += red[s][t][(MT - 1) * 16 + f];
         }
         out[(long)t * ldo + f0 + f] = from_f32<TO>(act.act == FL_ACT_NONE ? v : fl_gated(v, u, act));
     }
 }
 
-template <typename TO, int NT>
+template <typename TO, int WARPS, int NT>
 static int mx_launch_few(const bf16* x, long ldx, const uint8_t* w, TO* out, long ldo, int m, int n, int k, bool gated, bool constant_w,
                          FlGate act, cudaStream_t stream) {
-    const dim3 block(MXF_WARPS * 32);
+    const dim3 block(WARPS * 32);
     if (gated)
-        return fl_launch(mx_few_kernel<TO, 2, NT, true>, dim3((n + 15) / 16), block, 0, stream, x, ldx, w, out, ldo, m, n, k, constant_w, act);
+        return fl_launch(mx_few_kernel<TO, WARPS, 2, NT, true>, dim3((n + 15) / 16), block, 0, stream, x, ldx, w, out, ldo, m, n, k, constant_w, act);
     if (n >= 8192)
-        return fl_launch(mx_few_kernel<TO, 2, NT, false>, dim3((n + 31) / 32), block, 0, stream, x, ldx, w, out, ldo, m, n, k, constant_w, act);
-    return fl_launch(mx_few_kernel<TO, 1, NT, false>, dim3((n + 15) / 16), block, 0, stream, x, ldx, w, out, ldo, m, n, k, constant_w, act);
+        return fl_launch(mx_few_kernel<TO, WARPS, 2, NT, false>, dim3((n + 31) / 32), block, 0, stream, x, ldx, w, out, ldo, m, n, k, constant_w, act);
+    return fl_launch(mx_few_kernel<TO, WARPS, 1, NT, false>, dim3((n + 15) / 16), block, 0, stream, x, ldx, w, out, ldo, m, n, k, constant_w, act);
 }
 
 // x: up to 16 bfloat16 rows with `ldx` elements between them (a multiple of 8, from 16 bytes on).  n: output features (gated: half
@@ -326,8 +356,10 @@ FL_API int fl_mx_few(const void* x, long ldx, const void* w, void* out, int out_
     const FlGate gate = {act, p0, p1};
     if (m > 16) return (int)cudaErrorInvalidValue;
     FL_DISPATCH(out_code, TO, {
-        if (m <= 8) return mx_launch_few<TO, 1>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, gated != 0, constant_w != 0, gate, stream);
-        return mx_launch_few<TO, 2>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, gated != 0, constant_w != 0, gate, stream);
+        const int warps = getenv("MXW") ? atoi(getenv("MXW")) : 8;
+        if (warps == 4 && m <= 8) return mx_launch_few<TO, 4, 1>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, gated != 0, constant_w != 0, gate, stream);
+        if (m <= 8) return mx_launch_few<TO, 8, 1>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, gated != 0, constant_w != 0, gate, stream);
+        return mx_launch_few<TO, 8, 2>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, gated != 0, constant_w != 0, gate, stream);
     })
     return (int)cudaErrorInvalidValue;
 }
