@@ -11,6 +11,7 @@
 // are fewer tiles than SMs a cluster of up to 8 CTAs shares K; its partial sums stay in shared memory, and each CTA adds up
 // its share of the tokens from all of them, in rank order.
 #include "tcgen05.cuh"
+#include <stdio.h>
 
 #define MX_ROWS 128
 #define MX_CODES 8192
@@ -82,30 +83,66 @@ __device__ __forceinline__ bool mxt_wait(uint64_t* bar, uint32_t parity, volatil
     if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag) ? 1u : 0u;
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
-__device__ __forceinline__ uint32_t mxt_at_rank(uint32_t saddr, uint32_t rank) {
-    uint32_t a;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
-    return a;
+// Tokens t, t + 8, .. of the float sums [token][2 x 128 rows], added up over the cluster's CTAs in rank order, through the
+// activation and out; `n`: how many features there are from the tile's first on.
+template <int V> struct MxtVec { float v[V]; };
+template <int V> __device__ __forceinline__ MxtVec<V> mxt_get(const float* sums, int ranks, int rank) {
+    MxtVec<V> r;
+    if (ranks == 1) {
+        if (V == 4) {
+            const float4 x = *reinterpret_cast<const float4*>(sums);
+            r.v[V > 3 ? 3 : 0] = x.w, r.v[V > 2 ? 2 : 0] = x.z, r.v[V > 1 ? 1 : 0] = x.y, r.v[0] = x.x;
+        } else {
+            r.v[0] = *sums;
+        }
+        return r;
+    }
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(sums)), "r"(rank));
+    if (V == 4)
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(r.v[0]), "=f"(r.v[V > 1 ? 1 : 0]), "=f"(r.v[V > 2 ? 2 : 0]), "=f"(r.v[V > 3 ? 3 : 0])
+                     : "r"(at)
+                     : "memory");
+    else
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r.v[0]) : "r"(at) : "memory");
+    return r;
 }
-__device__ __forceinline__ float4 mxt_ld_cluster(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-
-// 8 features of one token on their way out
-template <typename TO>
-__device__ __forceinline__ void mxt_store8(TO* dst, const float (&v)[8], int n, bool vec) {
-    TO o[8];
+template <typename TO, bool GATED, int V>
+__device__ __forceinline__ void mxt_rows(const float* sums, int t, int last, int ranks, TO* out, long ldo, int n, const FlGate act) {
+    constexpr int PARTS = (GATED ? 4 : 8) / V;         // steps of 32 V features
+    const int f0 = (threadIdx.x & 31) * V;
+#pragma unroll 2
+    for (; t < last; t += 8) {
+        float g[PARTS * V], u[PARTS * V];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = from_f32<TO>(v[i]);
-    if (vec && n >= 8) {
+        for (int i = 0; i < PARTS * V; ++i) g[i] = 0.0f, u[i] = GATED ? 0.0f : 1.0f;
+        const float* row = sums + t * MXT_PITCH + f0;
+#pragma unroll 4
+        for (int q = 0; q < ranks; ++q)
 #pragma unroll
-        for (int i = 0; i < (int)(8 * sizeof(TO) / 16); ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(o)[i];
-    } else {
+            for (int p = 0; p < PARTS; ++p) {
+                const MxtVec<V> x = mxt_get<V>(row + p * 32 * V, ranks, q);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) dst[i] = o[i];
+                for (int i = 0; i < V; ++i) g[p * V + i] += x.v[i];
+                if (GATED) {
+                    const MxtVec<V> y = mxt_get<V>(row + 128 + p * 32 * V, ranks, q);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) u[p * V + i] += y.v[i];
+                }
+            }
+        if (act.act != FL_ACT_NONE) gated_act(g, u, act);
+        TO* dst = out + (long)t * ldo + f0;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            if (f0 + p * 32 * V >= n) continue;                       // (n is a multiple of V)
+            __align__(16) TO o[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = from_f32<TO>(g[p * V + i]);
+            if (V == 1) dst[p * 32] = o[0];
+            else if (sizeof(TO) == 2) *reinterpret_cast<uint2*>(dst + p * 128) = *reinterpret_cast<const uint2*>(o);
+            else *reinterpret_cast<uint4*>(dst + p * 128) = *reinterpret_cast<const uint4*>(o);
+        }
     }
 }
 
@@ -150,32 +187,12 @@ __device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, uint64_
     // (a CTA of the cluster that gave up leaves its sums as they are: the status word tells that the results are not valid)
     if (warp < 8 && !*abort_flag) {
         const int share = (rows + ranks - 1) / ranks, first = rank * share, last = min(rows, first + share);
-        constexpr int PER = (GATED ? 128 : 256) / 8;                  // threads of a token
-        const int f = (threadIdx.x % PER) * 8;
-        const bool vec = (((uintptr_t)out | (uintptr_t)(ldo * (long)sizeof(TO))) & 15) == 0;
-        for (int t = first + threadIdx.x / PER; t < last && f0 + f < n; t += 256 / PER) {
-            float g[8] = {}, u[8] = {};
-            for (int q = 0; q < ranks; ++q) {
-                const uint32_t at = smem_u32(sums + t * MXT_PITCH + f);
-                const uint32_t a = ranks > 1 ? mxt_at_rank(at, (uint32_t)q) : at;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float4 v = mxt_ld_cluster(a + (uint32_t)(h * 16));
-                    g[4 * h] += v.x, g[4 * h + 1] += v.y, g[4 * h + 2] += v.z, g[4 * h + 3] += v.w;
-                    if (GATED) {
-                        const float4 x = mxt_ld_cluster(a + 512u + (uint32_t)(h * 16));
-                        u[4 * h] += x.x, u[4 * h + 1] += x.y, u[4 * h + 2] += x.z, u[4 * h + 3] += x.w;
-                    }
-                }
-            }
-            if (act.act != FL_ACT_NONE) {
-                if (!GATED)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) u[i] = 1.0f;
-                gated_act(g, u, act);
-            }
-            mxt_store8(out + (long)t * ldo + f0 + f, g, n - f0 - f, vec);
-        }
+        out += f0;
+        // a warp takes a token: four features a lane and 128 a step, or single ones side by side where rows are not aligned
+        if ((((uintptr_t)out | (uintptr_t)(ldo * (long)sizeof(TO))) & (4 * sizeof(TO) - 1)) == 0 && (n & 3) == 0)
+            mxt_rows<TO, GATED, 4>(sums, first + warp, last, ranks, out, ldo, n - f0, act);
+        else
+            mxt_rows<TO, GATED, 1>(sums, first + warp, last, ranks, out, ldo, n - f0, act);
     }
     __syncwarp();
     if (ranks > 1) cluster_sync_all();                                // the others may still read this CTA's sums
@@ -332,12 +349,7 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
 
 // A cluster of CTAs along the grid's x.
 template <typename... KArgs, typename... Args>
-static int mxt_launch_cluster(void (*kernel)(KArgs...), bool& configured, int smem, dim3 grid, cudaStream_t stream, Args... args) {
-    if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return (int)e;
-        configured = true;
-    }
+static int mxt_launch_cluster(void (*kernel)(KArgs...), int smem, dim3 grid, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(MXT_THREADS);
@@ -354,11 +366,39 @@ static int mxt_launch_cluster(void (*kernel)(KArgs...), bool& configured, int sm
     return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-// CTAs of a cluster that share K: as many as there are SMs for, and chunks
-static int mxt_ranks(long tiles, int chunks, int num_sms) {
-    int ranks = 1;
-    while (ranks < 8 && tiles * ranks * 2 <= num_sms && ranks * 2 <= chunks) ranks *= 2;
-    return ranks;
+// How many CTAs of a cluster share K: the number of least time, in the time of a chunk of one CTA, with MXT_FIXED for what a CTA
+// takes besides its chunks.  slots[r]: clusters of r CTAs that the device holds at once.
+#define MXT_FIXED 8
+static int mxt_ranks(long tiles, int chunks, const int* slots) {
+    int best = 1;
+    long least = 0;
+    for (int r = 1; r <= 8 && r <= chunks; ++r) {
+        if (slots[r] < 1) continue;
+        const long time = (tiles + slots[r] - 1) / slots[r] * ((chunks + r - 1) / r + MXT_FIXED) + r / 4;
+        if (least == 0 || time < least) best = r, least = time;
+    }
+    return best;
+}
+// Asked of the driver at a kernel's first launch (the current device's; all that the library runs on are alike).
+template <typename... KArgs>
+static const int* mxt_slots(void (*kernel)(KArgs...), int smem, int (&slots)[9]) {
+    if (slots[0]) return slots;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return nullptr;
+    for (int r = 1; r <= 8; ++r) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(r);
+        cfg.blockDim = dim3(MXT_THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = r;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&slots[r], kernel, &cfg) != cudaSuccess) return nullptr;
+    }
+    slots[0] = 1;
+    return slots;
 }
 
 template <typename TO, bool GATED>
@@ -370,15 +410,17 @@ static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ld
     const int tokens_y = (m + bn - 1) / bn;
     if (tokens_y > 65535 || row_tiles > 65535) return -1;
     const int chunks = (k + 127) / 128;
-    const int ranks = mxt_ranks((long)tokens_y * row_tiles, chunks, num_sms);
+    static int found[9] = {};
+    const int* slots = mxt_slots(mxt_kernel<TO, GATED>, MXT_SMEM, found);
+    if (!slots) return (int)cudaGetLastError();
+    const int ranks = mxt_ranks((long)tokens_y * row_tiles, chunks, slots);
     const int per_rank = (chunks + ranks - 1) / ranks;
     int stages = MXT_RING / (bn * 128);
     if (stages > MXT_MAX_STAGES) stages = MXT_MAX_STAGES;
     CUtensorMap map;
     int rc = make_map(&map, x, m, k, ldx, bn);
     if (rc) return rc;
-    static bool configured = false;
-    return mxt_launch_cluster(mxt_kernel<TO, GATED>, configured, MXT_SMEM, dim3(ranks, tokens_y, row_tiles), stream, map, (const uint8_t*)w,
+    return mxt_launch_cluster(mxt_kernel<TO, GATED>, MXT_SMEM, dim3(ranks, tokens_y, row_tiles), stream, map, (const uint8_t*)w,
                               (TO*)out, ldo, m, n, k, bn, stages, ranks, per_rank, act, status);
 }
 
@@ -532,10 +574,15 @@ FL_API int fl_mxq_product(const void* a, const void* w, void* out, int out_code,
                           cudaStream_t stream) {
     const int chunks = (k + 127) / 128, token_tiles = (m + 127) / 128, row_tiles = (n + 255) / 256;
     if (token_tiles > 65535 || row_tiles > 65535) return -1;
-    const int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, num_sms), per_rank = (chunks + ranks - 1) / ranks;
     FL_DISPATCH(out_code, TO, {
-        static bool configured = false;
-        return mxt_launch_cluster(mxq_kernel<TO>, configured, MXQ_SMEM, dim3(ranks, token_tiles, row_tiles), stream, (const uint8_t*)a,
+        static int found[9] = {};
+        const int* slots = mxt_slots(mxq_kernel<TO>, MXQ_SMEM, found);
+        if (!slots) return (int)cudaGetLastError();
+        int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, slots);
+        if (getenv("MXR")) ranks = atoi(getenv("MXR"));
+        const int per_rank = (chunks + ranks - 1) / ranks;
+        if (getenv("MXV")) printf("slots %d %d %d %d %d %d %d %d ranks %d\n", slots[1], slots[2], slots[3], slots[4], slots[5], slots[6], slots[7], slots[8], ranks);
+        return mxt_launch_cluster(mxq_kernel<TO>, MXQ_SMEM, dim3(ranks, token_tiles, row_tiles), stream, (const uint8_t*)a,
                                   (const uint8_t*)w, (TO*)out, ldo, m, n, chunks, ranks, per_rank, status);
     })
     return (int)cudaErrorInvalidValue;
