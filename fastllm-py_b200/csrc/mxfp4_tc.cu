@@ -6,55 +6,71 @@
 // the weights touches neither global nor shared memory, whose bandwidth the MMA needs for the tokens.
 //
 // A CTA takes two tiles of 128 rows of W (of a gated unit: a gate tile and the up tile of the same features) and up to 128
-// tokens.  Warps 0-7: each thread reads one row's codes from global memory, two chunks ahead, and writes 64 elements of K a
-// time to tensor memory, a ring of MXT_A stages; then the epilogue.  Warp 8: the tokens' TMA.  Warp 9: the MMAs.  Where there
-// are fewer tiles than SMs a cluster of up to 8 CTAs shares K; its partial sums stay in shared memory, and each CTA adds up
-// its share of the tokens from all of them, in rank order.
+// tokens, K in stages of a chunk (128): one copy a row tile, two boxes of the tokens.  Warps 0-15 turn the codes into bfloat16, a
+// thread 64 elements of one row (warps 0-7 the first half of a chunk, 8-15 the second), and write them to a ring of MXT_A places
+// in tensor memory; then they are the epilogue.  Warp 16 sends for the copies, warp 17 issues the MMAs.  Where there are fewer
+// tiles than SMs a cluster of up to 8 CTAs shares K; its partial sums stay in shared memory, and each CTA adds up its share of the
+// tokens from all of them, in rank order.
 #include "tcgen05.cuh"
-#include <stdio.h>
 
 #define MX_ROWS 128
 #define MX_CODES 8192
 #define MX_CHUNK 8704
 #define MXT_BN 128                          // most tokens of a tile
-#define MXT_A 4                             // stages of 2 x 32 columns in tensor memory
-#define MXT_RING (144 * 1024)               // the tokens' ring; the epilogue's sums take its place
-#define MXT_MAX_STAGES 16
+#define MXT_A 4                             // places of 2 x 32 columns in tensor memory
+#define MXT_W_BYTES (2 * (MX_CODES + 1024)) // two row tiles of a chunk: codes, the scales of the one or two packed tiles they lie in
+#define MXT_RING (208 * 1024)               // the epilogue's sums take its place
+#define MXT_MAX_STAGES 10
 #define MXT_PITCH 256                       // floats between the tokens of the sums
 // (No other kernel that takes tensor memory fits an SM beside this much shared memory: an allocation never waits for a CTA that
 // waits for its predecessor in the stream.)
 #define MXT_SMEM (MXT_RING + 1024 + 1024)
-#define MXT_THREADS 320
+#define MXT_WARPS 16                        // that convert, and of the epilogue
+#define MXT_THREADS ((MXT_WARPS + 2) * 32)
 enum { MXT_ERR_WAIT = 121 };
 
 __device__ __forceinline__ int mx_scale_at(int r) { return MX_CODES + (r & 31) * 16 + (r >> 5) * 4; }
 
 // A word of 8 codes as 4 pairs of bfloat16, element 2 i in the low half of w[i]: sign and magnitude of nibbles i and 4 + i where
-// a bfloat16 of exponent 2^-126 has them (the magnitudes 0 and 0.5 are subnormal), times 2^126 times the block's scale, exactly.
-// m1 = 2^(s - 1); where that has no bfloat16 (s > 128) m1 = 2^127 and m2 the rest.
+// a bfloat16 of exponent 2^-126 has them (the magnitudes 0 and 0.5 are subnormal), times m1.  A product with two powers of two puts
+// a nibble in both places at once.
 __device__ __forceinline__ uint32_t mx_mul(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
 __device__ __forceinline__ void mx_pairs(uint32_t q, uint32_t m1, uint32_t* w) {
-    w[0] = mx_mul(((q << 12) & 0x80008000u) | ((q << 6) & 0x01C001C0u), m1);
-    w[1] = mx_mul(((q << 8) & 0x80008000u) | ((q << 2) & 0x01C001C0u), m1);
-    w[2] = mx_mul(((q << 4) & 0x80008000u) | ((q >> 2) & 0x01C001C0u), m1);
+    constexpr uint32_t PLACES = 0x81C081C0u, NIBBLE = 0x000F000Fu;
+    w[0] = mx_mul(((q & NIBBLE) * 0x1040u) & PLACES, m1);
+    w[1] = mx_mul(((q & (NIBBLE << 4)) * 0x104u) & PLACES, m1);
+    w[2] = mx_mul((((q >> 8) & NIBBLE) * 0x1040u) & PLACES, m1);
     w[3] = mx_mul((q & 0x80008000u) | ((q >> 6) & 0x01C001C0u), m1);
 }
 __device__ __forceinline__ uint32_t mx_both(uint32_t h) { return h | h << 16; }
-// 16 bytes of codes, one block of a row with scale byte s, as 16 pairs
-__device__ __forceinline__ void mx_block(const uint4 q, int s, uint32_t* w) {
-    const uint32_t m1 = mx_both(s == 255 ? 0x7FC0u : (uint32_t)(min(s, 128) + 126) << 7);
-    mx_pairs(q.x, m1, w);
-    mx_pairs(q.y, m1, w + 4);
-    mx_pairs(q.z, m1, w + 8);
-    mx_pairs(q.w, m1, w + 12);
-    if (s > 128) {
-        const uint32_t m2 = mx_both(s == 255 ? 0x3F80u : (uint32_t)(s - 1) << 7);
+// Two blocks of a row, 16 bytes of codes each with scale bytes in the low half of `s`, as 32 pairs: exactly the values, the
+// factor being 2^126 times the scale, 2^(s - 1).  Where that has no bfloat16 (s > 128: a block whose largest magnitude is 4 or
+// more) it is 2^127 and the rest; a warp without such a block spends nothing on that.
+__device__ __forceinline__ void mx_blocks(const uint4 a, const uint4 b, uint32_t s, uint32_t* w) {
+    const uint32_t sa = s & 255u, sb = s >> 8 & 255u;
+    uint32_t ma = (sa + 126u) * 0x00800080u, mb = (sb + 126u) * 0x00800080u;
+    const bool large = __any_sync(0xffffffffu, max(sa, sb) > 128u);
+    if (large) {
+        ma = mx_both(sa == 255 ? 0x7FC0u : (min(sa, 128u) + 126u) << 7);
+        mb = mx_both(sb == 255 ? 0x7FC0u : (min(sb, 128u) + 126u) << 7);
+    }
+    mx_pairs(a.x, ma, w);
+    mx_pairs(a.y, ma, w + 4);
+    mx_pairs(a.z, ma, w + 8);
+    mx_pairs(a.w, ma, w + 12);
+    mx_pairs(b.x, mb, w + 16);
+    mx_pairs(b.y, mb, w + 20);
+    mx_pairs(b.z, mb, w + 24);
+    mx_pairs(b.w, mb, w + 28);
+    if (large) {
+        ma = mx_both(sa == 255 || sa <= 128 ? 0x3F80u : (sa - 1) << 7);
+        mb = mx_both(sb == 255 || sb <= 128 ? 0x3F80u : (sb - 1) << 7);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = mx_mul(w[i], m2);
+        for (int i = 0; i < 16; ++i) w[i] = mx_mul(w[i], ma), w[16 + i] = mx_mul(w[16 + i], mb);
     }
 }
 
@@ -74,6 +90,15 @@ __device__ __forceinline__ void mxt_umma_ts(uint32_t tmem_d, uint32_t tmem_a, ui
         "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// One lane of a warp that is together.  The issuing warps stay together and elect for each batch of instructions: what the matrix
+// instructions take then is the same in the whole warp and lives in uniform registers.  Issued by a branch of lane 0 each of them
+// cost 140 to 190 clocks, whatever its size (2048 tokens, K 4096, 22016 features: 472 us, and 331 with the election).
+__device__ __forceinline__ bool mxt_elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ int mxt_warp() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
 __device__ __forceinline__ void mxt_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -83,7 +108,7 @@ __device__ __forceinline__ bool mxt_wait(uint64_t* bar, uint32_t parity, volatil
     if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag) ? 1u : 0u;
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
-// Tokens t, t + 8, .. of the float sums [token][2 x 128 rows], added up over the cluster's CTAs in rank order, through the
+// Tokens t, t + MXT_WARPS, .. of the float sums [token][2 x 128 rows], added up over the cluster's CTAs in rank order, through the
 // activation and out; `n`: how many features there are from the tile's first on.
 template <int V> struct MxtVec { float v[V]; };
 template <int V> __device__ __forceinline__ MxtVec<V> mxt_get(const float* sums, int ranks, int rank) {
@@ -113,7 +138,7 @@ __device__ __forceinline__ void mxt_rows(const float* sums, int t, int last, int
     constexpr int PARTS = (GATED ? 4 : 8) / V;         // steps of 32 V features
     const int f0 = (threadIdx.x & 31) * V;
 #pragma unroll 2
-    for (; t < last; t += 8) {
+    for (; t < last; t += MXT_WARPS) {
         float g[PARTS * V], u[PARTS * V];
 #pragma unroll
         for (int i = 0; i < PARTS * V; ++i) g[i] = 0.0f, u[i] = GATED ? 0.0f : 1.0f;
@@ -155,22 +180,22 @@ __device__ __forceinline__ void mxt_give_up(volatile int* abort_flag, int* statu
 
 // What both kernels end with, by the whole CTA: the accumulators (valid where `any`, else zero) as float sums [token][2 x 128
 // rows] in shared memory, where the ring was (every copy has been read by an MMA that is done), and this CTA's share of the tokens from all of the cluster's.
-// `ok`: of warps 0-7, whether the accumulators may be waited for.  Leaves with the cluster's sums no longer needed.
+// `ok`: of the first MXT_WARPS warps, whether the accumulators may be waited for.  Leaves with the cluster's sums no longer needed.
 template <typename TO, bool GATED>
 __device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, uint64_t* acc_bar, volatile int* abort_flag, int* status, bool ok,
                                            bool any, int rows, int ranks, int rank, TO* __restrict__ out, long ldo, int f0, int n,
                                            const FlGate act) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp < 8) {
+    const int warp = mxt_warp(), lane = threadIdx.x & 31;
+    if (warp < MXT_WARPS) {
         if (ok && !mxt_wait(acc_bar, 0, abort_flag)) {
             if (lane == 0) mxt_give_up(abort_flag, status);
             ok = false;
         }
         if (ok) {
             tc_fence_after();
-            const int tile = warp >> 2, f = tile * 128 + (threadIdx.x & 127);
+            const int tile = warp >> 2 & 1, f = tile * 128 + (threadIdx.x & 127);
             const uint32_t src = tmem_d + (uint32_t)(tile * 128) + ((uint32_t)((warp & 3) * 32) << 16);
-            for (int c = 0; c < rows; c += 16) {
+            for (int c = (warp >> 3) * 16; c < rows; c += 32) {
                 uint32_t v[16];
                 tmem_ld16(src + (uint32_t)c, v);
                 tmem_ld_wait();
@@ -185,7 +210,7 @@ __device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, uint64_
     else __syncthreads();
     tc_fence_after();
     // (a CTA of the cluster that gave up leaves its sums as they are: the status word tells that the results are not valid)
-    if (warp < 8 && !*abort_flag) {
+    if (warp < MXT_WARPS && !*abort_flag) {
         const int share = (rows + ranks - 1) / ranks, first = rank * share, last = min(rows, first + share);
         out += f0;
         // a warp takes a token: four features a lane and 128 a step, or single ones side by side where rows are not aligned
@@ -199,12 +224,18 @@ __device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, uint64_
     else __syncthreads();
 }
 
-// grid: ranks of a cluster x token tiles x row tiles (pairs of them).  bn: tokens of a tile, a multiple of 16.  stages: of
-// bn x 64 elements in the ring.
+__device__ __forceinline__ void mxt_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+                 "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// grid: ranks of a cluster x token tiles x row tiles (pairs of them).  bn: tokens of a tile, a multiple of 16.  A stage is bn x 128
+// tokens' elements as two boxes, then W.
 template <typename TO, bool GATED>
 __global__ void __launch_bounds__(MXT_THREADS, 1)
 mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ w, TO* __restrict__ out, long ldo, int m, int n,
-           int k, int bn, int stages, int ranks, int per_rank, FlGate act, int* __restrict__ status) {
+           int k, int bn, int stages, int ranks, int per_rank, bool constant_w, FlGate act, int* __restrict__ status) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* ring = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* full_bar = (uint64_t*)(ring + MXT_RING);
@@ -214,19 +245,22 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
     uint64_t* acc_bar = a_empty + MXT_A;
     uint32_t* tmem_slot = (uint32_t*)(acc_bar + 1);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = mxt_warp(), lane = threadIdx.x & 31;
     const int rank = blockIdx.x;
     const int t0 = blockIdx.y * bn;
     const int f0 = blockIdx.z * (GATED ? 128 : 256);
     const int chunks = (k + 127) / 128;
     const int c_begin = rank * per_rank, c_end = min(chunks, c_begin + per_rank);
-    const int blocks = 2 * max(0, c_end - c_begin);              // of 64 elements along K
-    const int stage_bytes = bn * 128;
+    const int x_bytes = bn * 256, stage_bytes = x_bytes + MXT_W_BYTES;
+    // the second row tile: none, a packed tile, or (a gated unit's up rows) the end of one and the beginning of the next
+    const int tiles = GATED || n - f0 > 128 ? 2 : 1;
+    const long row1 = GATED ? (long)n + f0 : (long)f0 + 128;
+    const int off = (int)(row1 & (MX_ROWS - 1));
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
             mbar_init(&full_bar[s], 1);
-            mbar_init(&empty_bar[s], 1);
+            mbar_init(&empty_bar[s], MXT_WARPS + 1);
         }
         for (int s = 0; s < MXT_A; ++s) {
             mbar_init(&a_full[s], 8);
@@ -237,114 +271,145 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 9) {
+    if (warp == MXT_WARPS + 1) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_d = *tmem_slot, tmem_a = tmem_d + 256;   // accumulators of 128 columns each, then the ring of A
-    auto give_up = [&]() { mxt_give_up(abort_flag, status); };
+    const uint32_t tmem_d = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_a = tmem_d + 256;   // accumulators of 128 columns each, then the ring of A
     pdl_trigger();
-    pdl_wait();
     int issued = 0;
     bool ok = !*abort_flag;
-    if (warp < 8) {
-        // ---- a thread's row of W: codes two chunks ahead in registers, 64 elements a time to tensor memory
-        const int tile = warp >> 2;
-        const long row = (GATED ? (long)tile * n : (long)tile * 128) + f0 + (threadIdx.x & 127);
-        const bool real = GATED ? f0 + (threadIdx.x & 127) < n : row < n;
-        const int r = (int)(row & (MX_ROWS - 1));
-        const uint8_t* src = w + row / MX_ROWS * chunks * (long)MX_CHUNK;
-        const uint32_t dst = tmem_a + (uint32_t)(tile * 32) + ((uint32_t)((warp & 3) * 32) << 16);
-        uint4 q[2][4];
-        uint32_t sc[2];
-        auto fetch = [&](int buf, int c) {
-            const uint8_t* p = src + (long)c * MX_CHUNK;
-            const bool there = real && c < c_end;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) q[buf][b] = there ? __ldg(reinterpret_cast<const uint4*>(p + b * 2048 + r * 16)) : make_uint4(0, 0, 0, 0);
-            sc[buf] = there ? __ldg(reinterpret_cast<const uint32_t*>(p + mx_scale_at(r))) : 0;
-        };
-        fetch(0, c_begin);
-        fetch(1, c_begin + 1);
-        int sa = 0;
-        uint32_t pa = 0;
-        auto convert = [&](int buf, int c) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (!ok) return;
-                uint32_t v[32];
-                mx_block(q[buf][2 * h], (int)(sc[buf] >> (16 * h)) & 255, v);
-                mx_block(q[buf][2 * h + 1], (int)(sc[buf] >> (16 * h + 8)) & 255, v + 16);
-                if (!mxt_wait(&a_empty[sa], pa ^ 1u, abort_flag)) {
-                    if (lane == 0) give_up();
-                    ok = false;
-                    return;
-                }
-                tc_fence_after();
-                mxt_tmem_st16(dst + (uint32_t)(sa * 64), v);
-                mxt_tmem_st16(dst + (uint32_t)(sa * 64 + 16), v + 16);
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mxt_arrive(&a_full[sa]);
-                if (++sa == MXT_A) { sa = 0; pa ^= 1u; }
+    if (warp < MXT_WARPS) {
+        pdl_wait();                                              // (the output may still be read by the preceding kernel)
+        // ---- codes to bfloat16: a thread's row of tile `tile`, half `half` of every chunk
+        const int tile = warp >> 2 & 1, half = warp >> 3, r = threadIdx.x & 127;
+        const bool here = tile < tiles;
+        const int rr = (tile ? off : 0) + r;                     // the row's place in the packed tiles
+        const int codes_at = x_bytes + tile * (MX_CODES + 1024) + half * 4096 + r * 16;
+        const int scale_at = x_bytes + tile * (MX_CODES + 1024) + (rr >> 7) * 512 + mx_scale_at(rr & 127) + half * 2;
+        const uint32_t dst = tmem_a + (uint32_t)(half * 64 + tile * 32) + ((uint32_t)((warp & 3) * 32) << 16);
+        int s = 0;
+        uint32_t ph = 0, sa = 0, pa = 0;                         // place of A: 2 sa + half
+        for (int c = c_begin; c < c_end && ok; ++c) {
+            if (!mxt_wait(&full_bar[s], ph, abort_flag)) {
+                if (lane == 0) mxt_give_up(abort_flag, status);
+                ok = false;
+                break;
             }
-            fetch(buf, c + 2);
-        };
-        for (int c = c_begin; c < c_end && ok; c += 2) {
-            convert(0, c);
-            if (c + 1 < c_end && ok) convert(1, c + 1);
-        }
-    } else if (warp == 8) {
-        if (lane == 0) {
-            // ---- producer of the tokens' tiles
-            int s = 0;
-            uint32_t ph = 0;
-            for (int i = 0; i < blocks && ok; ++i) {
-                if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag)) {
-                    give_up();
-                    break;
-                }
-                mbar_expect_tx(&full_bar[s], (uint32_t)stage_bytes);
-                tma_load_2d(ring + s * stage_bytes, &map_x, &full_bar[s], (2 * c_begin + i) * 64, t0);
-                ++issued;
-                if (++s == stages) { s = 0; ph ^= 1u; }
-            }
-        }
-    } else if (lane == 0) {
-        // ---- MMA issuer
-        const uint32_t idesc = instr_desc_bf16(128, bn);
-        int s = 0, sa = 0;
-        uint32_t ph = 0, pa = 0;
-        for (int i = 0; i < blocks && ok; ++i) {
-            if (!mbar_wait(&full_bar[s], ph, abort_flag) || !mbar_wait(&a_full[sa], pa, abort_flag)) {
-                give_up();
+            const unsigned char* stage = ring + s * stage_bytes;
+            const uint4 qa = *reinterpret_cast<const uint4*>(stage + codes_at), qb = *reinterpret_cast<const uint4*>(stage + codes_at + 2048);
+            const uint32_t sc = *reinterpret_cast<const uint16_t*>(stage + scale_at);
+            __syncwarp();
+            if (lane == 0) mxt_arrive(&empty_bar[s]);
+            uint32_t v[32];
+            if (here) mx_blocks(qa, qb, sc, v);
+            if (!mxt_wait(&a_empty[2 * sa + half], pa ^ 1u, abort_flag)) {
+                if (lane == 0) mxt_give_up(abort_flag, status);
                 ok = false;
                 break;
             }
             tc_fence_after();
-            const uint64_t bdesc = smem_desc_sw128(smem_u32(ring + s * stage_bytes));
-#pragma unroll
-            for (int tile = 0; tile < 2; ++tile)
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    mxt_umma_ts(tmem_d + (uint32_t)(tile * 128), tmem_a + (uint32_t)(sa * 64 + tile * 32 + kk * 8), bdesc + (uint64_t)(2 * kk),
-                                idesc, (i > 0 || kk > 0) ? 1u : 0u);
-            umma_commit(&empty_bar[s]);
-            umma_commit(&a_empty[sa]);
+            if (here) {
+                mxt_tmem_st16(dst + sa * 128u, v);
+                mxt_tmem_st16(dst + sa * 128u + 16u, v + 16);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mxt_arrive(&a_full[2 * sa + half]);
             if (++s == stages) { s = 0; ph ^= 1u; }
-            if (++sa == MXT_A) { sa = 0; pa ^= 1u; }
+            if (++sa == MXT_A / 2) { sa = 0; pa ^= 1u; }
         }
-        if (ok) umma_commit(acc_bar);
+    } else if (warp == MXT_WARPS) {
+        if (lane == 0) {
+            // ---- producer
+            const long tile_bytes = (long)chunks * MX_CHUNK;
+            const uint8_t* src0 = w + (long)(f0 / MX_ROWS) * tile_bytes;
+            const uint8_t* src1 = w + row1 / MX_ROWS * tile_bytes;
+            const bool second = off != 0 && (row1 / MX_ROWS + 1) * MX_ROWS < 2l * n;         // (only up rows straddle)
+            const uint32_t w_bytes = MX_CHUNK + (tiles < 2 ? 0 : off == 0 ? MX_CHUNK : 4 * (MX_ROWS - off) * 16 + 512 + (second ? 4 * off * 16 + 512 : 0));
+            auto send_w = [&](int s, int c) {
+                unsigned char* dst = ring + s * stage_bytes + x_bytes;
+                mbar_expect_tx(&full_bar[s], (uint32_t)x_bytes + w_bytes);
+                mxt_copy(dst, src0 + (long)c * MX_CHUNK, MX_CHUNK, &full_bar[s]);
+                if (tiles < 2) return;
+                dst += MX_CODES + 1024;
+                const uint8_t* src = src1 + (long)c * MX_CHUNK;
+                if (off == 0) {
+                    mxt_copy(dst, src, MX_CHUNK, &full_bar[s]);
+                    return;
+                }
+                for (int b = 0; b < 4; ++b) mxt_copy(dst + b * 2048, src + b * 2048 + off * 16, (uint32_t)(MX_ROWS - off) * 16, &full_bar[s]);
+                mxt_copy(dst + MX_CODES, src + MX_CODES, 512, &full_bar[s]);
+                if (!second) return;
+                src += tile_bytes;
+                for (int b = 0; b < 4; ++b) mxt_copy(dst + b * 2048 + (MX_ROWS - off) * 16, src + b * 2048, (uint32_t)off * 16, &full_bar[s]);
+                mxt_copy(dst + MX_CODES + 512, src + MX_CODES, 512, &full_bar[s]);
+            };
+            auto send_x = [&](int s, int c) {
+                tma_load_2d(ring + s * stage_bytes, &map_x, &full_bar[s], c * 128, t0);
+                tma_load_2d(ring + s * stage_bytes + x_bytes / 2, &map_x, &full_bar[s], c * 128 + 64, t0);
+            };
+            // a constant W's first stages are sent for before the preceding kernel is waited for
+            const int ahead = constant_w && ok ? min(stages, c_end - c_begin) : 0;
+            for (int i = 0; i < ahead; ++i) send_w(i, c_begin + i);
+            pdl_wait();
+            for (int i = 0; i < ahead; ++i) send_x(i, c_begin + i);
+            issued = max(ahead, 0);
+            int s = issued % stages;
+            uint32_t ph = (uint32_t)(issued / stages) & 1u;
+            for (int c = c_begin + issued; c < c_end && ok; ++c) {
+                if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag)) {
+                    mxt_give_up(abort_flag, status);
+                    break;
+                }
+                send_w(s, c);
+                send_x(s, c);
+                ++issued;
+                if (++s == stages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else {
+        // ---- MMA issuer
+        const uint32_t idesc = instr_desc_bf16(128, bn), ring_at = smem_u32(ring);
+        int s = 0;
+        uint32_t ph = 0, sa = 0, pa = 0;
+        for (int c = c_begin; c < c_end && ok; ++c) {
+            bool there = mxt_wait(&full_bar[s], ph, abort_flag);
+            for (int half = 0; half < 2 && there; ++half) {
+                there = mxt_wait(&a_full[2 * sa + half], pa, abort_flag);
+                if (!there) break;
+                tc_fence_after();
+                const uint64_t bdesc = smem_desc_sw128(ring_at + (uint32_t)(s * stage_bytes + half * (x_bytes / 2)));
+                if (mxt_elect()) {
+                    for (int tile = 0; tile < tiles; ++tile)
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            mxt_umma_ts(tmem_d + (uint32_t)(tile * 128), tmem_a + sa * 128u + (uint32_t)(half * 64 + tile * 32 + kk * 8),
+                                        bdesc + (uint64_t)(2 * kk), idesc, (c > c_begin || half > 0 || kk > 0) ? 1u : 0u);
+                    umma_commit(&a_empty[2 * sa + half]);
+                    if (half == 1) umma_commit(&empty_bar[s]);
+                }
+                __syncwarp();
+            }
+            if (!there) {
+                if (lane == 0) mxt_give_up(abort_flag, status);
+                ok = false;
+                break;
+            }
+            if (++s == stages) { s = 0; ph ^= 1u; }
+            if (++sa == MXT_A / 2) { sa = 0; pa ^= 1u; }
+        }
+        if (ok && mxt_elect()) umma_commit(acc_bar);
     }
-    mxt_finish<TO, GATED>(reinterpret_cast<float*>(ring), tmem_d, acc_bar, abort_flag, status, ok, blocks > 0, min(bn, m - t0), ranks, rank,
+    mxt_finish<TO, GATED>(reinterpret_cast<float*>(ring), tmem_d, acc_bar, abort_flag, status, ok, c_end > c_begin, min(bn, m - t0), ranks, rank,
                           out + (long)t0 * ldo, ldo, f0, n, act);
-    if (warp == 8 && lane == 0 && *abort_flag) tma_drain(full_bar, stages, issued);
+    if (warp == MXT_WARPS && lane == 0 && *abort_flag) tma_drain(full_bar, stages, issued);
     __syncthreads();
-    if (warp == 9) tmem_dealloc(tmem_d, 512);
+    if (warp == MXT_WARPS + 1) tmem_dealloc(tmem_d, 512);
 }
 
 // A cluster of CTAs along the grid's x.
@@ -402,36 +467,35 @@ static const int* mxt_slots(void (*kernel)(KArgs...), int smem, int (&slots)[9])
 }
 
 template <typename TO, bool GATED>
-static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ldo, int m, int n, int k, FlGate act, int num_sms,
+static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ldo, int m, int n, int k, bool constant_w, FlGate act,
                       int* status, cudaStream_t stream) {
     const int token_tiles = (m + MXT_BN - 1) / MXT_BN;
     const int bn = ((m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
     const int row_tiles = (n + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
-    const int tokens_y = (m + bn - 1) / bn;
-    if (tokens_y > 65535 || row_tiles > 65535) return -1;
-    const int chunks = (k + 127) / 128;
+    const int tokens_y = (m + bn - 1) / bn, chunks = (k + 127) / 128;
+    if (tokens_y > 65535 || row_tiles > 65535) return (int)cudaErrorInvalidValue;
     static int found[9] = {};
     const int* slots = mxt_slots(mxt_kernel<TO, GATED>, MXT_SMEM, found);
     if (!slots) return (int)cudaGetLastError();
     const int ranks = mxt_ranks((long)tokens_y * row_tiles, chunks, slots);
     const int per_rank = (chunks + ranks - 1) / ranks;
-    int stages = MXT_RING / (bn * 128);
+    int stages = MXT_RING / (bn * 256 + MXT_W_BYTES);
     if (stages > MXT_MAX_STAGES) stages = MXT_MAX_STAGES;
     CUtensorMap map;
     int rc = make_map(&map, x, m, k, ldx, bn);
     if (rc) return rc;
-    return mxt_launch_cluster(mxt_kernel<TO, GATED>, MXT_SMEM, dim3(ranks, tokens_y, row_tiles), stream, map, (const uint8_t*)w,
-                              (TO*)out, ldo, m, n, k, bn, stages, ranks, per_rank, act, status);
+    return mxt_launch_cluster(mxt_kernel<TO, GATED>, MXT_SMEM, dim3(ranks, tokens_y, row_tiles), stream, map, (const uint8_t*)w, (TO*)out, ldo, m,
+                              n, k, bn, stages, ranks, per_rank, constant_w, act, status);
 }
 
 // x: bfloat16 rows, 16-byte aligned, `ldx` elements apart (a multiple of 8).  n: output features (gated: half of w's rows).
-// -1: not for this kernel.
+// constant_w: no kernel before this one in the stream writes w, so its first bytes may be read while that one still runs.
 FL_API int fl_mxt_product(const void* x, long ldx, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int gated,
-                          int act, float p0, float p1, int num_sms, int* status, cudaStream_t stream) {
+                          int act, float p0, float p1, int constant_w, int* status, cudaStream_t stream) {
     const FlGate gate = {act, p0, p1};
     FL_DISPATCH(out_code, TO, {
-        return gated ? mxt_launch<TO, true>(x, ldx, w, out, ldo, m, n, k, gate, num_sms, status, stream)
-                     : mxt_launch<TO, false>(x, ldx, w, out, ldo, m, n, k, gate, num_sms, status, stream);
+        return gated ? mxt_launch<TO, true>(x, ldx, w, out, ldo, m, n, k, constant_w != 0, gate, status, stream)
+                     : mxt_launch<TO, false>(x, ldx, w, out, ldo, m, n, k, constant_w != 0, gate, status, stream);
     })
     return (int)cudaErrorInvalidValue;
 }
@@ -446,11 +510,6 @@ FL_API int fl_mxt_product(const void* x, long ldx, const void* w, void* out, int
 #define MXQ_SF 12                                              // columns of a stage's scales
 #define MXQ_SMEM (MXQ_STAGES * MXQ_STAGE + 1024)
 
-__device__ __forceinline__ void mxq_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
-                 "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
-}
 // no swizzle: `lead` bytes between core matrices along K, 128 between those of neighbouring groups of 8 rows
 __device__ __forceinline__ uint64_t mxq_desc(uint32_t saddr, uint32_t lead) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
@@ -484,7 +543,7 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
     uint64_t* acc_bar = empty_bar + MXQ_STAGES;
     uint32_t* tmem_slot = (uint32_t*)(acc_bar + 1);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = mxt_warp(), lane = threadIdx.x & 31;
     const int rank = blockIdx.x;
     const int t0 = blockIdx.y * 128, f0 = blockIdx.z * 256;
     const int rows = min(128, m - t0), tiles = n - f0 > 128 ? 2 : 1;
@@ -500,19 +559,19 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 9) {
+    if (warp == MXT_WARPS + 1) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_d = *tmem_slot, tmem_sf = tmem_d + 256;
+    const uint32_t tmem_d = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_sf = tmem_d + 256;
     pdl_trigger();
     pdl_wait();
     int issued = 0;
     const bool ok = !*abort_flag;
-    if (warp == 8) {
+    if (warp == MXT_WARPS) {
         if (lane == 0) {
             const uint8_t* src_a = a + (long)blockIdx.y * chunks * MX_CHUNK;
             const uint8_t* src_w = w + (long)blockIdx.z * 2 * chunks * MX_CHUNK;
@@ -525,28 +584,28 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
                 }
                 unsigned char* dst = ring + s * MXQ_STAGE;
                 mbar_expect_tx(&full_bar[s], (uint32_t)((tiles + 1) * MX_CHUNK));
-                mxq_copy(dst, src_a + (long)c * MX_CHUNK, MX_CHUNK, &full_bar[s]);
+                mxt_copy(dst, src_a + (long)c * MX_CHUNK, MX_CHUNK, &full_bar[s]);
                 for (int t = 0; t < tiles; ++t)
-                    mxq_copy(dst + (1 + t) * MX_CHUNK, src_w + ((long)t * chunks + c) * MX_CHUNK, MX_CHUNK, &full_bar[s]);
+                    mxt_copy(dst + (1 + t) * MX_CHUNK, src_w + ((long)t * chunks + c) * MX_CHUNK, MX_CHUNK, &full_bar[s]);
                 ++issued;
                 if (++s == MXQ_STAGES) { s = 0; ph ^= 1u; }
             }
         }
-    } else if (warp == 9) {
-        if (lane == 0) {
-            const int bn = (rows + 15) / 16 * 16;
-            const uint32_t idesc[2] = {mxq_idesc(bn, 0), mxq_idesc(bn, 2)};
-            int s = 0;
-            uint32_t ph = 0;
-            bool going = ok;
-            for (int c = c_begin; c < c_end && going; ++c) {
-                if (!mbar_wait(&full_bar[s], ph, abort_flag)) {
-                    mxt_give_up(abort_flag, status);
-                    going = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t at = smem_u32(ring + s * MXQ_STAGE), sf = tmem_sf + (uint32_t)(s * MXQ_SF);
+    } else if (warp == MXT_WARPS + 1) {
+        const int bn = (rows + 15) / 16 * 16;
+        const uint32_t idesc[2] = {mxq_idesc(bn, 0), mxq_idesc(bn, 2)}, ring_at = smem_u32(ring);
+        int s = 0;
+        uint32_t ph = 0;
+        bool going = ok;
+        for (int c = c_begin; c < c_end && going; ++c) {
+            if (!mxt_wait(&full_bar[s], ph, abort_flag)) {
+                if (lane == 0) mxt_give_up(abort_flag, status);
+                going = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t at = ring_at + (uint32_t)(s * MXQ_STAGE), sf = tmem_sf + (uint32_t)(s * MXQ_SF);
+            if (mxt_elect()) {
                 // (the stage's columns: its last use's MMAs were done before its copies were sent for)
                 for (int t = 0; t <= tiles; ++t)
                     mxq_copy_scales(sf + (uint32_t)(4 * t), mxq_desc(at + (uint32_t)(t * MX_CHUNK + MX_CODES), 128));
@@ -557,31 +616,30 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
                                  mxq_desc(at + (uint32_t)(h * 4096), 2048), idesc[h], sf + (uint32_t)(4 + 4 * t), sf,
                                  (c > c_begin || h > 0) ? 1u : 0u);
                 umma_commit(&empty_bar[s]);
-                if (++s == MXQ_STAGES) { s = 0; ph ^= 1u; }
             }
-            if (going) umma_commit(acc_bar);
+            __syncwarp();
+            if (++s == MXQ_STAGES) { s = 0; ph ^= 1u; }
         }
+        if (going && mxt_elect()) umma_commit(acc_bar);
     }
     mxt_finish<TO, false>(reinterpret_cast<float*>(ring), tmem_d, acc_bar, abort_flag, status, ok, c_end > c_begin, rows, ranks, rank,
                           out + (long)t0 * ldo, ldo, f0, n, FlGate{FL_ACT_NONE, 0.0f, 0.0f});
-    if (warp == 8 && lane == 0 && *abort_flag) tma_drain(full_bar, MXQ_STAGES, issued);
+    if (warp == MXT_WARPS && lane == 0 && *abort_flag) tma_drain(full_bar, MXQ_STAGES, issued);
     __syncthreads();
-    if (warp == 9) tmem_dealloc(tmem_d, 512);
+    if (warp == MXT_WARPS + 1) tmem_dealloc(tmem_d, 512);
 }
 
-// a [m, k] and w [n, k] packed.  -1: not for this kernel.
-FL_API int fl_mxq_product(const void* a, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int num_sms, int* status,
+// a [m, k] and w [n, k] packed.
+FL_API int fl_mxq_product(const void* a, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int* status,
                           cudaStream_t stream) {
     const int chunks = (k + 127) / 128, token_tiles = (m + 127) / 128, row_tiles = (n + 255) / 256;
-    if (token_tiles > 65535 || row_tiles > 65535) return -1;
+    if (token_tiles > 65535 || row_tiles > 65535) return (int)cudaErrorInvalidValue;
     FL_DISPATCH(out_code, TO, {
         static int found[9] = {};
         const int* slots = mxt_slots(mxq_kernel<TO>, MXQ_SMEM, found);
         if (!slots) return (int)cudaGetLastError();
-        int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, slots);
-        if (getenv("MXR")) ranks = atoi(getenv("MXR"));
+        const int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, slots);
         const int per_rank = (chunks + ranks - 1) / ranks;
-        if (getenv("MXV")) printf("slots %d %d %d %d %d %d %d %d ranks %d\n", slots[1], slots[2], slots[3], slots[4], slots[5], slots[6], slots[7], slots[8], ranks);
         return mxt_launch_cluster(mxq_kernel<TO>, MXQ_SMEM, dim3(ranks, token_tiles, row_tiles), stream, (const uint8_t*)a,
                                   (const uint8_t*)w, (TO*)out, ldo, m, n, chunks, ranks, per_rank, status);
     })

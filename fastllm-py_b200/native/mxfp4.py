@@ -108,7 +108,7 @@ _FEW = ("mxfp4", "fl_mx_few", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_lo
                                c_int, c_void_p])
 _MANY = ("mxfp4_tc", "fl_mxt_product", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_float,
                                         c_float, c_int, c_void_p, c_void_p])
-_BOTH = ("mxfp4_tc", "fl_mxq_product", [c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_void_p, c_void_p])
+_BOTH = ("mxfp4_tc", "fl_mxq_product", [c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_void_p, c_void_p])
 
 
 def _fn(which):
@@ -118,12 +118,12 @@ def _fn(which):
     return fn
 
 
-def _status(t: torch.Tensor):
-    """(address of the device's status word, its number of SMs)."""
+def _status(t: torch.Tensor) -> int:
+    """Address of the device's status word."""
     found = _fns.get(t.get_device())
     if found is None:
         from . import gemm_tc
-        found = _fns[t.get_device()] = (gemm_tc.status_word(t.device).data_ptr(), ops.sm_count(t.device))
+        found = _fns[t.get_device()] = gemm_tc.status_word(t.device).data_ptr()
     return found
 
 
@@ -148,7 +148,8 @@ def dequantize(q: Matrix, out: torch.Tensor) -> None:
     ops._check(_fn(_DEQUANTIZE)(data.data_ptr(), out.data_ptr(), code, pitch, q.rows, q.k, stream), "mxfp4.dequantize")
 
 
-FEW_ROWS = 16                                    # most rows that the kernel for few of them takes
+import os
+FEW_ROWS = int(os.environ.get('MXF', '16'))                                    # most rows that the kernel for few of them takes
 
 
 def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, constant_w) -> None:
@@ -165,9 +166,8 @@ def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, consta
         rc = _fn(_FEW)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
                        constant_w, stream)
     else:
-        status, sms = _status(x)
         rc = _fn(_MANY)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
-                        sms, status, stream)
+                        constant_w, _status(x), stream)
     ops._check(rc, name)
 
 
@@ -195,5 +195,4 @@ def product(a: Matrix, b: Matrix, out: torch.Tensor) -> None:
         raise KernelError(f"mxfp4.product: {a.shape} x {b.shape}^T -> {tuple(out.shape)}")
     code, x, w = ops.dtype_code(out), a.data, b.data
     stream = _stream_of(x, w, out)
-    status, sms = _status(x)
-    ops._check(_fn(_BOTH)(x.data_ptr(), w.data_ptr(), out.data_ptr(), code, out_pitch, a.rows, b.rows, a.k, sms, status, stream), "mxfp4.product")
+    ops._check(_fn(_BOTH)(x.data_ptr(), w.data_ptr(), out.data_ptr(), code, out_pitch, a.rows, b.rows, a.k, _status(x), stream), "mxfp4.product")
