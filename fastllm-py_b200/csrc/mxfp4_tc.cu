@@ -7,8 +7,8 @@
 //
 // A CTA takes two tiles of 128 rows of W (of a gated unit: a gate tile and the up tile of the same features) and up to 128
 // tokens, K in stages of a chunk (128): one copy a row tile, two boxes of the tokens.  Warps 0-15 turn the codes into bfloat16, a
-// thread 64 elements of one row (warps 0-7 the first half of a chunk, 8-15 the second), and write them to a ring of MXT_A places
-// in tensor memory; then they are the epilogue.  Warp 16 sends for the copies, warp 17 issues the MMAs.  Where there are fewer
+// thread one row of a chunk (warps 0-7 of every other one, 8-15 of those between), and write them to one of the two places in
+// tensor memory; then they are the epilogue.  Warp 16 sends for the copies, warp 17 issues the MMAs.  Where there are fewer
 // tiles than SMs a cluster of up to 8 CTAs shares K; its partial sums stay in shared memory, and each CTA adds up its share of the
 // tokens from all of them, in rank order.
 #include "tcgen05.cuh"
@@ -17,7 +17,7 @@
 #define MX_CODES 8192
 #define MX_CHUNK 8704
 #define MXT_BN 128                          // most tokens of a tile
-#define MXT_A 4                             // places of 2 x 32 columns in tensor memory
+#define MXT_A 2                             // places of 2 x 64 columns in tensor memory
 #define MXT_W_BYTES (2 * (MX_CODES + 1024)) // two row tiles of a chunk: codes, the scales of the one or two packed tiles they lie in
 #define MXT_RING (208 * 1024)               // the epilogue's sums take its place
 #define MXT_MAX_STAGES 10
@@ -47,31 +47,21 @@ __device__ __forceinline__ void mx_pairs(uint32_t q, uint32_t m1, uint32_t* w) {
     w[3] = mx_mul((q & 0x80008000u) | ((q >> 6) & 0x01C001C0u), m1);
 }
 __device__ __forceinline__ uint32_t mx_both(uint32_t h) { return h | h << 16; }
-// Two blocks of a row, 16 bytes of codes each with scale bytes in the low half of `s`, as 32 pairs: exactly the values, the
-// factor being 2^126 times the scale, 2^(s - 1).  Where that has no bfloat16 (s > 128: a block whose largest magnitude is 4 or
-// more) it is 2^127 and the rest; a warp without such a block spends nothing on that.
-__device__ __forceinline__ void mx_blocks(const uint4 a, const uint4 b, uint32_t s, uint32_t* w) {
-    const uint32_t sa = s & 255u, sb = s >> 8 & 255u;
-    uint32_t ma = (sa + 126u) * 0x00800080u, mb = (sb + 126u) * 0x00800080u;
-    const bool large = __any_sync(0xffffffffu, max(sa, sb) > 128u);
-    if (large) {
-        ma = mx_both(sa == 255 ? 0x7FC0u : (min(sa, 128u) + 126u) << 7);
-        mb = mx_both(sb == 255 ? 0x7FC0u : (min(sb, 128u) + 126u) << 7);
-    }
-    mx_pairs(a.x, ma, w);
-    mx_pairs(a.y, ma, w + 4);
-    mx_pairs(a.z, ma, w + 8);
-    mx_pairs(a.w, ma, w + 12);
-    mx_pairs(b.x, mb, w + 16);
-    mx_pairs(b.y, mb, w + 20);
-    mx_pairs(b.z, mb, w + 24);
-    mx_pairs(b.w, mb, w + 28);
-    if (large) {
-        ma = mx_both(sa == 255 || sa <= 128 ? 0x3F80u : (sa - 1) << 7);
-        mb = mx_both(sb == 255 || sb <= 128 ? 0x3F80u : (sb - 1) << 7);
+// A block of a row, 16 bytes of codes with scale byte s, as 16 pairs: exactly the values, the factor being 2^126 times the
+// scale, 2^(s - 1).
+__device__ __forceinline__ void mx_block(const uint4 q, uint32_t m1, uint32_t* w) {
+    mx_pairs(q.x, m1, w);
+    mx_pairs(q.y, m1, w + 4);
+    mx_pairs(q.z, m1, w + 8);
+    mx_pairs(q.w, m1, w + 12);
+}
+__device__ __forceinline__ uint32_t mx_factor(uint32_t s) { return (s + 126u) * 0x00800080u; }
+// Where that has no bfloat16 (s > 128: a block whose largest magnitude is 4 or more) it is 2^127 and the rest.
+__device__ __forceinline__ void mx_block_large(const uint4 q, uint32_t s, uint32_t* w) {
+    mx_block(q, mx_both(s == 255 ? 0x7FC0u : (min(s, 128u) + 126u) << 7), w);
+    const uint32_t m2 = mx_both(s == 255 || s <= 128 ? 0x3F80u : (s - 1) << 7);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = mx_mul(w[i], ma), w[16 + i] = mx_mul(w[16 + i], mb);
-    }
+    for (int i = 0; i < 16; ++i) w[i] = mx_mul(w[i], m2);
 }
 
 __device__ __forceinline__ void mxt_tmem_st16(uint32_t taddr, const uint32_t* r) {
@@ -260,7 +250,7 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
             mbar_init(&full_bar[s], 1);
-            mbar_init(&empty_bar[s], MXT_WARPS + 1);
+            mbar_init(&empty_bar[s], MXT_WARPS / 2 + 1);
         }
         for (int s = 0; s < MXT_A; ++s) {
             mbar_init(&a_full[s], 8);
@@ -284,44 +274,62 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
     bool ok = !*abort_flag;
     if (warp < MXT_WARPS) {
         pdl_wait();                                              // (the output may still be read by the preceding kernel)
-        // ---- codes to bfloat16: a thread's row of tile `tile`, half `half` of every chunk
-        const int tile = warp >> 2 & 1, half = warp >> 3, r = threadIdx.x & 127;
+        // ---- codes to bfloat16: a thread's row of tile `tile`, every other chunk
+        const int tile = warp >> 2 & 1, turn = warp >> 3, r = threadIdx.x & 127;
         const bool here = tile < tiles;
         const int rr = (tile ? off : 0) + r;                     // the row's place in the packed tiles
-        const int codes_at = x_bytes + tile * (MX_CODES + 1024) + half * 4096 + r * 16;
-        const int scale_at = x_bytes + tile * (MX_CODES + 1024) + (rr >> 7) * 512 + mx_scale_at(rr & 127) + half * 2;
-        const uint32_t dst = tmem_a + (uint32_t)(half * 64 + tile * 32) + ((uint32_t)((warp & 3) * 32) << 16);
-        int s = 0;
-        uint32_t ph = 0, sa = 0, pa = 0;                         // place of A: 2 sa + half
-        for (int c = c_begin; c < c_end && ok; ++c) {
+        const int codes_at = x_bytes + tile * (MX_CODES + 1024) + r * 16;
+        const int scale_at = x_bytes + tile * (MX_CODES + 1024) + (rr >> 7) * 512 + mx_scale_at(rr & 127);
+        const uint32_t dst = tmem_a + (uint32_t)(turn * 128 + tile * 64) + ((uint32_t)((warp & 3) * 32) << 16);
+        int s = turn;
+        uint32_t ph = 0, pa = 0;
+        if (s >= stages) s -= stages, ph ^= 1u;
+        for (int c = c_begin + turn; c < c_end && ok; c += 2) {
             if (!mxt_wait(&full_bar[s], ph, abort_flag)) {
                 if (lane == 0) mxt_give_up(abort_flag, status);
                 ok = false;
                 break;
             }
             const unsigned char* stage = ring + s * stage_bytes;
-            const uint4 qa = *reinterpret_cast<const uint4*>(stage + codes_at), qb = *reinterpret_cast<const uint4*>(stage + codes_at + 2048);
-            const uint32_t sc = *reinterpret_cast<const uint16_t*>(stage + scale_at);
+            uint4 q[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) q[b] = *reinterpret_cast<const uint4*>(stage + codes_at + b * 2048);
+            const uint32_t sc = *reinterpret_cast<const uint32_t*>(stage + scale_at);
             __syncwarp();
             if (lane == 0) mxt_arrive(&empty_bar[s]);
+            // (a byte above 128: its top bit is set, and it is not 128 itself)
+            const bool large = __any_sync(0xffffffffu, (sc & 0x80808080u & ((sc & 0x7F7F7F7Fu) + 0x7F7F7F7Fu)) != 0);
             uint32_t v[32];
-            if (here) mx_blocks(qa, qb, sc, v);
-            if (!mxt_wait(&a_empty[2 * sa + half], pa ^ 1u, abort_flag)) {
+            auto two = [&](int b) {
+                if (!large) {
+                    mx_block(q[b], mx_factor(sc >> (8 * b) & 255u), v);
+                    mx_block(q[b + 1], mx_factor(sc >> (8 * b + 8) & 255u), v + 16);
+                } else {
+                    mx_block_large(q[b], sc >> (8 * b) & 255u, v);
+                    mx_block_large(q[b + 1], sc >> (8 * b + 8) & 255u, v + 16);
+                }
+            };
+            if (here) two(0);
+            if (!mxt_wait(&a_empty[turn], pa ^ 1u, abort_flag)) {
                 if (lane == 0) mxt_give_up(abort_flag, status);
                 ok = false;
                 break;
             }
             tc_fence_after();
             if (here) {
-                mxt_tmem_st16(dst + sa * 128u, v);
-                mxt_tmem_st16(dst + sa * 128u + 16u, v + 16);
+                mxt_tmem_st16(dst, v);
+                mxt_tmem_st16(dst + 16u, v + 16);
+                two(2);
+                mxt_tmem_st16(dst + 32u, v);
+                mxt_tmem_st16(dst + 48u, v + 16);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mxt_arrive(&a_full[2 * sa + half]);
-            if (++s == stages) { s = 0; ph ^= 1u; }
-            if (++sa == MXT_A / 2) { sa = 0; pa ^= 1u; }
+            if (lane == 0) mxt_arrive(&a_full[turn]);
+            pa ^= 1u;
+            s += 2;
+            if (s >= stages) s -= stages, ph ^= 1u;
         }
     } else if (warp == MXT_WARPS) {
         if (lane == 0) {
@@ -376,32 +384,29 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
         // ---- MMA issuer
         const uint32_t idesc = instr_desc_bf16(128, bn), ring_at = smem_u32(ring);
         int s = 0;
-        uint32_t ph = 0, sa = 0, pa = 0;
+        uint32_t ph = 0, turn = 0, pa = 0;
         for (int c = c_begin; c < c_end && ok; ++c) {
-            bool there = mxt_wait(&full_bar[s], ph, abort_flag);
-            for (int half = 0; half < 2 && there; ++half) {
-                there = mxt_wait(&a_full[2 * sa + half], pa, abort_flag);
-                if (!there) break;
-                tc_fence_after();
-                const uint64_t bdesc = smem_desc_sw128(ring_at + (uint32_t)(s * stage_bytes + half * (x_bytes / 2)));
-                if (mxt_elect()) {
-                    for (int tile = 0; tile < tiles; ++tile)
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            mxt_umma_ts(tmem_d + (uint32_t)(tile * 128), tmem_a + sa * 128u + (uint32_t)(half * 64 + tile * 32 + kk * 8),
-                                        bdesc + (uint64_t)(2 * kk), idesc, (c > c_begin || half > 0 || kk > 0) ? 1u : 0u);
-                    umma_commit(&a_empty[2 * sa + half]);
-                    if (half == 1) umma_commit(&empty_bar[s]);
-                }
-                __syncwarp();
-            }
-            if (!there) {
+            if (!mxt_wait(&full_bar[s], ph, abort_flag) || !mxt_wait(&a_full[turn], pa, abort_flag)) {
                 if (lane == 0) mxt_give_up(abort_flag, status);
                 ok = false;
                 break;
             }
+            tc_fence_after();
+            const uint64_t bdesc = smem_desc_sw128(ring_at + (uint32_t)(s * stage_bytes));
+            const uint64_t half = (uint64_t)(x_bytes / 2) >> 4;
+            if (mxt_elect()) {
+                for (int tile = 0; tile < tiles; ++tile)
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk)
+                        mxt_umma_ts(tmem_d + (uint32_t)(tile * 128), tmem_a + turn * 128u + (uint32_t)(tile * 64 + kk * 8),
+                                    bdesc + (uint64_t)(2 * (kk & 3)) + (kk >= 4 ? half : 0), idesc, (c > c_begin || kk > 0) ? 1u : 0u);
+                umma_commit(&a_empty[turn]);
+                umma_commit(&empty_bar[s]);
+            }
+            __syncwarp();
             if (++s == stages) { s = 0; ph ^= 1u; }
-            if (++sa == MXT_A / 2) { sa = 0; pa ^= 1u; }
+            turn ^= 1u;
+            pa ^= turn ^ 1u;
         }
         if (ok && mxt_elect()) umma_commit(acc_bar);
     }
