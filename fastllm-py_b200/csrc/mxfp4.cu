@@ -33,10 +33,13 @@ __device__ __forceinline__ float mx_value(uint32_t word, int j) {
 // nearest, ties to even codes, and saturates at 6.  A block with a NaN or an infinity has s = 255 and codes 0.
 //
 // Bound by memory: k (2 or 4) bytes of a row in, 17 k / 32 out.  A warp takes 8 rows of a chunk, 4 lanes a row: a lane's 8
-// elements of each of the four blocks are loaded before the first is used, and a warp's codes of a block are 128 bytes side
-// by side.
-template <typename T> __device__ __forceinline__ void mx_load8(const T* src, int n, bool vec, float (&v)[8]) {
-    if (vec && n >= 8) {
+// elements of each of the four blocks are loaded before the first is used.  The rows are two neighbours in each quarter of the
+// tile: their scales are 32 bytes side by side, as two rows' codes of a block are, so that every 32-byte sector is written whole.
+// Rows that do not begin on 16 bytes are read an element a lane instead, a block a warp.
+__device__ __forceinline__ int mx_row_of(int unit, int i) { return 2 * unit + (i & 1) + 32 * (i >> 1); }      // unit 0 .. 15, i 0 .. 7
+
+template <typename T> __device__ __forceinline__ void mx_load8(const T* src, int n, float (&v)[8]) {           // zeros behind n
+    if (n >= 8) {
         if (sizeof(T) == 2) {
             const uint4 r = *reinterpret_cast<const uint4*>(src);
             const uint32_t w[4] = {r.x, r.y, r.z, r.w};
@@ -54,52 +57,87 @@ template <typename T> __device__ __forceinline__ void mx_load8(const T* src, int
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32<T>(src[i]) : 0.0f;
 }
+__device__ __forceinline__ uint32_t mx_two_codes(float lo, float hi) {        // e2m1 of two values, the first in the low nibble
+    uint32_t two;
+    asm("{\n\t.reg .b8 q;\n\tcvt.rn.satfinite.e2m1x2.f32 q, %2, %1;\n\tcvt.u32.u8 %0, q;\n\t}" : "=r"(two) : "f"(lo), "f"(hi));
+    return two;
+}
+// the scale byte of a block whose largest magnitude has these bits (magnitudes compare as integers do, a NaN above all)
+__device__ __forceinline__ int mx_scale_byte(uint32_t top) {
+    const int e = (int)(top >> 23);
+    return e == 255 ? 255 : max(e - 2, 0);
+}
+__device__ __forceinline__ float mx_inverse(int s) { return __uint_as_float((uint32_t)(254 - min(s, 253)) << 23); }   // 2^(127 - s)
 
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ data, int m,
-                                                          int k, int chunks, long units, bool vec) {
+                                                          int k, int chunks, long units) {
     pdl_wait();
     pdl_trigger();
     const long unit = (long)blockIdx.x * 8 + (threadIdx.x >> 5);     // 8 rows x one chunk; 16 units fill a tile's chunk
     if (unit >= units) return;                                       // (whole warps)
     const int lane = threadIdx.x & 31, t = lane & 3;
     const int chunk = (int)(unit % chunks);
-    const long row0 = unit / chunks * 8;
-    const long row = row0 + (lane >> 2);
-    const int r = (int)(row & (MX_ROWS - 1));
-    uint8_t* dst = data + (row / MX_ROWS * chunks + chunk) * MX_CHUNK;
-    float v[4][8];
+    const long tile = unit / chunks >> 4;
+    const int u = (int)(unit / chunks & 15);
+    uint8_t* dst = data + (tile * chunks + chunk) * MX_CHUNK;
+    if (VEC) {
+        const int r = mx_row_of(u, lane >> 2);
+        const long row = tile * MX_ROWS + r;
+        float v[4][8];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        const int c = chunk * 128 + b * 32 + t * 8;
-        mx_load8(x + row * ld + c, row < m ? k - c : 0, vec, v[b]);
-    }
-    uint32_t scales = 0;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        // magnitudes compare as integers do, a NaN above all
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[b][i]) & 0x7FFFFFFFu);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = (int)(top >> 23);
-        const int s = e == 255 ? 255 : max(e - 2, 0);
-        scales |= (uint32_t)s << (8 * b);
-        const float inv = __uint_as_float((uint32_t)(254 - min(s, 253)) << 23);     // 2^(127 - s)
-        uint32_t word = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t two;                                             // element 2 i in the low nibble, 2 i + 1 in the high one
-            asm("{\n\t.reg .b8 q;\n\tcvt.rn.satfinite.e2m1x2.f32 q, %2, %1;\n\tcvt.u32.u8 %0, q;\n\t}"
-                : "=r"(two)
-                : "f"(v[b][2 * i] * inv), "f"(v[b][2 * i + 1] * inv));
-            word |= (two & 0xFu) << (4 * i) | (two >> 4) << (16 + 4 * i);
+        for (int b = 0; b < 4; ++b) {
+            const int c = chunk * 128 + b * 32 + t * 8;
+            mx_load8(x + row * ld + c, row < m ? k - c : 0, v[b]);
         }
-        if (s == 255) word = 0;
-        *reinterpret_cast<uint32_t*>(dst + b * 2048 + r * 16 + t * 4) = word;
+        uint32_t scales = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[b][i]) & 0x7FFFFFFFu);
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int s = mx_scale_byte(top);
+            scales |= (uint32_t)s << (8 * b);
+            const float inv = mx_inverse(s);
+            uint32_t word = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t two = mx_two_codes(v[b][2 * i] * inv, v[b][2 * i + 1] * inv);
+                word |= (two & 0xFu) << (4 * i) | (two >> 4) << (16 + 4 * i);
+            }
+            *reinterpret_cast<uint32_t*>(dst + b * 2048 + r * 16 + t * 4) = s == 255 ? 0 : word;
+        }
+        if (t == 0) *reinterpret_cast<uint32_t*>(dst + mx_scale_at(r)) = scales;
+        return;
     }
-    if (t == 0) *reinterpret_cast<uint32_t*>(dst + mx_scale_at(r)) = scales;
+#pragma unroll 2
+    for (int i = 0; i < 8; ++i) {
+        const int r = mx_row_of(u, i);
+        const long row = tile * MX_ROWS + r;
+        float v[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int c = chunk * 128 + b * 32 + lane;
+            v[b] = row < m && c < k ? to_f32<T>(x[row * ld + c]) : 0.0f;
+        }
+        uint32_t scales = 0, mine = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int s = mx_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7FFFFFFFu));
+            scales |= (uint32_t)s << (8 * b);
+            // the lane's code where its word has it, the eight lanes of a word added up
+            uint32_t word = s == 255 ? 0 : mx_two_codes(v[b] * mx_inverse(s), 0.0f) << (4 * ((lane & 1) * 4 + (lane >> 1 & 3)));
+            word |= __shfl_xor_sync(0xffffffffu, word, 1);
+            word |= __shfl_xor_sync(0xffffffffu, word, 2);
+            word |= __shfl_xor_sync(0xffffffffu, word, 4);
+            word = __shfl_sync(0xffffffffu, word, (lane & 3) * 8);
+            if (lane >> 2 == b) mine = word;                          // lanes 4 b .. 4 b + 3 hold the block's words
+        }
+        if (lane < 16) *reinterpret_cast<uint32_t*>(dst + (lane >> 2) * 2048 + r * 16 + (lane & 3) * 4) = mine;
+        else if (lane == 16) *reinterpret_cast<uint32_t*>(dst + mx_scale_at(r)) = scales;
+    }
 }
 
 FL_API int fl_mx_quantize(const void* x, int code, long ld, void* data, int m, int k, cudaStream_t stream) {
@@ -108,56 +146,74 @@ FL_API int fl_mx_quantize(const void* x, int code, long ld, void* data, int m, i
     if ((units + 7) / 8 > 0x7FFFFFFFl) return (int)cudaErrorInvalidValue;
     FL_DISPATCH(code, T, {
         const bool vec = (((uintptr_t)x | (uintptr_t)(ld * (long)sizeof(T))) & 15) == 0;
-        return fl_launch(mx_quantize_kernel<T>, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, stream, (const T*)x, ld,
-                         (uint8_t*)data, m, k, chunks, units, vec);
+        return fl_launch(vec ? mx_quantize_kernel<T, true> : mx_quantize_kernel<T, false>, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, stream,
+                         (const T*)x, ld, (uint8_t*)data, m, k, chunks, units);
     })
     return (int)cudaErrorInvalidValue;
 }
 
-template <typename T>
+// Back: the same division of the work; rows that do not begin on 16 bytes are written an element a lane, the words of a row
+// handed round by shuffles.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __restrict__ data, T* __restrict__ out, long ld, int m,
-                                                            int k, int chunks, long units, bool vec) {
+                                                            int k, int chunks, long units) {
     pdl_wait();
     pdl_trigger();
     const long unit = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (unit >= units) return;
     const int lane = threadIdx.x & 31, t = lane & 3;
     const int chunk = (int)(unit % chunks);
-    const long row = unit / chunks * 8 + (lane >> 2);
-    if (row >= m) return;
-    const int r = (int)(row & (MX_ROWS - 1));
-    const uint8_t* src = data + (row / MX_ROWS * chunks + chunk) * MX_CHUNK;
+    const long tile = unit / chunks >> 4;
+    const int u = (int)(unit / chunks & 15), r = mx_row_of(u, lane >> 2);
+    const uint8_t* src = data + (tile * chunks + chunk) * MX_CHUNK;
     const uint32_t scales = *reinterpret_cast<const uint32_t*>(src + mx_scale_at(r));
     uint32_t word[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) word[b] = *reinterpret_cast<const uint32_t*>(src + b * 2048 + r * 16 + t * 4);
+    if (VEC) {
+        const long row = tile * MX_ROWS + r;
+        if (row >= m) return;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        const int c = chunk * 128 + b * 32 + t * 8;
-        const float scale = mx_scale((int)(scales >> (8 * b)) & 255);
-        T v[8];
+        for (int b = 0; b < 4; ++b) {
+            const int c = chunk * 128 + b * 32 + t * 8;
+            const float scale = mx_scale((int)(scales >> (8 * b)) & 255);
+            __align__(16) T v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = from_f32<T>(mx_value(word[b], i) * scale);
-        T* dst = out + row * ld + c;
-        if (vec && c + 8 <= k) {
+            for (int i = 0; i < 8; ++i) v[i] = from_f32<T>(mx_value(word[b], i) * scale);
+            T* dst = out + row * ld + c;
+            if (c + 8 <= k) {
 #pragma unroll
-            for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(v)[i];
-        } else {
+                for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(v)[i];
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i < k) dst[i] = v[i];
+                for (int i = 0; i < 8; ++i)
+                    if (c + i < k) dst[i] = v[i];
+            }
+        }
+        return;
+    }
+    const int place = 4 * ((lane & 1) * 4 + (lane >> 1 & 3));         // of element lane % 8 in its word
+#pragma unroll 2
+    for (int i = 0; i < 8; ++i) {
+        const long row = tile * MX_ROWS + mx_row_of(u, i);
+        const uint32_t sc = __shfl_sync(0xffffffffu, scales, 4 * i);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const uint32_t code = __shfl_sync(0xffffffffu, word[b], 4 * i + (lane >> 3)) >> place;
+            const int c = chunk * 128 + b * 32 + lane;
+            if (row < m && c < k) out[row * ld + c] = from_f32<T>(mx_value(code, 0) * mx_scale((int)(sc >> (8 * b)) & 255));
         }
     }
 }
 
 FL_API int fl_mx_dequantize(const void* data, void* out, int code, long ld, int m, int k, cudaStream_t stream) {
     const int chunks = (k + 127) / 128;
-    const long units = (long)((m + 7) / 8) * chunks;
+    const long units = (long)((m + MX_ROWS - 1) / MX_ROWS) * 16 * chunks;
     if ((units + 7) / 8 > 0x7FFFFFFFl) return (int)cudaErrorInvalidValue;
     FL_DISPATCH(code, T, {
         const bool vec = (((uintptr_t)out | (uintptr_t)(ld * (long)sizeof(T))) & 15) == 0;
-        return fl_launch(mx_dequantize_kernel<T>, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, stream, (const uint8_t*)data,
-                         (T*)out, ld, m, k, chunks, units, vec);
+        return fl_launch(vec ? mx_dequantize_kernel<T, true> : mx_dequantize_kernel<T, false>, dim3((unsigned)((units + 7) / 8)), dim3(256), 0,
+                         stream, (const uint8_t*)data, (T*)out, ld, m, k, chunks, units);
     })
     return (int)cudaErrorInvalidValue;
 }
