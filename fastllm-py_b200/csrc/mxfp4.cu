@@ -27,6 +27,28 @@ __device__ __forceinline__ float mx_value(uint32_t word, int j) {
     return __uint_as_float(((code & 8u) << 28) | ((code & 7u) << 22)) * 8.507059173023462e37f;
 }
 
+__device__ __forceinline__ uint32_t mx_mul(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// A word of 8 codes as 4 pairs of bfloat16, element 2 i in the low half of w[i]: sign and magnitude of nibbles i and 4 + i where
+// a bfloat16 of exponent 2^-126 has them (the magnitudes 0 and 0.5 are subnormal), times m1.  A product with two powers of two puts
+// a nibble in both places at once.
+__device__ __forceinline__ void mx_pairs(uint32_t q, uint32_t m1, uint32_t* w) {
+    constexpr uint32_t PLACES = 0x81C081C0u, NIBBLE = 0x000F000Fu;
+    w[0] = mx_mul(((q & NIBBLE) * 0x1040u) & PLACES, m1);
+    w[1] = mx_mul(((q & (NIBBLE << 4)) * 0x104u) & PLACES, m1);
+    w[2] = mx_mul((((q >> 8) & NIBBLE) * 0x1040u) & PLACES, m1);
+    w[3] = mx_mul((q & 0x80008000u) | ((q >> 6) & 0x01C001C0u), m1);
+}
+__device__ __forceinline__ uint32_t mx_both(uint32_t h) { return h | h << 16; }
+// The factors of a block with scale byte s: m1 = 2^(s - 1), both halves alike; where that has no bfloat16 (s > 128: a block whose
+// largest magnitude is 4 or more) m1 is 2^127 and m2 the rest, else 1.
+__device__ __forceinline__ uint32_t mx_factor(uint32_t s) { return (s + 126u) * 0x00800080u; }
+__device__ __forceinline__ uint32_t mx_factor_large(uint32_t s) { return mx_both(s == 255 ? 0x7FC0u : (min(s, 128u) + 126u) << 7); }
+__device__ __forceinline__ uint32_t mx_factor_rest(uint32_t s) { return mx_both(s == 255 || s <= 128 ? 0x3F80u : (s - 1) << 7); }
+
 // ---------------------------------------------------------------- rounding
 // s = max(exponent byte of the block's largest magnitude - 2, 0): the largest then lies in [4, 8) units of S, or all are below
 // that.  x / S is exact (a product with a power of two; what underflows rounds to 0 either way); the conversion rounds to
@@ -57,10 +79,20 @@ template <typename T> __device__ __forceinline__ void mx_load8(const T* src, int
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32<T>(src[i]) : 0.0f;
 }
-__device__ __forceinline__ uint32_t mx_two_codes(float lo, float hi) {        // e2m1 of two values, the first in the low nibble
-    uint32_t two;
-    asm("{\n\t.reg .b8 q;\n\tcvt.rn.satfinite.e2m1x2.f32 q, %2, %1;\n\tcvt.u32.u8 %0, q;\n\t}" : "=r"(two) : "f"(lo), "f"(hi));
-    return two;
+__device__ __forceinline__ uint32_t mx_one_code(float v) {
+    uint32_t code;
+    asm("{\n\t.reg .b8 q;\n\tcvt.rn.satfinite.e2m1x2.f32 q, %2, %1;\n\tcvt.u32.u8 %0, q;\n\t}" : "=r"(code) : "f"(v), "f"(0.0f));
+    return code;
+}
+// a word of codes: a conversion makes a byte of two neighbouring nibbles
+__device__ __forceinline__ uint32_t mx_word(const float (&v)[8], float inv) {
+    uint32_t word;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(word)
+        : "f"(v[0] * inv), "f"(v[2] * inv), "f"(v[4] * inv), "f"(v[6] * inv), "f"(v[1] * inv), "f"(v[3] * inv), "f"(v[5] * inv), "f"(v[7] * inv));
+    return word;
 }
 // the scale byte of a block whose largest magnitude has these bits (magnitudes compare as integers do, a NaN above all)
 __device__ __forceinline__ int mx_scale_byte(uint32_t top) {
@@ -71,15 +103,14 @@ __device__ __forceinline__ float mx_inverse(int s) { return __uint_as_float((uin
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ data, int m,
-                                                          int k, int chunks, long units) {
+                                                          int k, int chunks) {
     pdl_wait();
     pdl_trigger();
-    const long unit = (long)blockIdx.x * 8 + (threadIdx.x >> 5);     // 8 rows x one chunk; 16 units fill a tile's chunk
-    if (unit >= units) return;                                       // (whole warps)
+    const int chunk = blockIdx.y * 8 + (threadIdx.x >> 5);           // a unit of 8 rows x one chunk; 16 units fill a tile's chunk
+    if (chunk >= chunks) return;                                     // (whole warps)
     const int lane = threadIdx.x & 31, t = lane & 3;
-    const int chunk = (int)(unit % chunks);
-    const long tile = unit / chunks >> 4;
-    const int u = (int)(unit / chunks & 15);
+    const long tile = blockIdx.x >> 4;
+    const int u = blockIdx.x & 15;
     uint8_t* dst = data + (tile * chunks + chunk) * MX_CHUNK;
     if (VEC) {
         const int r = mx_row_of(u, lane >> 2);
@@ -101,12 +132,7 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const T* __restrict__ 
             const int s = mx_scale_byte(top);
             scales |= (uint32_t)s << (8 * b);
             const float inv = mx_inverse(s);
-            uint32_t word = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t two = mx_two_codes(v[b][2 * i] * inv, v[b][2 * i + 1] * inv);
-                word |= (two & 0xFu) << (4 * i) | (two >> 4) << (16 + 4 * i);
-            }
+            const uint32_t word = mx_word(v[b], inv);
             *reinterpret_cast<uint32_t*>(dst + b * 2048 + r * 16 + t * 4) = s == 255 ? 0 : word;
         }
         if (t == 0) *reinterpret_cast<uint32_t*>(dst + mx_scale_at(r)) = scales;
@@ -128,7 +154,7 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const T* __restrict__ 
             const int s = mx_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7FFFFFFFu));
             scales |= (uint32_t)s << (8 * b);
             // the lane's code where its word has it, the eight lanes of a word added up
-            uint32_t word = s == 255 ? 0 : mx_two_codes(v[b] * mx_inverse(s), 0.0f) << (4 * ((lane & 1) * 4 + (lane >> 1 & 3)));
+            uint32_t word = s == 255 ? 0 : mx_one_code(v[b] * mx_inverse(s)) << (4 * ((lane & 1) * 4 + (lane >> 1 & 3)));
             word |= __shfl_xor_sync(0xffffffffu, word, 1);
             word |= __shfl_xor_sync(0xffffffffu, word, 2);
             word |= __shfl_xor_sync(0xffffffffu, word, 4);
@@ -142,12 +168,12 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const T* __restrict__ 
 
 FL_API int fl_mx_quantize(const void* x, int code, long ld, void* data, int m, int k, cudaStream_t stream) {
     const int chunks = (k + 127) / 128;
-    const long units = (long)((m + MX_ROWS - 1) / MX_ROWS) * 16 * chunks;
-    if ((units + 7) / 8 > 0x7FFFFFFFl) return (int)cudaErrorInvalidValue;
+    const dim3 grid((unsigned)((m + MX_ROWS - 1) / MX_ROWS) * 16, (chunks + 7) / 8);
+    if (grid.y > 65535) return (int)cudaErrorInvalidValue;
     FL_DISPATCH(code, T, {
         const bool vec = (((uintptr_t)x | (uintptr_t)(ld * (long)sizeof(T))) & 15) == 0;
-        return fl_launch(vec ? mx_quantize_kernel<T, true> : mx_quantize_kernel<T, false>, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, stream,
-                         (const T*)x, ld, (uint8_t*)data, m, k, chunks, units);
+        return fl_launch(vec ? mx_quantize_kernel<T, true> : mx_quantize_kernel<T, false>, grid, dim3(256), 0, stream,
+                         (const T*)x, ld, (uint8_t*)data, m, k, chunks);
     })
     return (int)cudaErrorInvalidValue;
 }
@@ -156,15 +182,14 @@ FL_API int fl_mx_quantize(const void* x, int code, long ld, void* data, int m, i
 // handed round by shuffles.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __restrict__ data, T* __restrict__ out, long ld, int m,
-                                                            int k, int chunks, long units) {
+                                                            int k, int chunks) {
     pdl_wait();
     pdl_trigger();
-    const long unit = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (unit >= units) return;
+    const int chunk = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (chunk >= chunks) return;
     const int lane = threadIdx.x & 31, t = lane & 3;
-    const int chunk = (int)(unit % chunks);
-    const long tile = unit / chunks >> 4;
-    const int u = (int)(unit / chunks & 15), r = mx_row_of(u, lane >> 2);
+    const long tile = blockIdx.x >> 4;
+    const int u = blockIdx.x & 15, r = mx_row_of(u, lane >> 2);
     const uint8_t* src = data + (tile * chunks + chunk) * MX_CHUNK;
     const uint32_t scales = *reinterpret_cast<const uint32_t*>(src + mx_scale_at(r));
     uint32_t word[4];
@@ -172,14 +197,27 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __res
     for (int b = 0; b < 4; ++b) word[b] = *reinterpret_cast<const uint32_t*>(src + b * 2048 + r * 16 + t * 4);
     if (VEC) {
         const long row = tile * MX_ROWS + r;
+        const bool large = __any_sync(0xffffffffu, (scales & 0x80808080u & ((scales & 0x7F7F7F7Fu) + 0x7F7F7F7Fu)) != 0);
         if (row >= m) return;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const int c = chunk * 128 + b * 32 + t * 8;
-            const float scale = mx_scale((int)(scales >> (8 * b)) & 255);
+            const uint32_t s = scales >> (8 * b) & 255u;
+            uint32_t w[4];                                            // in bfloat16, which has all that float has of these values
+            mx_pairs(word[b], large ? mx_factor_large(s) : mx_factor(s), w);
+            if (large)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = mx_mul(w[i], mx_factor_rest(s));
             __align__(16) T v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = from_f32<T>(mx_value(word[b], i) * scale);
+            for (int i = 0; i < 4; ++i) {
+                if (sizeof(T) == 2) {
+                    reinterpret_cast<uint32_t*>(v)[i] = w[i];
+                } else {
+                    reinterpret_cast<uint32_t*>(v)[(sizeof(T) / 2) * i] = w[i] << 16;
+                    reinterpret_cast<uint32_t*>(v)[(sizeof(T) / 2) * i + sizeof(T) / 4] = w[i] & 0xFFFF0000u;
+                }
+            }
             T* dst = out + row * ld + c;
             if (c + 8 <= k) {
 #pragma unroll
@@ -208,12 +246,12 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __res
 
 FL_API int fl_mx_dequantize(const void* data, void* out, int code, long ld, int m, int k, cudaStream_t stream) {
     const int chunks = (k + 127) / 128;
-    const long units = (long)((m + MX_ROWS - 1) / MX_ROWS) * 16 * chunks;
-    if ((units + 7) / 8 > 0x7FFFFFFFl) return (int)cudaErrorInvalidValue;
+    const dim3 grid((unsigned)((m + MX_ROWS - 1) / MX_ROWS) * 16, (chunks + 7) / 8);
+    if (grid.y > 65535) return (int)cudaErrorInvalidValue;
     FL_DISPATCH(code, T, {
         const bool vec = (((uintptr_t)out | (uintptr_t)(ld * (long)sizeof(T))) & 15) == 0;
-        return fl_launch(vec ? mx_dequantize_kernel<T, true> : mx_dequantize_kernel<T, false>, dim3((unsigned)((units + 7) / 8)), dim3(256), 0,
-                         stream, (const uint8_t*)data, (T*)out, ld, m, k, chunks, units);
+        return fl_launch(vec ? mx_dequantize_kernel<T, true> : mx_dequantize_kernel<T, false>, grid, dim3(256), 0,
+                         stream, (const uint8_t*)data, (T*)out, ld, m, k, chunks);
     })
     return (int)cudaErrorInvalidValue;
 }
@@ -224,22 +262,6 @@ FL_API int fl_mx_dequantize(const void* data, void* out, int code, long ld, int 
 // tokens its 8 columns.  Lane 4 g + q reads the 16 bytes of rows g and g + 8 of block q, so a lane has one scale for 32 codes;
 // which elements of K meet in one instruction does not matter as long as both operands agree, and a lane's 8 consecutive elements
 // of a token are the partners of one word of codes.  The warps' sums meet in shared memory and are added in order.
-__device__ __forceinline__ uint32_t mx_mul(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-// A word of 8 codes as 4 pairs of bfloat16, element 2 i in the low half of w[i]: sign and magnitude of nibbles i and 4 + i where
-// a bfloat16 of exponent 2^-126 has them (the magnitudes 0 and 0.5 are subnormal), times m1.  A product with two powers of two puts
-// a nibble in both places at once.
-__device__ __forceinline__ void mx_pairs(uint32_t q, uint32_t m1, uint32_t* w) {
-    constexpr uint32_t PLACES = 0x81C081C0u, NIBBLE = 0x000F000Fu;
-    w[0] = mx_mul(((q & NIBBLE) * 0x1040u) & PLACES, m1);
-    w[1] = mx_mul(((q & (NIBBLE << 4)) * 0x104u) & PLACES, m1);
-    w[2] = mx_mul((((q >> 8) & NIBBLE) * 0x1040u) & PLACES, m1);
-    w[3] = mx_mul((q & 0x80008000u) | ((q >> 6) & 0x01C001C0u), m1);
-}
-__device__ __forceinline__ uint32_t mx_both(uint32_t h) { return h | h << 16; }
 __device__ __forceinline__ void mx_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
