@@ -40,7 +40,7 @@ __device__ __forceinline__ void mx_pairs(uint32_t q, uint32_t m1, uint32_t* w) {
     w[0] = mx_mul(((q & NIBBLE) * 0x1040u) & PLACES, m1);
     w[1] = mx_mul(((q & (NIBBLE << 4)) * 0x104u) & PLACES, m1);
     w[2] = mx_mul((((q >> 8) & NIBBLE) * 0x1040u) & PLACES, m1);
-    w[3] = mx_mul((q & 0x80008000u) | ((q >> 6) & 0x01C001C0u), m1);
+    w[3] = mx_mul((((q >> 8) & (NIBBLE << 4)) * 0x104u) & PLACES, m1);
 }
 __device__ __forceinline__ uint32_t mx_both(uint32_t h) { return h | h << 16; }
 // The factors of a block with scale byte s: m1 = 2^(s - 1), both halves alike; where that has no bfloat16 (s > 128: a block whose
@@ -257,11 +257,15 @@ FL_API int fl_mx_dequantize(const void* data, void* out, int code, long ld, int 
 }
 
 // ---------------------------------------------------------------- products of few rows
-// out[t, f] = sum_k x[t, k] W[f, k] for up to 16 tokens, or of a gated unit act(gate, up) of features f and n + f: reading W
-// is the time.  A warp takes 16 (MT = 2: 2 x 16) rows of W and every WARPS-th chunk of K; the rows are the 16 of m16n8k16 and the
-// tokens its 8 columns.  Lane 4 g + q reads the 16 bytes of rows g and g + 8 of block q, so a lane has one scale for 32 codes;
-// which elements of K meet in one instruction does not matter as long as both operands agree, and a lane's 8 consecutive elements
-// of a token are the partners of one word of codes.  The warps' sums meet in shared memory and are added in order.
+// out[t, f] = sum_k x[t, k] W[f, k] for up to 8 tokens, or of a gated unit act(gate, up) of features f and n + f: reading W is the
+// time, and turning its codes into bfloat16 next to it.  A CTA takes 2 x 16 rows of W (of a gated unit 16 gate rows and the 16 up
+// rows of the same features), a warp of it every WARPS-th chunk of K.  The rows are the 16 of m16n8k16 and the tokens its 8 columns.
+// Lane 4 g + q reads the 16 bytes of rows g and g + 8 of block q, so a lane has one scale for 32 codes; which elements of K meet in
+// one instruction does not matter as long as both operands agree, and a lane's 8 consecutive elements of a token are the partners of
+// one word of codes.  The warps' sums meet in shared memory and are added in order.
+//
+// LB warps fit an SM.  With 24 a warp has registers for one chunk: its rows are loaded anew for the next one as soon as their codes
+// have been read, and its tokens at the end.  With 16 the next codes are on their way during the whole chunk.
 __device__ __forceinline__ void mx_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -277,18 +281,18 @@ __device__ __forceinline__ uint4 mx_tokens8(const bf16* row, int c, int k) {
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-template <typename TO, int WARPS, int MT, int NT, bool GATED>
-__global__ void __launch_bounds__(WARPS * 32, (NT == 1 ? 24 : 16) / WARPS)
+template <typename TO, int WARPS, bool GATED, int LB>
+__global__ void __launch_bounds__(WARPS * 32, LB / WARPS)
 mx_few_kernel(const bf16* __restrict__ x, long ldx, const uint8_t* __restrict__ w, TO* __restrict__ out, long ldo, int m, int n, int k,
               bool constant_w, FlGate act) {
-    static_assert(!GATED || MT == 2, "a gated unit's two rows are a warp's two tiles");
-    constexpr int ROWS = GATED ? 16 : 16 * MT;                       // output features of a block
-    __shared__ float red[WARPS][NT * 8][MT * 16 + 1];
+    constexpr int MT = 2, ROWS = GATED ? 16 : 32;                    // tiles of 16 rows, output features of a CTA
+    constexpr bool EARLY = LB <= 16;
+    __shared__ float red[WARPS][8][MT * 16 + 1];
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int chunks = (k + 127) / 128;
     const int f0 = blockIdx.x * ROWS;
-    // codes of block q of a row, from the warp's first chunk on (a row that does not exist: of the last one; not stored)
+    // codes of block q of a row, of the warp's next chunk (a row that does not exist: of the last one; not stored)
     const uint8_t* src[MT][2];
     int sc_at[MT][2];                                                // from there to the block's scale
 #pragma unroll
@@ -298,146 +302,136 @@ mx_few_kernel(const bf16* __restrict__ x, long ldx, const uint8_t* __restrict__ 
             const int f = min(f0 + (GATED ? 0 : 16 * t) + 8 * h + g, n - 1);
             const long row = (GATED ? (long)t * n : 0) + f;
             const int r = (int)(row & (MX_ROWS - 1));
-            src[t][h] = w + (row / MX_ROWS * chunks + min(warp, chunks - 1)) * (long)MX_CHUNK + q * 2048 + r * 16;
+            src[t][h] = w + (row / MX_ROWS * chunks + warp) * (long)MX_CHUNK + q * 2048 + r * 16;
             sc_at[t][h] = (int)mx_scale_at(r) + q - (q * 2048 + r * 16);
         }
-    const bf16* token[NT];                                           // (likewise)
+    uint4 z[MT][2];
+    uint32_t s[MT][2];
+    auto fetch = [&](int t) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) token[j] = x + (long)min(j * 8 + g, m - 1) * ldx + q * 32;
-    uint4 codes[MT][2];
-    uint32_t scale[MT][2];
-    auto fetch = [&]() {
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                codes[t][h] = *reinterpret_cast<const uint4*>(src[t][h]);
-                scale[t][h] = src[t][h][sc_at[t][h]];
-            }
+        for (int h = 0; h < 2; ++h) {
+            z[t][h] = *reinterpret_cast<const uint4*>(src[t][h]);
+            s[t][h] = src[t][h][sc_at[t][h]];
+            src[t][h] += WARPS * MX_CHUNK;
+        }
+    };
+    const bf16* token = x + (long)min(g, m - 1) * ldx;               // (likewise)
+    uint4 xs[4];
+    auto fetch_x = [&](int c, int e) {                               // 8 elements; zeros behind k
+        const bf16* at = token + c * 128 + q * 32 + e * 8;
+        if (c * 128 + 128 <= k) xs[e] = *reinterpret_cast<const uint4*>(at);       // (the same in all lanes)
+        else xs[e] = mx_tokens8(token, c * 128 + q * 32 + e * 8, k);
     };
     if (!constant_w) pdl_wait();
-    fetch();
+    if (warp < chunks)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) fetch(t);
     if (constant_w) pdl_wait();
-    float acc[MT][NT][4] = {};
+    if (!EARLY && warp < chunks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) fetch_x(warp, e);
+    float acc[MT][4] = {};
 #pragma unroll 1
     for (int c = warp; c < chunks; c += WARPS) {
-        uint4 now[MT][2];
-        uint32_t m1[MT][2], most = 0;
+        const bool more = c + WARPS < chunks;
+        uint4 y[MT][2];
+        uint32_t sy[MT][2], most = 0;
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                now[t][h] = codes[t][h];
-                m1[t][h] = scale[t][h];
-                most = max(most, m1[t][h]);
+                y[t][h] = z[t][h];
+                sy[t][h] = s[t][h];
+                most = max(most, sy[t][h]);
             }
-        uint4 xs[NT][4];
+        if (EARLY) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            if (c * 128 + 128 <= k) {
+            for (int e = 0; e < 4; ++e) fetch_x(c, e);
+            if (more)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) xs[j][i] = *reinterpret_cast<const uint4*>(token[j] + c * 128 + i * 8);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) xs[j][i] = mx_tokens8(token[j] - q * 32, c * 128 + q * 32 + i * 8, k);
-            }
+                for (int t = 0; t < MT; ++t) fetch(t);
         }
-        if (c + WARPS < chunks) {
-#pragma unroll
-            for (int t = 0; t < MT; ++t) src[t][0] += WARPS * MX_CHUNK, src[t][1] += WARPS * MX_CHUNK;
-            fetch();
-        }
-        // Multiplied by 2^(s - 1); where that has no bfloat16 (s > 128: a block whose largest magnitude is 4 or more) by 2^127 and
-        // by the rest.
         if (!__any_sync(0xffffffffu, most > 128u)) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                m1[t][0] = (m1[t][0] + 126u) * 0x00800080u, m1[t][1] = (m1[t][1] + 126u) * 0x00800080u;
+                const uint32_t m1[2] = {mx_factor(sy[t][0]), mx_factor(sy[t][1])};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int e = 0; e < 4; ++e) {
                     uint32_t v[2][4];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) mx_pairs(i == 0 ? now[t][h].x : i == 1 ? now[t][h].y : i == 2 ? now[t][h].z : now[t][h].w, m1[t][h], v[h]);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        mx_mma(acc[t][j], v[0][0], v[1][0], v[0][1], v[1][1], xs[j][i].x, xs[j][i].y);
-                        mx_mma(acc[t][j], v[0][2], v[1][2], v[0][3], v[1][3], xs[j][i].z, xs[j][i].w);
-                    }
+                    for (int h = 0; h < 2; ++h) mx_pairs(e == 0 ? y[t][h].x : e == 1 ? y[t][h].y : e == 2 ? y[t][h].z : y[t][h].w, m1[h], v[h]);
+                    mx_mma(acc[t], v[0][0], v[1][0], v[0][1], v[1][1], xs[e].x, xs[e].y);
+                    mx_mma(acc[t], v[0][2], v[1][2], v[0][3], v[1][3], xs[e].z, xs[e].w);
                 }
+                if (!EARLY && more) fetch(t);
             }
-        } else {
+        } else {                                                     // some block's scale takes two factors
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                uint32_t m2[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t s = m1[t][h];
-                    m1[t][h] = mx_both(s == 255 ? 0x7FC0u : (min(s, 128u) + 126u) << 7);
-                    m2[h] = mx_both(s == 255 || s <= 128 ? 0x3F80u : (s - 1) << 7);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int e = 0; e < 4; ++e) {
                     uint32_t v[2][4];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        mx_pairs(i == 0 ? now[t][h].x : i == 1 ? now[t][h].y : i == 2 ? now[t][h].z : now[t][h].w, m1[t][h], v[h]);
+                        mx_pairs(e == 0 ? y[t][h].x : e == 1 ? y[t][h].y : e == 2 ? y[t][h].z : y[t][h].w, mx_factor_large(sy[t][h]), v[h]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[h][e] = mx_mul(v[h][e], m2[h]);
+                        for (int j = 0; j < 4; ++j) v[h][j] = mx_mul(v[h][j], mx_factor_rest(sy[t][h]));
                     }
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        mx_mma(acc[t][j], v[0][0], v[1][0], v[0][1], v[1][1], xs[j][i].x, xs[j][i].y);
-                        mx_mma(acc[t][j], v[0][2], v[1][2], v[0][3], v[1][3], xs[j][i].z, xs[j][i].w);
-                    }
+                    mx_mma(acc[t], v[0][0], v[1][0], v[0][1], v[1][1], xs[e].x, xs[e].y);
+                    mx_mma(acc[t], v[0][2], v[1][2], v[0][3], v[1][3], xs[e].z, xs[e].w);
                 }
+                if (!EARLY && more) fetch(t);
             }
         }
+        if (!EARLY && more)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) fetch_x(c + WARPS, e);
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) red[warp][j * 8 + 2 * q + (e & 1)][t * 16 + g + 8 * (e >> 1)] = acc[t][j][e];
+        for (int e = 0; e < 4; ++e) red[warp][2 * q + (e & 1)][t * 16 + g + 8 * (e >> 1)] = acc[t][e];
     __syncthreads();
     for (int i = threadIdx.x; i < ROWS * m; i += WARPS * 32) {
         const int t = i / ROWS, f = i % ROWS;
         if (f0 + f >= n) continue;
         float v = 0.0f, u = 1.0f;
 #pragma unroll
-        for (int s = 0; s < WARPS; ++s) v += red[s][t][f];
+        for (int j = 0; j < WARPS; ++j) v += red[j][t][f];
         if (GATED) {
             u = 0.0f;
 #pragma unroll
-            for (int s = 0; s < WARPS; ++s) u += red[s][t][(MT - 1) * 16 + f];
+            for (int j = 0; j < WARPS; ++j) u += red[j][t][(MT - 1) * 16 + f];
         }
         out[(long)t * ldo + f0 + f] = from_f32<TO>(act.act == FL_ACT_NONE ? v : fl_gated(v, u, act));
     }
 }
 
-template <typename TO, int WARPS, int NT>
-static int mx_launch_few(const bf16* x, long ldx, const uint8_t* w, TO* out, long ldo, int m, int n, int k, bool gated, bool constant_w,
+template <typename TO, int WARPS, bool GATED, int LB>
+static int mx_launch_few(const bf16* x, long ldx, const uint8_t* w, TO* out, long ldo, int m, int n, int k, bool constant_w,
                          FlGate act, cudaStream_t stream) {
-    const dim3 block(WARPS * 32);
-    if (gated)
-        return fl_launch(mx_few_kernel<TO, WARPS, 2, NT, true>, dim3((n + 15) / 16), block, 0, stream, x, ldx, w, out, ldo, m, n, k, constant_w, act);
-    if (n >= 8192)
-        return fl_launch(mx_few_kernel<TO, WARPS, 2, NT, false>, dim3((n + 31) / 32), block, 0, stream, x, ldx, w, out, ldo, m, n, k, constant_w, act);
-    return fl_launch(mx_few_kernel<TO, WARPS, 1, NT, false>, dim3((n + 15) / 16), block, 0, stream, x, ldx, w, out, ldo, m, n, k, constant_w, act);
+    constexpr int ROWS = GATED ? 16 : 32;
+    return fl_launch(mx_few_kernel<TO, WARPS, GATED, LB>, dim3((n + ROWS - 1) / ROWS), dim3(WARPS * 32), 0, stream, x, ldx, w, out, ldo, m, n, k,
+                     constant_w, act);
 }
 
-// x: up to 16 bfloat16 rows with `ldx` elements between them (a multiple of 8, from 16 bytes on).  n: output features (gated: half
+// x: up to 8 bfloat16 rows with `ldx` elements between them (a multiple of 8, from 16 bytes on).  n: output features (gated: half
 // of w's rows).  act: an FlAct or FL_ACT_NONE; a product that is not gated has f(v, 1).  constant_w: no kernel before this one
 // in the stream writes w, so its first bytes may be read while that one still runs.
 FL_API int fl_mx_few(const void* x, long ldx, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int gated,
-                     int act, float p0, float p1, int constant_w, cudaStream_t stream) {
+                     int act, float p0, float p1, int constant_w, int num_sms, cudaStream_t stream) {
     const FlGate gate = {act, p0, p1};
-    if (m > 16) return (int)cudaErrorInvalidValue;
+    if (m > 8) return (int)cudaErrorInvalidValue;
+    // Warps of a CTA: as many as keep an SM's 24 (or 16) busy with the CTAs that there are.  One token, 4096 -> 12288: 13.6 us with 16
+    // warps, 10.2 with 8, 16.6 with 4; 11008 -> 4096: 9.5, 20.7 and 24.4; 4096 -> 102400: 98, 65 and 60.
+    const int ctas = gated ? (n + 15) / 16 : (n + 31) / 32;
     FL_DISPATCH(out_code, TO, {
-        const int warps = getenv("MXW") ? atoi(getenv("MXW")) : 8;
-        if (warps == 4 && m <= 8) return mx_launch_few<TO, 4, 1>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, gated != 0, constant_w != 0, gate, stream);
-        if (m <= 8) return mx_launch_few<TO, 8, 1>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, gated != 0, constant_w != 0, gate, stream);
-        return mx_launch_few<TO, 8, 2>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, gated != 0, constant_w != 0, gate, stream);
+#define MX_FEW(WARPS, LB)                                                                                                              \
+    return gated ? mx_launch_few<TO, WARPS, true, LB>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, constant_w != 0, gate, stream) \
+                 : mx_launch_few<TO, WARPS, false, LB>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, constant_w != 0, gate, stream)
+        if (ctas <= num_sms) MX_FEW(16, 16);
+        if (ctas <= 3 * num_sms) MX_FEW(8, 24);
+        MX_FEW(4, 24);
     })
     return (int)cudaErrorInvalidValue;
 }

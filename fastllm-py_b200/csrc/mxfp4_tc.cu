@@ -44,22 +44,24 @@ __device__ __forceinline__ void mx_pairs(uint32_t q, uint32_t m1, uint32_t* w) {
     w[0] = mx_mul(((q & NIBBLE) * 0x1040u) & PLACES, m1);
     w[1] = mx_mul(((q & (NIBBLE << 4)) * 0x104u) & PLACES, m1);
     w[2] = mx_mul((((q >> 8) & NIBBLE) * 0x1040u) & PLACES, m1);
-    w[3] = mx_mul((q & 0x80008000u) | ((q >> 6) & 0x01C001C0u), m1);
+    w[3] = mx_mul((((q >> 8) & (NIBBLE << 4)) * 0x104u) & PLACES, m1);
 }
 __device__ __forceinline__ uint32_t mx_both(uint32_t h) { return h | h << 16; }
-// A block of a row, 16 bytes of codes with scale byte s, as 16 pairs: exactly the values, the factor being 2^126 times the
-// scale, 2^(s - 1).
+// The factors of a block with scale byte s: m1 = 2^(s - 1), both halves alike; where that has no bfloat16 (s > 128: a block whose
+// largest magnitude is 4 or more) m1 is 2^127 and the rest a second factor, else 1.
+__device__ __forceinline__ uint32_t mx_factor(uint32_t s) { return (s + 126u) * 0x00800080u; }
+__device__ __forceinline__ uint32_t mx_factor_large(uint32_t s) { return mx_both(s == 255 ? 0x7FC0u : (min(s, 128u) + 126u) << 7); }
+__device__ __forceinline__ uint32_t mx_factor_rest(uint32_t s) { return mx_both(s == 255 || s <= 128 ? 0x3F80u : (s - 1) << 7); }
+// A block of a row, 16 bytes of codes with scale byte s, as 16 pairs: exactly the values.
 __device__ __forceinline__ void mx_block(const uint4 q, uint32_t m1, uint32_t* w) {
     mx_pairs(q.x, m1, w);
     mx_pairs(q.y, m1, w + 4);
     mx_pairs(q.z, m1, w + 8);
     mx_pairs(q.w, m1, w + 12);
 }
-__device__ __forceinline__ uint32_t mx_factor(uint32_t s) { return (s + 126u) * 0x00800080u; }
-// Where that has no bfloat16 (s > 128: a block whose largest magnitude is 4 or more) it is 2^127 and the rest.
 __device__ __forceinline__ void mx_block_large(const uint4 q, uint32_t s, uint32_t* w) {
-    mx_block(q, mx_both(s == 255 ? 0x7FC0u : (min(s, 128u) + 126u) << 7), w);
-    const uint32_t m2 = mx_both(s == 255 || s <= 128 ? 0x3F80u : (s - 1) << 7);
+    mx_block(q, mx_factor_large(s), w);
+    const uint32_t m2 = mx_factor_rest(s);
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = mx_mul(w[i], m2);
 }
@@ -98,7 +100,7 @@ __device__ __forceinline__ bool mxt_wait(uint64_t* bar, uint32_t parity, volatil
     if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag) ? 1u : 0u;
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
-// Tokens t, t + MXT_WARPS, .. of the float sums [token][2 x 128 rows], added up over the cluster's CTAs in rank order, through the
+// Tokens t, t + STEP, .. of the float sums [token][PITCH] (FEAT features, of a gated unit then their up values), added up over the cluster's CTAs in rank order, through the
 // activation and out; `n`: how many features there are from the tile's first on.
 template <int V> struct MxtVec { float v[V]; };
 template <int V> __device__ __forceinline__ MxtVec<V> mxt_get(const float* sums, int ranks, int rank) {
@@ -108,7 +110,8 @@ template <int V> __device__ __forceinline__ MxtVec<V> mxt_get(const float* sums,
             const float4 x = *reinterpret_cast<const float4*>(sums);
             r.v[V > 3 ? 3 : 0] = x.w, r.v[V > 2 ? 2 : 0] = x.z, r.v[V > 1 ? 1 : 0] = x.y, r.v[0] = x.x;
         } else {
-            r.v[0] = *sums;
+#pragma unroll
+            for (int i = 0; i < V; ++i) r.v[i] = sums[i];
         }
         return r;
     }
@@ -119,20 +122,22 @@ template <int V> __device__ __forceinline__ MxtVec<V> mxt_get(const float* sums,
                      : "=f"(r.v[0]), "=f"(r.v[V > 1 ? 1 : 0]), "=f"(r.v[V > 2 ? 2 : 0]), "=f"(r.v[V > 3 ? 3 : 0])
                      : "r"(at)
                      : "memory");
+    else if (V == 2)
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(r.v[0]), "=f"(r.v[V > 1 ? 1 : 0]) : "r"(at) : "memory");
     else
         asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r.v[0]) : "r"(at) : "memory");
     return r;
 }
-template <typename TO, bool GATED, int V>
+template <typename TO, bool GATED, int FEAT, int PITCH, int V, int STEP>
 __device__ __forceinline__ void mxt_rows(const float* sums, int t, int last, int ranks, TO* out, long ldo, int n, const FlGate act) {
-    constexpr int PARTS = (GATED ? 4 : 8) / V;         // steps of 32 V features
+    constexpr int PARTS = FEAT / (32 * V);                            // steps of 32 V features
     const int f0 = (threadIdx.x & 31) * V;
 #pragma unroll 2
-    for (; t < last; t += MXT_WARPS) {
+    for (; t < last; t += STEP) {
         float g[PARTS * V], u[PARTS * V];
 #pragma unroll
         for (int i = 0; i < PARTS * V; ++i) g[i] = 0.0f, u[i] = GATED ? 0.0f : 1.0f;
-        const float* row = sums + t * MXT_PITCH + f0;
+        const float* row = sums + t * PITCH + f0;
 #pragma unroll 4
         for (int q = 0; q < ranks; ++q)
 #pragma unroll
@@ -141,7 +146,7 @@ __device__ __forceinline__ void mxt_rows(const float* sums, int t, int last, int
 #pragma unroll
                 for (int i = 0; i < V; ++i) g[p * V + i] += x.v[i];
                 if (GATED) {
-                    const MxtVec<V> y = mxt_get<V>(row + 128 + p * 32 * V, ranks, q);
+                    const MxtVec<V> y = mxt_get<V>(row + FEAT + p * 32 * V, ranks, q);
 #pragma unroll
                     for (int i = 0; i < V; ++i) u[p * V + i] += y.v[i];
                 }
@@ -154,9 +159,11 @@ __device__ __forceinline__ void mxt_rows(const float* sums, int t, int last, int
             __align__(16) TO o[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) o[i] = from_f32<TO>(g[p * V + i]);
-            if (V == 1) dst[p * 32] = o[0];
-            else if (sizeof(TO) == 2) *reinterpret_cast<uint2*>(dst + p * 128) = *reinterpret_cast<const uint2*>(o);
-            else *reinterpret_cast<uint4*>(dst + p * 128) = *reinterpret_cast<const uint4*>(o);
+            TO* d = dst + p * 32 * V;
+            if (V == 1) *d = o[0];
+            else if (V * sizeof(TO) == 4) *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(o);
+            else if (V * sizeof(TO) == 8) *reinterpret_cast<uint2*>(d) = *reinterpret_cast<const uint2*>(o);
+            else *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(o);
         }
     }
 }
@@ -168,9 +175,36 @@ __device__ __forceinline__ void mxt_give_up(volatile int* abort_flag, int* statu
     }
 }
 
-// What both kernels end with, by the whole CTA: the accumulators (valid where `any`, else zero) as float sums [token][2 x 128
-// rows] in shared memory, where the ring was (every copy has been read by an MMA that is done), and this CTA's share of the tokens from all of the cluster's.
-// `ok`: of the first MXT_WARPS warps, whether the accumulators may be waited for.  Leaves with the cluster's sums no longer needed.
+// The end of a CTA whose sums of `rows` tokens are written, by all its threads: its share of the tokens from all of the cluster's
+// CTAs, by its first WARPS warps.  Leaves with the cluster's sums no longer needed.
+template <typename TO, bool GATED, int FEAT, int PITCH, int WARPS>
+__device__ __forceinline__ void mxt_join(const float* sums, volatile int* abort_flag, int rows, int ranks, int rank, TO* __restrict__ out,
+                                         long ldo, int f0, int n, const FlGate act) {
+    const int warp = mxt_warp();
+    __syncwarp();
+    tc_fence_before();
+    if (ranks > 1) cluster_sync_all();
+    else __syncthreads();
+    tc_fence_after();
+    // (a CTA of the cluster that gave up leaves its sums as they are: the status word tells that the results are not valid)
+    if (warp < WARPS && !*abort_flag) {
+        const int share = (rows + ranks - 1) / ranks, first = rank * share, last = min(rows, first + share);
+        constexpr int V = FEAT >= 128 ? 4 : 2;
+        out += f0;
+        // a warp takes a token: V features a lane and 32 V a step, or single ones side by side where rows are not aligned
+        if ((((uintptr_t)out | (uintptr_t)(ldo * (long)sizeof(TO))) & (V * sizeof(TO) - 1)) == 0 && (n & (V - 1)) == 0)
+            mxt_rows<TO, GATED, FEAT, PITCH, V, WARPS>(sums, first + warp, last, ranks, out, ldo, n - f0, act);
+        else
+            mxt_rows<TO, GATED, FEAT, PITCH, 1, WARPS>(sums, first + warp, last, ranks, out, ldo, n - f0, act);
+    }
+    __syncwarp();
+    if (ranks > 1) cluster_sync_all();                                // the others may still read this CTA's sums
+    else __syncthreads();
+}
+
+// What the kernels with accumulators in tensor memory end with, by the whole CTA: the accumulators (valid where `any`, else zero)
+// as float sums [token][2 x 128 rows] in shared memory, where the ring was (every copy has been read by an MMA that is done), then
+// mxt_join.  `ok`: of the first MXT_WARPS warps, whether the accumulators may be waited for.
 template <typename TO, bool GATED>
 __device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, uint64_t* acc_bar, volatile int* abort_flag, int* status, bool ok,
                                            bool any, int rows, int ranks, int rank, TO* __restrict__ out, long ldo, int f0, int n,
@@ -194,30 +228,77 @@ __device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, uint64_
             }
         }
     }
-    __syncwarp();
-    tc_fence_before();
-    if (ranks > 1) cluster_sync_all();
-    else __syncthreads();
-    tc_fence_after();
-    // (a CTA of the cluster that gave up leaves its sums as they are: the status word tells that the results are not valid)
-    if (warp < MXT_WARPS && !*abort_flag) {
-        const int share = (rows + ranks - 1) / ranks, first = rank * share, last = min(rows, first + share);
-        out += f0;
-        // a warp takes a token: four features a lane and 128 a step, or single ones side by side where rows are not aligned
-        if ((((uintptr_t)out | (uintptr_t)(ldo * (long)sizeof(TO))) & (4 * sizeof(TO) - 1)) == 0 && (n & 3) == 0)
-            mxt_rows<TO, GATED, 4>(sums, first + warp, last, ranks, out, ldo, n - f0, act);
-        else
-            mxt_rows<TO, GATED, 1>(sums, first + warp, last, ranks, out, ldo, n - f0, act);
-    }
-    __syncwarp();
-    if (ranks > 1) cluster_sync_all();                                // the others may still read this CTA's sums
-    else __syncthreads();
+    mxt_join<TO, GATED, GATED ? 128 : 256, MXT_PITCH, MXT_WARPS>(sums, abort_flag, rows, ranks, rank, out, ldo, f0, n, act);
 }
 
 __device__ __forceinline__ void mxt_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
                  "r"(bytes), "r"(smem_u32(bar))
                  : "memory");
+}
+
+// The copies of a CTA's chunks c_begin .. c_end - 1, by one thread; returns how many stages were sent for.  A stage: bn x 128 elements
+// of the tokens as two boxes, then the row tiles, each four pieces of codes PIECE bytes apart and the scales of the one or two packed
+// tiles that its rows lie in.  Tile 0 begins with row f0 of W, tile 1 (if tiles is 2) with row row1.
+template <int PIECE>
+__device__ __forceinline__ int mxt_produce(const CUtensorMap& map_x, const uint8_t* __restrict__ w, unsigned char* ring, uint64_t* full_bar,
+                                           uint64_t* empty_bar, int stages, int stage_bytes, int bn, int t0, int n, int chunks, int f0, long row1,
+                                           int tiles, int c_begin, int c_end, bool constant_w, bool ok, volatile int* abort_flag, int* status) {
+    constexpr int TILE = 4 * PIECE + 1024;
+    const int off = (int)(row1 & (MX_ROWS - 1)), x_bytes = bn * 256;
+    const long tile_bytes = (long)chunks * MX_CHUNK;
+    const uint8_t* src0 = w + (long)(f0 / MX_ROWS) * tile_bytes;
+    const uint8_t* src1 = w + row1 / MX_ROWS * tile_bytes;
+    const bool second = off != 0 && (row1 / MX_ROWS + 1) * MX_ROWS < 2l * n;             // (only up rows straddle)
+    const uint32_t w_bytes = MX_CHUNK + (tiles < 2 ? 0 : off == 0 ? MX_CHUNK : 4 * (MX_ROWS - off) * 16 + 512 + (second ? 4 * off * 16 + 512 : 0));
+    auto send_tile = [&](unsigned char* dst, const uint8_t* src, uint64_t* bar) {
+        if (PIECE == 2048) {
+            mxt_copy(dst, src, MX_CHUNK, bar);
+        } else {
+            for (int b = 0; b < 4; ++b) mxt_copy(dst + b * PIECE, src + b * 2048, 2048, bar);
+            mxt_copy(dst + 4 * PIECE, src + MX_CODES, 512, bar);
+        }
+    };
+    auto send_w = [&](int s, int c) {
+        unsigned char* dst = ring + s * stage_bytes + x_bytes;
+        mbar_expect_tx(&full_bar[s], (uint32_t)x_bytes + w_bytes);
+        send_tile(dst, src0 + (long)c * MX_CHUNK, &full_bar[s]);
+        if (tiles < 2) return;
+        dst += TILE;
+        const uint8_t* src = src1 + (long)c * MX_CHUNK;
+        if (off == 0) {
+            send_tile(dst, src, &full_bar[s]);
+            return;
+        }
+        for (int b = 0; b < 4; ++b) mxt_copy(dst + b * PIECE, src + b * 2048 + off * 16, (uint32_t)(MX_ROWS - off) * 16, &full_bar[s]);
+        mxt_copy(dst + 4 * PIECE, src + MX_CODES, 512, &full_bar[s]);
+        if (!second) return;
+        src += tile_bytes;
+        for (int b = 0; b < 4; ++b) mxt_copy(dst + b * PIECE + (MX_ROWS - off) * 16, src + b * 2048, (uint32_t)off * 16, &full_bar[s]);
+        mxt_copy(dst + 4 * PIECE + 512, src + MX_CODES, 512, &full_bar[s]);
+    };
+    auto send_x = [&](int s, int c) {
+        tma_load_2d(ring + s * stage_bytes, &map_x, &full_bar[s], c * 128, t0);
+        tma_load_2d(ring + s * stage_bytes + x_bytes / 2, &map_x, &full_bar[s], c * 128 + 64, t0);
+    };
+    // a constant W's first stages are sent for before the preceding kernel is waited for
+    const int ahead = constant_w && ok ? max(0, min(stages, c_end - c_begin)) : 0;
+    for (int i = 0; i < ahead; ++i) send_w(i, c_begin + i);
+    pdl_wait();
+    for (int i = 0; i < ahead; ++i) send_x(i, c_begin + i);
+    int issued = ahead, s = issued % stages;
+    uint32_t ph = (uint32_t)(issued / stages) & 1u;
+    for (int c = c_begin + issued; c < c_end && ok; ++c) {
+        if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag)) {
+            mxt_give_up(abort_flag, status);
+            break;
+        }
+        send_w(s, c);
+        send_x(s, c);
+        ++issued;
+        if (++s == stages) { s = 0; ph ^= 1u; }
+    }
+    return issued;
 }
 
 // grid: ranks of a cluster x token tiles x row tiles (pairs of them).  bn: tokens of a tile, a multiple of 16.  A stage is bn x 128
@@ -334,51 +415,8 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
     } else if (warp == MXT_WARPS) {
         if (lane == 0) {
             // ---- producer
-            const long tile_bytes = (long)chunks * MX_CHUNK;
-            const uint8_t* src0 = w + (long)(f0 / MX_ROWS) * tile_bytes;
-            const uint8_t* src1 = w + row1 / MX_ROWS * tile_bytes;
-            const bool second = off != 0 && (row1 / MX_ROWS + 1) * MX_ROWS < 2l * n;         // (only up rows straddle)
-            const uint32_t w_bytes = MX_CHUNK + (tiles < 2 ? 0 : off == 0 ? MX_CHUNK : 4 * (MX_ROWS - off) * 16 + 512 + (second ? 4 * off * 16 + 512 : 0));
-            auto send_w = [&](int s, int c) {
-                unsigned char* dst = ring + s * stage_bytes + x_bytes;
-                mbar_expect_tx(&full_bar[s], (uint32_t)x_bytes + w_bytes);
-                mxt_copy(dst, src0 + (long)c * MX_CHUNK, MX_CHUNK, &full_bar[s]);
-                if (tiles < 2) return;
-                dst += MX_CODES + 1024;
-                const uint8_t* src = src1 + (long)c * MX_CHUNK;
-                if (off == 0) {
-                    mxt_copy(dst, src, MX_CHUNK, &full_bar[s]);
-                    return;
-                }
-                for (int b = 0; b < 4; ++b) mxt_copy(dst + b * 2048, src + b * 2048 + off * 16, (uint32_t)(MX_ROWS - off) * 16, &full_bar[s]);
-                mxt_copy(dst + MX_CODES, src + MX_CODES, 512, &full_bar[s]);
-                if (!second) return;
-                src += tile_bytes;
-                for (int b = 0; b < 4; ++b) mxt_copy(dst + b * 2048 + (MX_ROWS - off) * 16, src + b * 2048, (uint32_t)off * 16, &full_bar[s]);
-                mxt_copy(dst + MX_CODES + 512, src + MX_CODES, 512, &full_bar[s]);
-            };
-            auto send_x = [&](int s, int c) {
-                tma_load_2d(ring + s * stage_bytes, &map_x, &full_bar[s], c * 128, t0);
-                tma_load_2d(ring + s * stage_bytes + x_bytes / 2, &map_x, &full_bar[s], c * 128 + 64, t0);
-            };
-            // a constant W's first stages are sent for before the preceding kernel is waited for
-            const int ahead = constant_w && ok ? min(stages, c_end - c_begin) : 0;
-            for (int i = 0; i < ahead; ++i) send_w(i, c_begin + i);
-            pdl_wait();
-            for (int i = 0; i < ahead; ++i) send_x(i, c_begin + i);
-            issued = max(ahead, 0);
-            int s = issued % stages;
-            uint32_t ph = (uint32_t)(issued / stages) & 1u;
-            for (int c = c_begin + issued; c < c_end && ok; ++c) {
-                if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag)) {
-                    mxt_give_up(abort_flag, status);
-                    break;
-                }
-                send_w(s, c);
-                send_x(s, c);
-                ++issued;
-                if (++s == stages) { s = 0; ph ^= 1u; }
-            }
+            issued = mxt_produce<2048>(map_x, w, ring, full_bar, empty_bar, stages, stage_bytes, bn, t0, n, chunks, f0, row1, tiles, c_begin, c_end,
+                                       constant_w, ok, abort_flag, status);
         }
     } else {
         // ---- MMA issuer
@@ -419,10 +457,10 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
 
 // A cluster of CTAs along the grid's x.
 template <typename... KArgs, typename... Args>
-static int mxt_launch_cluster(void (*kernel)(KArgs...), int smem, dim3 grid, cudaStream_t stream, Args... args) {
+static int mxt_launch_cluster(void (*kernel)(KArgs...), int threads, int smem, dim3 grid, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(MXT_THREADS);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -436,28 +474,30 @@ static int mxt_launch_cluster(void (*kernel)(KArgs...), int smem, dim3 grid, cud
     return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-// How many CTAs of a cluster share K: the number of least time, in the time of a chunk of one CTA, with MXT_FIXED for what a CTA
-// takes besides its chunks.  slots[r]: clusters of r CTAs that the device holds at once.
-#define MXT_FIXED 8
-static int mxt_ranks(long tiles, int chunks, const int* slots) {
+// How many CTAs of a cluster share K: the number of least time, which is returned in `time`, in the time of one row tile's chunk;
+// `per`: what a CTA's chunk takes, `fixed`: what a CTA takes besides.  slots[r]: clusters of r CTAs that the device holds at once.
+static int mxt_ranks(long tiles, int chunks, const int* slots, int per, int fixed, long* time = nullptr) {
     int best = 1;
     long least = 0;
     for (int r = 1; r <= 8 && r <= chunks; ++r) {
         if (slots[r] < 1) continue;
-        const long time = (tiles + slots[r] - 1) / slots[r] * ((chunks + r - 1) / r + MXT_FIXED) + r / 4;
-        if (least == 0 || time < least) best = r, least = time;
+        const long t = (tiles + slots[r] - 1) / slots[r] * ((chunks + r - 1) / r * per + fixed);
+        if (least == 0 || t < least) best = r, least = t;
     }
+    if (time) *time = least;
     return best;
 }
 // Asked of the driver at a kernel's first launch (the current device's; all that the library runs on are alike).
 template <typename... KArgs>
-static const int* mxt_slots(void (*kernel)(KArgs...), int smem, int (&slots)[9]) {
+static const int* mxt_slots(void (*kernel)(KArgs...), int threads, int smem, int (&slots)[9]) {
     if (slots[0]) return slots;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return nullptr;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+        return nullptr;
     for (int r = 1; r <= 8; ++r) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(r);
-        cfg.blockDim = dim3(MXT_THREADS);
+        cfg.blockDim = dim3(threads);
         cfg.dynamicSmemBytes = smem;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -480,16 +520,16 @@ static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ld
     const int tokens_y = (m + bn - 1) / bn, chunks = (k + 127) / 128;
     if (tokens_y > 65535 || row_tiles > 65535) return (int)cudaErrorInvalidValue;
     static int found[9] = {};
-    const int* slots = mxt_slots(mxt_kernel<TO, GATED>, MXT_SMEM, found);
+    const int* slots = mxt_slots(mxt_kernel<TO, GATED>, MXT_THREADS, MXT_SMEM, found);
     if (!slots) return (int)cudaGetLastError();
-    const int ranks = mxt_ranks((long)tokens_y * row_tiles, chunks, slots);
+    const int ranks = mxt_ranks((long)tokens_y * row_tiles, chunks, slots, 1, 8);
     const int per_rank = (chunks + ranks - 1) / ranks;
     int stages = MXT_RING / (bn * 256 + MXT_W_BYTES);
     if (stages > MXT_MAX_STAGES) stages = MXT_MAX_STAGES;
     CUtensorMap map;
     int rc = make_map(&map, x, m, k, ldx, bn);
     if (rc) return rc;
-    return mxt_launch_cluster(mxt_kernel<TO, GATED>, MXT_SMEM, dim3(ranks, tokens_y, row_tiles), stream, map, (const uint8_t*)w, (TO*)out, ldo, m,
+    return mxt_launch_cluster(mxt_kernel<TO, GATED>, MXT_THREADS, MXT_SMEM, dim3(ranks, tokens_y, row_tiles), stream, map, (const uint8_t*)w, (TO*)out, ldo, m,
                               n, k, bn, stages, ranks, per_rank, constant_w, act, status);
 }
 
@@ -641,11 +681,11 @@ FL_API int fl_mxq_product(const void* a, const void* w, void* out, int out_code,
     if (token_tiles > 65535 || row_tiles > 65535) return (int)cudaErrorInvalidValue;
     FL_DISPATCH(out_code, TO, {
         static int found[9] = {};
-        const int* slots = mxt_slots(mxq_kernel<TO>, MXQ_SMEM, found);
+        const int* slots = mxt_slots(mxq_kernel<TO>, MXT_THREADS, MXQ_SMEM, found);
         if (!slots) return (int)cudaGetLastError();
-        const int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, slots);
+        const int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, slots, 1, 8);
         const int per_rank = (chunks + ranks - 1) / ranks;
-        return mxt_launch_cluster(mxq_kernel<TO>, MXQ_SMEM, dim3(ranks, token_tiles, row_tiles), stream, (const uint8_t*)a,
+        return mxt_launch_cluster(mxq_kernel<TO>, MXT_THREADS, MXQ_SMEM, dim3(ranks, token_tiles, row_tiles), stream, (const uint8_t*)a,
                                   (const uint8_t*)w, (TO*)out, ldo, m, n, chunks, ranks, per_rank, status);
     })
     return (int)cudaErrorInvalidValue;

@@ -105,7 +105,7 @@ _fns: dict = {}                                  # launchers, and status words b
 _QUANTIZE = ("mxfp4", "fl_mx_quantize", [c_void_p, c_int, c_long, c_void_p, c_int, c_int, c_void_p])
 _DEQUANTIZE = ("mxfp4", "fl_mx_dequantize", [c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_void_p])
 _FEW = ("mxfp4", "fl_mx_few", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_float, c_float,
-                               c_int, c_void_p])
+                               c_int, c_int, c_void_p])
 _MANY = ("mxfp4_tc", "fl_mxt_product", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_float,
                                         c_float, c_int, c_void_p, c_void_p])
 _BOTH = ("mxfp4_tc", "fl_mxq_product", [c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_void_p, c_void_p])
@@ -148,8 +148,7 @@ def dequantize(q: Matrix, out: torch.Tensor) -> None:
     ops._check(_fn(_DEQUANTIZE)(data.data_ptr(), out.data_ptr(), code, pitch, q.rows, q.k, stream), "mxfp4.dequantize")
 
 
-import os
-FEW_ROWS = int(os.environ.get('MXF', '16'))                                    # most rows that the kernel for few of them takes
+FEW_ROWS = 8                                    # most rows that the kernel for few of them takes
 
 
 def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, constant_w) -> None:
@@ -164,7 +163,7 @@ def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, consta
         return
     if m <= FEW_ROWS:
         rc = _fn(_FEW)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
-                       constant_w, stream)
+                       constant_w, ops.sm_count(x.device), stream)
     else:
         rc = _fn(_MANY)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
                         constant_w, _status(x), stream)
