@@ -1,0 +1,348 @@
+// Products of many rows with a matrix in microscaled 4-bit floating point on pairs of CTAs (cta_group::2): prompts.
+//
+// A pair's tile is 256 rows of W x up to 192 tokens.  Each CTA turns its 128 rows of W into bfloat16 in its own tensor memory (as
+// mxfp4_tc.cu does) and loads half of the tokens; the MMA reads both halves, so a CTA moves and converts half of what two CTAs with
+// tiles of 256 x 128 would.  Tensor memory holds two accumulators of 192 columns and four places of 32 columns for W (64 elements
+// along K): the next tile's
+// MMAs run while the epilogue's warps empty the last one's accumulator, 32 tokens a round through shared memory.  (With 256 tokens
+// there is room for one accumulator.)  Persistent: a pair walks over its tiles.
+//
+// Warps 0-7 convert, four of them a chunk of 128 along K, a thread one row; warps 8-11 are the epilogue; warp 12 sends for the
+// copies, warp 13 of the pair's even CTA (the leader) issues the MMAs.
+#include "mxfp4_tc.cuh"
+
+#define MXP_BN 192                                       // most tokens of a tile
+#define MXP_STAGES 5
+#define MXP_STAGE (MXP_BN / 2 * 256 + MX_CODES + 1536)   // half of the tokens as two boxes, 128 rows' codes, scales of up to 3 packed tiles
+#define MXP_ROUND (32 * 128 * 4)                         // 32 tokens' sums
+#define MXP_SMEM (MXP_STAGES * ((MXP_STAGE + 1023) / 1024 * 1024) + 2 * MXP_ROUND + 1024 + 512)
+#define MXP_THREADS (14 * 32)
+
+// ------------------------------------------------------------------ what a pair needs
+// (What the leader's MMA reads of the other CTA is in tensor memory, which tcgen05's own fences order.  An arrival with a release at
+// the cluster's scope waits for the thread's writes everywhere: it took this file's kernel from 297 to 466 us at 2048 tokens, K
+// 4096, 22016 features.)
+__device__ __forceinline__ void mxp_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// A barrier of the four epilogue warps, and whether any thread came with `flag`: they leave together or not at all.
+__device__ __forceinline__ bool mxp_vote(bool flag) {
+    uint32_t any;
+    __syncwarp();
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, 2, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"((uint32_t)flag)
+        : "memory");
+    return any != 0;
+}
+
+// The accumulator of a tile, emptied by the epilogue's four warps in rounds of 32 tokens: this CTA's 128 rows, FEAT features of them on
+// their way out.  `rounds`: how many this CTA has done, which picks the half of `staged`.  False: given up.
+template <typename TO, bool GATED>
+__device__ __forceinline__ bool mxp_epilogue(uint32_t tmem_acc, float* staged, uint32_t& rounds, int tokens, TO* __restrict__ out, long ldo, int n,
+                                             const FlGate act, volatile int* abort_flag, uint64_t* acc_empty) {
+    constexpr int FEAT = GATED ? 64 : 128, V = GATED ? 2 : 4;
+    const int quarter = mxt_warp() & 3, r = quarter * 32 + (threadIdx.x & 31);
+    const bool vec = (((uintptr_t)out | (uintptr_t)(ldo * (long)sizeof(TO))) & (V * sizeof(TO) - 1)) == 0 && (n & (V - 1)) == 0;
+    for (int t = 0; t < tokens; t += 32, ++rounds) {
+        float* half = staged + (rounds & 1) * (32 * 128);
+        uint32_t v[32];
+        tmem_ld16(tmem_acc + ((uint32_t)(quarter * 32) << 16) + (uint32_t)t, v);
+        tmem_ld16(tmem_acc + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(t + 16), v + 16);
+        tmem_ld_wait();
+        if (t + 32 >= tokens) {                           // the accumulator has been read
+            tc_fence_before();
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) mbar_arrive_leader(acc_empty);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) half[j * 128 + r] = __uint_as_float(v[j]);
+        if (mxp_vote(*abort_flag != 0)) return false;     // (a half's readers have all come here before it is written again)
+        if (n <= 0) continue;
+        const int last = min(32, tokens - t);
+        if (vec) mxt_rows<TO, GATED, FEAT, 128, V, 4>(half, quarter, last, 1, out + (long)t * ldo, ldo, n, act);
+        else mxt_rows<TO, GATED, FEAT, 128, 1, 4>(half, quarter, last, 1, out + (long)t * ldo, ldo, n, act);
+    }
+    return true;
+}
+
+// row_tiles x token_tiles tiles; bn: tokens of a tile, a multiple of 32.
+template <typename TO, bool GATED>
+__global__ void __launch_bounds__(MXP_THREADS, 1)
+mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ w, TO* __restrict__ out, long ldo, int m, int n, int k,
+           int bn, int token_tiles, int tiles, FlGate act, int* __restrict__ status) {
+    constexpr int FEAT = GATED ? 64 : 128, STAGE = (MXP_STAGE + 1023) / 1024 * 1024;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* ring = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float* staged = reinterpret_cast<float*>(ring + MXP_STAGES * STAGE);
+    uint64_t* x_full = (uint64_t*)(ring + MXP_STAGES * STAGE + 2 * MXP_ROUND);      // (the leader's: both CTAs' tokens)
+    uint64_t* w_full = x_full + MXP_STAGES;
+    uint64_t* empty_bar = w_full + MXP_STAGES;
+    uint64_t* a_full = empty_bar + MXP_STAGES;                                      // (the leader's)
+    uint64_t* a_empty = a_full + 4;
+    uint64_t* acc_full = a_empty + 4;
+    uint64_t* acc_empty = acc_full + 2;                                             // (the leader's)
+    uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    const int warp = mxt_warp(), lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank(), pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+    const int chunks = (k + 127) / 128;
+    const int x_bytes = bn * 128;                                                   // of this CTA's half
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < MXP_STAGES; ++s) {
+            mbar_init(&x_full[s], 1);
+            mbar_init(&w_full[s], 1);
+            mbar_init(&empty_bar[s], 5);                     // four warps have read the codes, the MMAs the tokens
+        }
+        for (int p = 0; p < 4; ++p) {
+            mbar_init(&a_full[p], 8);                        // four warps in each CTA
+            mbar_init(&a_empty[p], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], 8);
+        }
+        *abort_flag = (*(volatile int*)status != 0) ? 1 : 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 13) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();                                      // both CTAs' barriers exist before anyone signals them
+    tc_fence_after();
+    // accumulator b at 192 b, place p of W at 384 + 32 p.  (Launched in plain stream order, as every kernel with cta_group::2.)
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    bool ok = !*abort_flag;
+    int issued = 0;
+    if (warp < 8) {
+        // ---- codes to bfloat16
+        const int turn = warp >> 2, r = threadIdx.x & 127;
+        const uint32_t dst = tmem + 384u + (uint32_t)(turn * 64) + ((uint32_t)((warp & 3) * 32) << 16);
+        int s = 0, it = 0;                                   // stage of the chunk, chunks so far
+        uint32_t ph = 0, pa = 0;
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+            const int f0 = tile / token_tiles * (2 * FEAT) + rank * FEAT;
+            // where the row's scales are: the gate rows lie in one packed tile, the up rows in one or two
+            const int rr = !GATED ? r : r < 64 ? (f0 & (MX_ROWS - 1)) + r : (int)(((long)n + f0) & (MX_ROWS - 1)) + r - 64;
+            const int scale_at = x_bytes + (!GATED || r < 64 ? 0 : 1 + (rr >> 7)) * 512 + (int)mx_scale_at(rr & 127);
+            for (int c = 0; c < chunks; ++c, ++it) {
+                if ((it & 1) == turn) {
+                    if (!mxt_wait(&w_full[s], ph, abort_flag)) {
+                        if (lane == 0) mxt_give_up(abort_flag, status);
+                        ok = false;
+                        break;
+                    }
+                    const unsigned char* stage = ring + s * STAGE;
+                    uint4 q[4];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) q[b] = *reinterpret_cast<const uint4*>(stage + x_bytes + b * 2048 + r * 16);
+                    const uint32_t sc = *reinterpret_cast<const uint32_t*>(stage + scale_at);
+                    // (a byte above 128: its top bit is set, and it is not 128 itself)
+                    const bool large = __any_sync(0xffffffffu, (sc & 0x80808080u & ((sc & 0x7F7F7F7Fu) + 0x7F7F7F7Fu)) != 0);
+                    if (lane == 0) mxt_arrive(&empty_bar[s]);
+                    uint32_t v[32];
+                    auto two = [&](int b) {
+                        if (!large) {
+                            mx_block(q[b], mx_factor(sc >> (8 * b) & 255u), v);
+                            mx_block(q[b + 1], mx_factor(sc >> (8 * b + 8) & 255u), v + 16);
+                        } else {
+                            mx_block_large(q[b], sc >> (8 * b) & 255u, v);
+                            mx_block_large(q[b + 1], sc >> (8 * b + 8) & 255u, v + 16);
+                        }
+                    };
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {            // half of the chunk, place 2 turn + h
+                        if (!ok) break;
+                        two(2 * h);
+                        if (!mxt_wait(&a_empty[2 * turn + h], pa ^ 1u, abort_flag)) {
+                            if (lane == 0) mxt_give_up(abort_flag, status);
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        mxt_tmem_st16(dst + (uint32_t)(h * 32), v);
+                        mxt_tmem_st16(dst + (uint32_t)(h * 32 + 16), v + 16);
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_leader(&a_full[2 * turn + h]);
+                    }
+                    if (!ok) break;
+                    pa ^= 1u;
+                }
+                if (++s == MXP_STAGES) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp < 12) {
+        // ---- epilogue
+        uint32_t rounds = 0;
+        int i = 0;
+        for (int tile = pair; tile < tiles; tile += pairs, ++i) {
+            const int b = i & 1;
+            if (ok && !mxt_wait(&acc_full[b], (uint32_t)(i >> 1) & 1u, abort_flag)) {
+                if (lane == 0) mxt_give_up(abort_flag, status);
+                ok = false;
+            }
+            if (mxp_vote(!ok)) break;
+            tc_fence_after();
+            const int t0 = tile % token_tiles * bn, f0 = tile / token_tiles * (2 * FEAT) + rank * FEAT;
+            if (!mxp_epilogue<TO, GATED>(tmem + (uint32_t)(b * 192), staged, rounds, min(bn, m - t0), out + (long)t0 * ldo + f0, ldo, n - f0, act,
+                                         abort_flag, &acc_empty[b]))
+                break;
+        }
+    } else if (warp == 12) {
+        // ---- producer: this CTA's half of the tokens, signalled to the leader, and its rows of W
+        const long tile_bytes = (long)chunks * MX_CHUNK;
+        int s = 0;
+        uint32_t ph = 0;
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+            const int t0 = tile % token_tiles * bn + rank * (bn / 2), f0 = tile / token_tiles * (2 * FEAT) + rank * FEAT;
+            const long row1 = (long)n + f0;
+            const int off0 = f0 & (MX_ROWS - 1), off1 = (int)(row1 & (MX_ROWS - 1)), first = min(64, MX_ROWS - off1);
+            const int rest = (row1 / MX_ROWS + 1) * MX_ROWS < 2l * n ? 64 - first : 0;
+            const uint8_t* src0 = w + (long)(f0 / MX_ROWS) * tile_bytes;
+            const uint8_t* src1 = w + row1 / MX_ROWS * tile_bytes;
+            // (a CTA whose rows lie behind the last has nothing to load and converts whatever is there: rows that go nowhere)
+            const uint32_t w_bytes = f0 >= n ? 0 : !GATED ? MX_CHUNK : 4 * 1024 + 512 + 4 * first * 16 + 512 + (rest ? 4 * rest * 16 + 512 : 0);
+            for (int c = 0; c < chunks; ++c) {
+                if (!mxt_wait(&empty_bar[s], ph ^ 1u, abort_flag)) {
+                    if (lane == 0) mxt_give_up(abort_flag, status);
+                    ok = false;
+                    break;
+                }
+                if (mxt_elect()) {
+                    unsigned char* dst = ring + s * STAGE;
+                    if (rank == 0) mbar_expect_tx(&x_full[s], 2 * (uint32_t)x_bytes);
+                    mbar_expect_tx(&w_full[s], w_bytes);
+                    tma_load_2d_pair(dst, &map_x, &x_full[s], c * 128, t0);
+                    tma_load_2d_pair(dst + x_bytes / 2, &map_x, &x_full[s], c * 128 + 64, t0);
+                    dst += x_bytes;
+                    const uint8_t* src = src0 + (long)c * MX_CHUNK;
+                    if (w_bytes == 0) {
+                    } else if (!GATED) {
+                        mxt_copy(dst, src, MX_CHUNK, &w_full[s]);
+                    } else {
+                        for (int b = 0; b < 4; ++b) mxt_copy(dst + b * 2048, src + b * 2048 + off0 * 16, 1024, &w_full[s]);
+                        mxt_copy(dst + MX_CODES, src + MX_CODES, 512, &w_full[s]);
+                        src = src1 + (long)c * MX_CHUNK;
+                        for (int b = 0; b < 4; ++b) mxt_copy(dst + b * 2048 + 1024, src + b * 2048 + off1 * 16, (uint32_t)first * 16, &w_full[s]);
+                        mxt_copy(dst + MX_CODES + 512, src + MX_CODES, 512, &w_full[s]);
+                        if (rest) {
+                            src += tile_bytes;
+                            for (int b = 0; b < 4; ++b)
+                                mxt_copy(dst + b * 2048 + 1024 + first * 16, src + b * 2048, (uint32_t)rest * 16, &w_full[s]);
+                            mxt_copy(dst + MX_CODES + 1024, src + MX_CODES, 512, &w_full[s]);
+                        }
+                    }
+                }
+                __syncwarp();
+                ++issued;
+                if (++s == MXP_STAGES) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (rank == 0) {
+        // ---- MMA issuer, for both CTAs
+        const uint32_t idesc = instr_desc_bf16(256, bn), ring_at = smem_u32(ring);
+        const uint64_t half = (uint64_t)(x_bytes / 2) >> 4;
+        int s = 0, i = 0, it = 0;
+        uint32_t ph = 0;
+        for (int tile = pair; tile < tiles && ok; tile += pairs, ++i) {
+            const int b = i & 1;
+            ok = mxt_wait(&acc_empty[b], ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag);
+            tc_fence_after();
+            const uint32_t acc = tmem + (uint32_t)(b * 192);
+            for (int c = 0; c < chunks && ok; ++c, ++it) {
+                const uint32_t turn = (uint32_t)it & 1u;
+                ok = mxt_wait(&x_full[s], ph, abort_flag);
+                const uint64_t bdesc = smem_desc_sw128(ring_at + (uint32_t)(s * STAGE));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    ok = ok && mxt_wait(&a_full[2 * turn + h], (uint32_t)(it >> 1) & 1u, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (mxt_elect()) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            mxp_umma_ts(acc, tmem + 384u + turn * 64u + (uint32_t)(h * 32 + kk * 8), bdesc + (uint64_t)(2 * kk) + (h ? half : 0), idesc,
+                                        (c > 0 || h > 0 || kk > 0) ? 1u : 0u);
+                        umma_commit_pair(&a_empty[2 * turn + h]);
+                        if (h) umma_commit_pair(&empty_bar[s]);
+                        if (h && c == chunks - 1) umma_commit_pair(&acc_full[b]);
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                if (++s == MXP_STAGES) { s = 0; ph ^= 1u; }
+            }
+            if (!ok && lane == 0) mxt_give_up(abort_flag, status);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12 && lane == 0 && *abort_flag) {
+        tma_drain(w_full, MXP_STAGES, issued);
+        if (rank == 0) tma_drain(x_full, MXP_STAGES, issued);
+    }
+    __syncthreads();
+    cluster_sync_all();                                      // neither leaves while the other's MMAs or copies may reach it
+    if (warp == 13) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+template <typename TO, bool GATED>
+static int mxp_launch(const void* x, long ldx, const void* w, void* out, long ldo, int m, int n, int k, FlGate act, int num_sms, int* status,
+                      cudaStream_t stream) {
+    const int token_tiles = (m + MXP_BN - 1) / MXP_BN, bn = ((m + token_tiles - 1) / token_tiles + 31) / 32 * 32;
+    const int rows = GATED ? 128 : 256;
+    const long tiles = (long)((n + rows - 1) / rows) * ((m + bn - 1) / bn);
+    if (tiles > 0x3FFFFFFFl || (long)((k + 127) / 128) * 2 > 0x3FFFFFFFl / (tiles / (num_sms / 2) + 1)) return (int)cudaErrorInvalidValue;
+    CUtensorMap map;
+    int rc = make_map(&map, x, m, k, ldx, bn / 2);
+    if (rc) return rc;
+    auto kernel = mxp_kernel<TO, GATED>;
+    static bool configured = false;
+    if (!configured) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MXP_SMEM);
+        if (e != cudaSuccess) return (int)e;
+        configured = true;
+    }
+    const long pairs = tiles < num_sms / 2 ? tiles : num_sms / 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * pairs));
+    cfg.blockDim = dim3(MXP_THREADS);
+    cfg.dynamicSmemBytes = MXP_SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, map, (const uint8_t*)w, (TO*)out, ldo, m, n, k, bn, (m + bn - 1) / bn, (int)tiles, act, status);
+}
+
+// As fl_mxt_product (mxfp4_tc.cu), for many tokens.
+FL_API int fl_mxp_product(const void* x, long ldx, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int gated, int act,
+                          float p0, float p1, int num_sms, int* status, cudaStream_t stream) {
+    const FlGate gate = {act, p0, p1};
+    FL_DISPATCH(out_code, TO, {
+        return gated ? mxp_launch<TO, true>(x, ldx, w, out, ldo, m, n, k, gate, num_sms, status, stream)
+                     : mxp_launch<TO, false>(x, ldx, w, out, ldo, m, n, k, gate, num_sms, status, stream);
+    })
+    return (int)cudaErrorInvalidValue;
+}

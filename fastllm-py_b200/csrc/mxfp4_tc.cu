@@ -1,4 +1,4 @@
-// Products of bfloat16 rows with a matrix in microscaled 4-bit floating point on the tensor cores (mxfp4.cu says what the
+// Products of bfloat16 rows with a matrix in microscaled 4-bit floating point on the tensor cores (mxfp4.cuh says what the
 // packed form is): out[t, f] = sum_k x[t, k] W[f, k], and the gated unit act(gate) * up of two such products.
 //
 // The weights are turned into bfloat16 on their way (exactly: a magnitude of two bits of significand times a power of two) and
@@ -11,11 +11,8 @@
 // tensor memory; then they are the epilogue.  Warp 16 sends for the copies, warp 17 issues the MMAs.  Where there are fewer
 // tiles than SMs a cluster of up to 8 CTAs shares K; its partial sums stay in shared memory, and each CTA adds up its share of the
 // tokens from all of them, in rank order.
-#include "tcgen05.cuh"
+#include "mxfp4_tc.cuh"
 
-#define MX_ROWS 128
-#define MX_CODES 8192
-#define MX_CHUNK 8704
 #define MXT_BN 128                          // most tokens of a tile
 #define MXT_A 2                             // places of 2 x 64 columns in tensor memory
 #define MXT_W_BYTES (2 * (MX_CODES + 1024)) // two row tiles of a chunk: codes, the scales of the one or two packed tiles they lie in
@@ -27,153 +24,6 @@
 #define MXT_SMEM (MXT_RING + 1024 + 1024)
 #define MXT_WARPS 16                        // that convert, and of the epilogue
 #define MXT_THREADS ((MXT_WARPS + 2) * 32)
-enum { MXT_ERR_WAIT = 121 };
-
-__device__ __forceinline__ int mx_scale_at(int r) { return MX_CODES + (r & 31) * 16 + (r >> 5) * 4; }
-
-// A word of 8 codes as 4 pairs of bfloat16, element 2 i in the low half of w[i]: sign and magnitude of nibbles i and 4 + i where
-// a bfloat16 of exponent 2^-126 has them (the magnitudes 0 and 0.5 are subnormal), times m1.  A product with two powers of two puts
-// a nibble in both places at once.
-__device__ __forceinline__ uint32_t mx_mul(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-__device__ __forceinline__ void mx_pairs(uint32_t q, uint32_t m1, uint32_t* w) {
-    constexpr uint32_t PLACES = 0x81C081C0u, NIBBLE = 0x000F000Fu;
-    w[0] = mx_mul(((q & NIBBLE) * 0x1040u) & PLACES, m1);
-    w[1] = mx_mul(((q & (NIBBLE << 4)) * 0x104u) & PLACES, m1);
-    w[2] = mx_mul((((q >> 8) & NIBBLE) * 0x1040u) & PLACES, m1);
-    w[3] = mx_mul((((q >> 8) & (NIBBLE << 4)) * 0x104u) & PLACES, m1);
-}
-__device__ __forceinline__ uint32_t mx_both(uint32_t h) { return h | h << 16; }
-// The factors of a block with scale byte s: m1 = 2^(s - 1), both halves alike; where that has no bfloat16 (s > 128: a block whose
-// largest magnitude is 4 or more) m1 is 2^127 and the rest a second factor, else 1.
-__device__ __forceinline__ uint32_t mx_factor(uint32_t s) { return (s + 126u) * 0x00800080u; }
-__device__ __forceinline__ uint32_t mx_factor_large(uint32_t s) { return mx_both(s == 255 ? 0x7FC0u : (min(s, 128u) + 126u) << 7); }
-__device__ __forceinline__ uint32_t mx_factor_rest(uint32_t s) { return mx_both(s == 255 || s <= 128 ? 0x3F80u : (s - 1) << 7); }
-// A block of a row, 16 bytes of codes with scale byte s, as 16 pairs: exactly the values.
-__device__ __forceinline__ void mx_block(const uint4 q, uint32_t m1, uint32_t* w) {
-    mx_pairs(q.x, m1, w);
-    mx_pairs(q.y, m1, w + 4);
-    mx_pairs(q.z, m1, w + 8);
-    mx_pairs(q.w, m1, w + 12);
-}
-__device__ __forceinline__ void mx_block_large(const uint4 q, uint32_t s, uint32_t* w) {
-    mx_block(q, mx_factor_large(s), w);
-    const uint32_t m2 = mx_factor_rest(s);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = mx_mul(w[i], m2);
-}
-
-__device__ __forceinline__ void mxt_tmem_st16(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-__device__ __forceinline__ void mxt_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// One lane of a warp that is together.  The issuing warps stay together and elect for each batch of instructions: what the matrix
-// instructions take then is the same in the whole warp and lives in uniform registers.  Issued by a branch of lane 0 each of them
-// cost 140 to 190 clocks, whatever its size (2048 tokens, K 4096, 22016 features: 472 us, and 331 with the election).
-__device__ __forceinline__ bool mxt_elect() {
-    uint32_t p;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
-    return p != 0;
-}
-__device__ __forceinline__ int mxt_warp() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
-__device__ __forceinline__ void mxt_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-// lane 0 waits for its warp
-__device__ __forceinline__ bool mxt_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-    uint32_t ok = 1;
-    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag) ? 1u : 0u;
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
-}
-// Tokens t, t + STEP, .. of the float sums [token][PITCH] (FEAT features, of a gated unit then their up values), added up over the cluster's CTAs in rank order, through the
-// activation and out; `n`: how many features there are from the tile's first on.
-template <int V> struct MxtVec { float v[V]; };
-template <int V> __device__ __forceinline__ MxtVec<V> mxt_get(const float* sums, int ranks, int rank) {
-    MxtVec<V> r;
-    if (ranks == 1) {
-        if (V == 4) {
-            const float4 x = *reinterpret_cast<const float4*>(sums);
-            r.v[V > 3 ? 3 : 0] = x.w, r.v[V > 2 ? 2 : 0] = x.z, r.v[V > 1 ? 1 : 0] = x.y, r.v[0] = x.x;
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) r.v[i] = sums[i];
-        }
-        return r;
-    }
-    uint32_t at;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(sums)), "r"(rank));
-    if (V == 4)
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(r.v[0]), "=f"(r.v[V > 1 ? 1 : 0]), "=f"(r.v[V > 2 ? 2 : 0]), "=f"(r.v[V > 3 ? 3 : 0])
-                     : "r"(at)
-                     : "memory");
-    else if (V == 2)
-        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(r.v[0]), "=f"(r.v[V > 1 ? 1 : 0]) : "r"(at) : "memory");
-    else
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r.v[0]) : "r"(at) : "memory");
-    return r;
-}
-template <typename TO, bool GATED, int FEAT, int PITCH, int V, int STEP>
-__device__ __forceinline__ void mxt_rows(const float* sums, int t, int last, int ranks, TO* out, long ldo, int n, const FlGate act) {
-    constexpr int PARTS = FEAT / (32 * V);                            // steps of 32 V features
-    const int f0 = (threadIdx.x & 31) * V;
-#pragma unroll 2
-    for (; t < last; t += STEP) {
-        float g[PARTS * V], u[PARTS * V];
-#pragma unroll
-        for (int i = 0; i < PARTS * V; ++i) g[i] = 0.0f, u[i] = GATED ? 0.0f : 1.0f;
-        const float* row = sums + t * PITCH + f0;
-#pragma unroll 4
-        for (int q = 0; q < ranks; ++q)
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p) {
-                const MxtVec<V> x = mxt_get<V>(row + p * 32 * V, ranks, q);
-#pragma unroll
-                for (int i = 0; i < V; ++i) g[p * V + i] += x.v[i];
-                if (GATED) {
-                    const MxtVec<V> y = mxt_get<V>(row + FEAT + p * 32 * V, ranks, q);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) u[p * V + i] += y.v[i];
-                }
-            }
-        if (act.act != FL_ACT_NONE) gated_act(g, u, act);
-        TO* dst = out + (long)t * ldo + f0;
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-            if (f0 + p * 32 * V >= n) continue;                       // (n is a multiple of V)
-            __align__(16) TO o[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = from_f32<TO>(g[p * V + i]);
-            TO* d = dst + p * 32 * V;
-            if (V == 1) *d = o[0];
-            else if (V * sizeof(TO) == 4) *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(o);
-            else if (V * sizeof(TO) == 8) *reinterpret_cast<uint2*>(d) = *reinterpret_cast<const uint2*>(o);
-            else *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(o);
-        }
-    }
-}
-
-__device__ __forceinline__ void mxt_give_up(volatile int* abort_flag, int* status) {
-    if (!*abort_flag) {
-        *abort_flag = 1;
-        atomicCAS(status, 0, MXT_ERR_WAIT);
-    }
-}
 
 // The end of a CTA whose sums of `rows` tokens are written, by all its threads: its share of the tokens from all of the cluster's
 // CTAs, by its first WARPS warps.  Leaves with the cluster's sums no longer needed.
@@ -231,51 +81,35 @@ __device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, uint64_
     mxt_join<TO, GATED, GATED ? 128 : 256, MXT_PITCH, MXT_WARPS>(sums, abort_flag, rows, ranks, rank, out, ldo, f0, n, act);
 }
 
-__device__ __forceinline__ void mxt_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
-                 "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
-}
-
-// The copies of a CTA's chunks c_begin .. c_end - 1, by one thread; returns how many stages were sent for.  A stage: bn x 128 elements
-// of the tokens as two boxes, then the row tiles, each four pieces of codes PIECE bytes apart and the scales of the one or two packed
-// tiles that its rows lie in.  Tile 0 begins with row f0 of W, tile 1 (if tiles is 2) with row row1.
-template <int PIECE>
+// The copies of a CTA's chunks c_begin .. c_end - 1, by one warp; returns how many stages were sent for.  A stage: bn x 128 elements
+// of the tokens as two boxes, then the row tiles, each 8192 bytes of codes and the scales of the one or two packed tiles that its
+// rows lie in.  Tile 0 begins with row f0 of W, tile 1 (if tiles is 2) with row row1.
 __device__ __forceinline__ int mxt_produce(const CUtensorMap& map_x, const uint8_t* __restrict__ w, unsigned char* ring, uint64_t* full_bar,
                                            uint64_t* empty_bar, int stages, int stage_bytes, int bn, int t0, int n, int chunks, int f0, long row1,
                                            int tiles, int c_begin, int c_end, bool constant_w, bool ok, volatile int* abort_flag, int* status) {
-    constexpr int TILE = 4 * PIECE + 1024;
     const int off = (int)(row1 & (MX_ROWS - 1)), x_bytes = bn * 256;
     const long tile_bytes = (long)chunks * MX_CHUNK;
     const uint8_t* src0 = w + (long)(f0 / MX_ROWS) * tile_bytes;
     const uint8_t* src1 = w + row1 / MX_ROWS * tile_bytes;
     const bool second = off != 0 && (row1 / MX_ROWS + 1) * MX_ROWS < 2l * n;             // (only up rows straddle)
     const uint32_t w_bytes = MX_CHUNK + (tiles < 2 ? 0 : off == 0 ? MX_CHUNK : 4 * (MX_ROWS - off) * 16 + 512 + (second ? 4 * off * 16 + 512 : 0));
-    auto send_tile = [&](unsigned char* dst, const uint8_t* src, uint64_t* bar) {
-        if (PIECE == 2048) {
-            mxt_copy(dst, src, MX_CHUNK, bar);
-        } else {
-            for (int b = 0; b < 4; ++b) mxt_copy(dst + b * PIECE, src + b * 2048, 2048, bar);
-            mxt_copy(dst + 4 * PIECE, src + MX_CODES, 512, bar);
-        }
-    };
     auto send_w = [&](int s, int c) {
         unsigned char* dst = ring + s * stage_bytes + x_bytes;
         mbar_expect_tx(&full_bar[s], (uint32_t)x_bytes + w_bytes);
-        send_tile(dst, src0 + (long)c * MX_CHUNK, &full_bar[s]);
+        mxt_copy(dst, src0 + (long)c * MX_CHUNK, MX_CHUNK, &full_bar[s]);
         if (tiles < 2) return;
-        dst += TILE;
+        dst += MX_CODES + 1024;
         const uint8_t* src = src1 + (long)c * MX_CHUNK;
         if (off == 0) {
-            send_tile(dst, src, &full_bar[s]);
+            mxt_copy(dst, src, MX_CHUNK, &full_bar[s]);
             return;
         }
-        for (int b = 0; b < 4; ++b) mxt_copy(dst + b * PIECE, src + b * 2048 + off * 16, (uint32_t)(MX_ROWS - off) * 16, &full_bar[s]);
-        mxt_copy(dst + 4 * PIECE, src + MX_CODES, 512, &full_bar[s]);
+        for (int b = 0; b < 4; ++b) mxt_copy(dst + b * 2048, src + b * 2048 + off * 16, (uint32_t)(MX_ROWS - off) * 16, &full_bar[s]);
+        mxt_copy(dst + MX_CODES, src + MX_CODES, 512, &full_bar[s]);
         if (!second) return;
         src += tile_bytes;
-        for (int b = 0; b < 4; ++b) mxt_copy(dst + b * PIECE + (MX_ROWS - off) * 16, src + b * 2048, (uint32_t)off * 16, &full_bar[s]);
-        mxt_copy(dst + 4 * PIECE + 512, src + MX_CODES, 512, &full_bar[s]);
+        for (int b = 0; b < 4; ++b) mxt_copy(dst + b * 2048 + (MX_ROWS - off) * 16, src + b * 2048, (uint32_t)off * 16, &full_bar[s]);
+        mxt_copy(dst + MX_CODES + 512, src + MX_CODES, 512, &full_bar[s]);
     };
     auto send_x = [&](int s, int c) {
         tma_load_2d(ring + s * stage_bytes, &map_x, &full_bar[s], c * 128, t0);
@@ -283,18 +117,25 @@ __device__ __forceinline__ int mxt_produce(const CUtensorMap& map_x, const uint8
     };
     // a constant W's first stages are sent for before the preceding kernel is waited for
     const int ahead = constant_w && ok ? max(0, min(stages, c_end - c_begin)) : 0;
-    for (int i = 0; i < ahead; ++i) send_w(i, c_begin + i);
+    if (mxt_elect())
+        for (int i = 0; i < ahead; ++i) send_w(i, c_begin + i);
+    __syncwarp();
     pdl_wait();
-    for (int i = 0; i < ahead; ++i) send_x(i, c_begin + i);
+    if (mxt_elect())
+        for (int i = 0; i < ahead; ++i) send_x(i, c_begin + i);
+    __syncwarp();
     int issued = ahead, s = issued % stages;
     uint32_t ph = (uint32_t)(issued / stages) & 1u;
     for (int c = c_begin + issued; c < c_end && ok; ++c) {
-        if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag)) {
-            mxt_give_up(abort_flag, status);
+        if (!mxt_wait(&empty_bar[s], ph ^ 1u, abort_flag)) {
+            if ((threadIdx.x & 31) == 0) mxt_give_up(abort_flag, status);
             break;
         }
-        send_w(s, c);
-        send_x(s, c);
+        if (mxt_elect()) {
+            send_w(s, c);
+            send_x(s, c);
+        }
+        __syncwarp();
         ++issued;
         if (++s == stages) { s = 0; ph ^= 1u; }
     }
@@ -413,11 +254,8 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
             if (s >= stages) s -= stages, ph ^= 1u;
         }
     } else if (warp == MXT_WARPS) {
-        if (lane == 0) {
-            // ---- producer
-            issued = mxt_produce<2048>(map_x, w, ring, full_bar, empty_bar, stages, stage_bytes, bn, t0, n, chunks, f0, row1, tiles, c_begin, c_end,
-                                       constant_w, ok, abort_flag, status);
-        }
+        issued = mxt_produce(map_x, w, ring, full_bar, empty_bar, stages, stage_bytes, bn, t0, n, chunks, f0, row1, tiles, c_begin, c_end, constant_w,
+                             ok, abort_flag, status);
     } else {
         // ---- MMA issuer
         const uint32_t idesc = instr_desc_bf16(128, bn), ring_at = smem_u32(ring);
@@ -617,24 +455,26 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
     int issued = 0;
     const bool ok = !*abort_flag;
     if (warp == MXT_WARPS) {
-        if (lane == 0) {
-            const uint8_t* src_a = a + (long)blockIdx.y * chunks * MX_CHUNK;
-            const uint8_t* src_w = w + (long)blockIdx.z * 2 * chunks * MX_CHUNK;
-            int s = 0;
-            uint32_t ph = 0;
-            for (int c = c_begin; c < c_end && ok; ++c) {
-                if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag)) {
-                    mxt_give_up(abort_flag, status);
-                    break;
-                }
+        // ---- producer
+        const uint8_t* src_a = a + (long)blockIdx.y * chunks * MX_CHUNK;
+        const uint8_t* src_w = w + (long)blockIdx.z * 2 * chunks * MX_CHUNK;
+        int s = 0;
+        uint32_t ph = 0;
+        for (int c = c_begin; c < c_end && ok; ++c) {
+            if (!mxt_wait(&empty_bar[s], ph ^ 1u, abort_flag)) {
+                if (lane == 0) mxt_give_up(abort_flag, status);
+                break;
+            }
+            if (mxt_elect()) {
                 unsigned char* dst = ring + s * MXQ_STAGE;
                 mbar_expect_tx(&full_bar[s], (uint32_t)((tiles + 1) * MX_CHUNK));
                 mxt_copy(dst, src_a + (long)c * MX_CHUNK, MX_CHUNK, &full_bar[s]);
                 for (int t = 0; t < tiles; ++t)
                     mxt_copy(dst + (1 + t) * MX_CHUNK, src_w + ((long)t * chunks + c) * MX_CHUNK, MX_CHUNK, &full_bar[s]);
-                ++issued;
-                if (++s == MXQ_STAGES) { s = 0; ph ^= 1u; }
             }
+            __syncwarp();
+            ++issued;
+            if (++s == MXQ_STAGES) { s = 0; ph ^= 1u; }
         }
     } else if (warp == MXT_WARPS + 1) {
         const int bn = (rows + 15) / 16 * 16;

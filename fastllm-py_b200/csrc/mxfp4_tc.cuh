@@ -1,0 +1,123 @@
+// Shared by the products with matrices in 4 bits on the tensor cores (mxfp4_tc.cu, mxfp4_pair.cu): how their warps wait, issue and
+// give up, and how sums of tokens leave shared memory.
+#pragma once
+
+#include "mxfp4.cuh"
+#include "tcgen05.cuh"
+
+enum { MXT_ERR_WAIT = 121 };
+
+__device__ __forceinline__ void mxt_tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void mxt_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// One lane of a warp that is together.  The issuing warps stay together and elect for each batch of instructions: what the matrix
+// instructions take then is the same in the whole warp and lives in uniform registers.  Issued by a branch of lane 0 each of them
+// cost 140 to 190 clocks, whatever its size (2048 tokens, K 4096, 22016 features: 472 us, and 331 with the election).
+__device__ __forceinline__ bool mxt_elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ int mxt_warp() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
+__device__ __forceinline__ void mxt_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// lane 0 waits for its warp
+__device__ __forceinline__ bool mxt_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    uint32_t ok = 1;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag) ? 1u : 0u;
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+// Tokens t, t + STEP, .. of the float sums [token][PITCH] (FEAT features, of a gated unit then their up values), added up over the cluster's CTAs in rank order, through the
+// activation and out; `n`: how many features there are from the tile's first on.
+template <int V> struct MxtVec { float v[V]; };
+template <int V> __device__ __forceinline__ MxtVec<V> mxt_get(const float* sums, int ranks, int rank) {
+    MxtVec<V> r;
+    if (ranks == 1) {
+        if (V == 4) {
+            const float4 x = *reinterpret_cast<const float4*>(sums);
+            r.v[V > 3 ? 3 : 0] = x.w, r.v[V > 2 ? 2 : 0] = x.z, r.v[V > 1 ? 1 : 0] = x.y, r.v[0] = x.x;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) r.v[i] = sums[i];
+        }
+        return r;
+    }
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(sums)), "r"(rank));
+    if (V == 4)
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(r.v[0]), "=f"(r.v[V > 1 ? 1 : 0]), "=f"(r.v[V > 2 ? 2 : 0]), "=f"(r.v[V > 3 ? 3 : 0])
+                     : "r"(at)
+                     : "memory");
+    else if (V == 2)
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(r.v[0]), "=f"(r.v[V > 1 ? 1 : 0]) : "r"(at) : "memory");
+    else
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r.v[0]) : "r"(at) : "memory");
+    return r;
+}
+template <typename TO, bool GATED, int FEAT, int PITCH, int V, int STEP>
+__device__ __forceinline__ void mxt_rows(const float* sums, int t, int last, int ranks, TO* out, long ldo, int n, const FlGate act) {
+    constexpr int PARTS = FEAT / (32 * V);                            // steps of 32 V features
+    const int f0 = (threadIdx.x & 31) * V;
+#pragma unroll 2
+    for (; t < last; t += STEP) {
+        float g[PARTS * V], u[PARTS * V];
+#pragma unroll
+        for (int i = 0; i < PARTS * V; ++i) g[i] = 0.0f, u[i] = GATED ? 0.0f : 1.0f;
+        const float* row = sums + t * PITCH + f0;
+#pragma unroll 4
+        for (int q = 0; q < ranks; ++q)
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                const MxtVec<V> x = mxt_get<V>(row + p * 32 * V, ranks, q);
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[p * V + i] += x.v[i];
+                if (GATED) {
+                    const MxtVec<V> y = mxt_get<V>(row + FEAT + p * 32 * V, ranks, q);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) u[p * V + i] += y.v[i];
+                }
+            }
+        if (act.act != FL_ACT_NONE) gated_act(g, u, act);
+        TO* dst = out + (long)t * ldo + f0;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            if (f0 + p * 32 * V >= n) continue;                       // (n is a multiple of V)
+            __align__(16) TO o[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = from_f32<TO>(g[p * V + i]);
+            TO* d = dst + p * 32 * V;
+            if (V == 1) *d = o[0];
+            else if (V * sizeof(TO) == 4) *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(o);
+            else if (V * sizeof(TO) == 8) *reinterpret_cast<uint2*>(d) = *reinterpret_cast<const uint2*>(o);
+            else *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(o);
+        }
+    }
+}
+
+__device__ __forceinline__ void mxt_give_up(volatile int* abort_flag, int* status) {
+    if (!*abort_flag) {
+        *abort_flag = 1;
+        atomicCAS(status, 0, MXT_ERR_WAIT);
+    }
+}
+
+__device__ __forceinline__ void mxt_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+                 "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}

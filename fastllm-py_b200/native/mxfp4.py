@@ -108,6 +108,8 @@ _FEW = ("mxfp4", "fl_mx_few", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_lo
                                c_int, c_int, c_void_p])
 _MANY = ("mxfp4_tc", "fl_mxt_product", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_float,
                                         c_float, c_int, c_void_p, c_void_p])
+_PAIRS = ("mxfp4_pair", "fl_mxp_product", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_float,
+                                           c_float, c_int, c_void_p, c_void_p])
 _BOTH = ("mxfp4_tc", "fl_mxq_product", [c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_void_p, c_void_p])
 
 
@@ -148,6 +150,8 @@ def dequantize(q: Matrix, out: torch.Tensor) -> None:
     ops._check(_fn(_DEQUANTIZE)(data.data_ptr(), out.data_ptr(), code, pitch, q.rows, q.k, stream), "mxfp4.dequantize")
 
 
+import os
+MANY_ROWS = int(os.environ.get('MXP', '256'))
 FEW_ROWS = 8                                    # most rows that the kernel for few of them takes
 
 
@@ -164,6 +168,9 @@ def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, consta
     if m <= FEW_ROWS:
         rc = _fn(_FEW)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
                        constant_w, ops.sm_count(x.device), stream)
+    elif m > MANY_ROWS:
+        rc = _fn(_PAIRS)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
+                         ops.sm_count(x.device), _status(x), stream)
     else:
         rc = _fn(_MANY)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
                         constant_w, _status(x), stream)
