@@ -7,16 +7,23 @@
 // MMAs run while the epilogue's warps empty the last one's accumulator, 32 tokens a round through shared memory.  (With 256 tokens
 // there is room for one accumulator.)  Persistent: a pair walks over its tiles.
 //
-// Warps 0-7 convert, four of them a chunk of 128 along K, a thread one row; warps 8-11 are the epilogue; warp 12 sends for the
-// copies, warp 13 of the pair's even CTA (the leader) issues the MMAs.
+// Warps 0-15 convert, four of them half of a chunk of 128 along K, a thread one row (with eight warps a chunk took 1300 clocks, mostly
+// waiting; its MMAs take 770); warps 16-19 are the epilogue; warps 20 and 22 send for the tokens and the codes, warp 21 of the pair's
+// even CTA (the leader) issues the MMAs.
+#pragma once
+
 #include "mxfp4_tc.cuh"
 
 #define MXP_BN 192                                       // most tokens of a tile
-#define MXP_STAGES 5
-#define MXP_STAGE (MXP_BN / 2 * 256 + MX_CODES + 1536)   // half of the tokens as two boxes, 128 rows' codes, scales of up to 3 packed tiles
+// The tokens and the codes have rings of their own: a chunk's codes are needed a conversion earlier than its tokens, which would
+// otherwise wait in shared memory for as long (2048 tokens, K 4096, 22016 features: 295 us with one ring of five stages).
+#define MXP_X_RING (144 * 1024)
+#define MXP_X_STAGES 8                                   // most of them: of bn / 2 x 128 elements, two boxes
+#define MXP_W_STAGES 4
+#define MXP_W_STAGE (MX_CODES + 1536)                    // 128 rows' codes, scales of up to 3 packed tiles
 #define MXP_ROUND (32 * 128 * 4)                         // 32 tokens' sums
-#define MXP_SMEM (MXP_STAGES * ((MXP_STAGE + 1023) / 1024 * 1024) + 2 * MXP_ROUND + 1024 + 512)
-#define MXP_THREADS (14 * 32)
+#define MXP_SMEM (MXP_X_RING + MXP_W_STAGES * MXP_W_STAGE + 2 * MXP_ROUND + 1024 + 512)
+#define MXP_THREADS (23 * 32)
 
 // ------------------------------------------------------------------ what a pair needs
 // (What the leader's MMA reads of the other CTA is in tensor memory, which tcgen05's own fences order.  An arrival with a release at
@@ -79,15 +86,17 @@ __device__ __forceinline__ bool mxp_epilogue(uint32_t tmem_acc, float* staged, u
 template <typename TO, bool GATED>
 __global__ void __launch_bounds__(MXP_THREADS, 1)
 mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ w, TO* __restrict__ out, long ldo, int m, int n, int k,
-           int bn, int token_tiles, int tiles, FlGate act, int* __restrict__ status) {
-    constexpr int FEAT = GATED ? 64 : 128, STAGE = (MXP_STAGE + 1023) / 1024 * 1024;
+           int bn, int x_stages, int token_tiles, int tiles, FlGate act, int* __restrict__ status) {
+    constexpr int FEAT = GATED ? 64 : 128;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* ring = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    float* staged = reinterpret_cast<float*>(ring + MXP_STAGES * STAGE);
-    uint64_t* x_full = (uint64_t*)(ring + MXP_STAGES * STAGE + 2 * MXP_ROUND);      // (the leader's: both CTAs' tokens)
-    uint64_t* w_full = x_full + MXP_STAGES;
-    uint64_t* empty_bar = w_full + MXP_STAGES;
-    uint64_t* a_full = empty_bar + MXP_STAGES;                                      // (the leader's)
+    unsigned char* w_ring = ring + MXP_X_RING;
+    float* staged = reinterpret_cast<float*>(w_ring + MXP_W_STAGES * MXP_W_STAGE);
+    uint64_t* x_full = (uint64_t*)(staged + 2 * (MXP_ROUND / 4));                   // (the leader's: both CTAs' tokens)
+    uint64_t* x_empty = x_full + MXP_X_STAGES;
+    uint64_t* w_full = x_empty + MXP_X_STAGES;
+    uint64_t* w_empty = w_full + MXP_W_STAGES;
+    uint64_t* a_full = w_empty + MXP_W_STAGES;                                      // (the leader's)
     uint64_t* a_empty = a_full + 4;
     uint64_t* acc_full = a_empty + 4;
     uint64_t* acc_empty = acc_full + 2;                                             // (the leader's)
@@ -99,10 +108,13 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
     const int x_bytes = bn * 128;                                                   // of this CTA's half
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < MXP_STAGES; ++s) {
+        for (int s = 0; s < x_stages; ++s) {
             mbar_init(&x_full[s], 1);
+            mbar_init(&x_empty[s], 1);
+        }
+        for (int s = 0; s < MXP_W_STAGES; ++s) {
             mbar_init(&w_full[s], 1);
-            mbar_init(&empty_bar[s], 5);                     // four warps have read the codes, the MMAs the tokens
+            mbar_init(&w_empty[s], 8);
         }
         for (int p = 0; p < 4; ++p) {
             mbar_init(&a_full[p], 8);                        // four warps in each CTA
@@ -116,7 +128,7 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 13) {
+    if (warp == 21) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
@@ -129,17 +141,17 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     bool ok = !*abort_flag;
     int issued = 0;
-    if (warp < 8) {
+    if (warp < 16) {
         // ---- codes to bfloat16
-        const int turn = warp >> 2, r = threadIdx.x & 127;
-        const uint32_t dst = tmem + 384u + (uint32_t)(turn * 64) + ((uint32_t)((warp & 3) * 32) << 16);
+        const int turn = warp >> 3, h = warp >> 2 & 1, r = threadIdx.x & 127;       // every other chunk, one half; place 2 turn + h
+        const uint32_t dst = tmem + 384u + (uint32_t)(turn * 64 + h * 32) + ((uint32_t)((warp & 3) * 32) << 16);
         int s = 0, it = 0;                                   // stage of the chunk, chunks so far
         uint32_t ph = 0, pa = 0;
         for (int tile = pair; tile < tiles && ok; tile += pairs) {
             const int f0 = tile / token_tiles * (2 * FEAT) + rank * FEAT;
             // where the row's scales are: the gate rows lie in one packed tile, the up rows in one or two
             const int rr = !GATED ? r : r < 64 ? (f0 & (MX_ROWS - 1)) + r : (int)(((long)n + f0) & (MX_ROWS - 1)) + r - 64;
-            const int scale_at = x_bytes + (!GATED || r < 64 ? 0 : 1 + (rr >> 7)) * 512 + (int)mx_scale_at(rr & 127);
+            const int scale_at = (!GATED || r < 64 ? 0 : 1 + (rr >> 7)) * 512 + (int)mx_scale_at(rr & 127) + 2 * h;
             for (int c = 0; c < chunks; ++c, ++it) {
                 if ((it & 1) == turn) {
                     if (!mxt_wait(&w_full[s], ph, abort_flag)) {
@@ -147,48 +159,38 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
                         ok = false;
                         break;
                     }
-                    const unsigned char* stage = ring + s * STAGE;
-                    uint4 q[4];
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) q[b] = *reinterpret_cast<const uint4*>(stage + x_bytes + b * 2048 + r * 16);
-                    const uint32_t sc = *reinterpret_cast<const uint32_t*>(stage + scale_at);
-                    // (a byte above 128: its top bit is set, and it is not 128 itself)
-                    const bool large = __any_sync(0xffffffffu, (sc & 0x80808080u & ((sc & 0x7F7F7F7Fu) + 0x7F7F7F7Fu)) != 0);
-                    if (lane == 0) mxt_arrive(&empty_bar[s]);
+                    const unsigned char* stage = w_ring + s * MXP_W_STAGE;
+                    const uint4 qa = *reinterpret_cast<const uint4*>(stage + h * 4096 + r * 16);
+                    const uint4 qb = *reinterpret_cast<const uint4*>(stage + h * 4096 + 2048 + r * 16);
+                    const uint32_t sa = stage[scale_at], sb = stage[scale_at + 1];
+                    const bool large = __any_sync(0xffffffffu, max(sa, sb) > 128u);
+                    if (lane == 0) mxt_arrive(&w_empty[s]);
                     uint32_t v[32];
-                    auto two = [&](int b) {
-                        if (!large) {
-                            mx_block(q[b], mx_factor(sc >> (8 * b) & 255u), v);
-                            mx_block(q[b + 1], mx_factor(sc >> (8 * b + 8) & 255u), v + 16);
-                        } else {
-                            mx_block_large(q[b], sc >> (8 * b) & 255u, v);
-                            mx_block_large(q[b + 1], sc >> (8 * b + 8) & 255u, v + 16);
-                        }
-                    };
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {            // half of the chunk, place 2 turn + h
-                        if (!ok) break;
-                        two(2 * h);
-                        if (!mxt_wait(&a_empty[2 * turn + h], pa ^ 1u, abort_flag)) {
-                            if (lane == 0) mxt_give_up(abort_flag, status);
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        mxt_tmem_st16(dst + (uint32_t)(h * 32), v);
-                        mxt_tmem_st16(dst + (uint32_t)(h * 32 + 16), v + 16);
-                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_leader(&a_full[2 * turn + h]);
+                    if (!large) {
+                        mx_block(qa, mx_factor(sa), v);
+                        mx_block(qb, mx_factor(sb), v + 16);
+                    } else {
+                        mx_block_large(qa, sa, v);
+                        mx_block_large(qb, sb, v + 16);
                     }
-                    if (!ok) break;
+                    if (!mxt_wait(&a_empty[2 * turn + h], pa ^ 1u, abort_flag)) {
+                        if (lane == 0) mxt_give_up(abort_flag, status);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    mxt_tmem_st16(dst, v);
+                    mxt_tmem_st16(dst + 16u, v + 16);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_leader(&a_full[2 * turn + h]);
                     pa ^= 1u;
                 }
-                if (++s == MXP_STAGES) { s = 0; ph ^= 1u; }
+                if (++s == MXP_W_STAGES) { s = 0; ph ^= 1u; }
             }
         }
-    } else if (warp < 12) {
+    } else if (warp < 20) {
         // ---- epilogue
         uint32_t rounds = 0;
         int i = 0;
@@ -205,13 +207,36 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
                                          abort_flag, &acc_empty[b]))
                 break;
         }
-    } else if (warp == 12) {
-        // ---- producer: this CTA's half of the tokens, signalled to the leader, and its rows of W
+    } else if (warp == 20) {
+        // ---- this CTA's half of the tokens, signalled to the leader
+        int s = 0;
+        uint32_t ph = 0;
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+            const int t0 = tile % token_tiles * bn + rank * (bn / 2);
+            for (int c = 0; c < chunks; ++c) {
+                if (!mxt_wait(&x_empty[s], ph ^ 1u, abort_flag)) {
+                    if (lane == 0) mxt_give_up(abort_flag, status);
+                    ok = false;
+                    break;
+                }
+                if (mxt_elect()) {
+                    unsigned char* dst = ring + s * x_bytes;
+                    if (rank == 0) mbar_expect_tx(&x_full[s], 2 * (uint32_t)x_bytes);
+                    tma_load_2d_pair(dst, &map_x, &x_full[s], c * 128, t0);
+                    tma_load_2d_pair(dst + x_bytes / 2, &map_x, &x_full[s], c * 128 + 64, t0);
+                }
+                __syncwarp();
+                ++issued;
+                if (++s == x_stages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 22) {
+        // ---- this CTA's rows of W
         const long tile_bytes = (long)chunks * MX_CHUNK;
         int s = 0;
         uint32_t ph = 0;
         for (int tile = pair; tile < tiles && ok; tile += pairs) {
-            const int t0 = tile % token_tiles * bn + rank * (bn / 2), f0 = tile / token_tiles * (2 * FEAT) + rank * FEAT;
+            const int f0 = tile / token_tiles * (2 * FEAT) + rank * FEAT;
             const long row1 = (long)n + f0;
             const int off0 = f0 & (MX_ROWS - 1), off1 = (int)(row1 & (MX_ROWS - 1)), first = min(64, MX_ROWS - off1);
             const int rest = (row1 / MX_ROWS + 1) * MX_ROWS < 2l * n ? 64 - first : 0;
@@ -220,18 +245,14 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
             // (a CTA whose rows lie behind the last has nothing to load and converts whatever is there: rows that go nowhere)
             const uint32_t w_bytes = f0 >= n ? 0 : !GATED ? MX_CHUNK : 4 * 1024 + 512 + 4 * first * 16 + 512 + (rest ? 4 * rest * 16 + 512 : 0);
             for (int c = 0; c < chunks; ++c) {
-                if (!mxt_wait(&empty_bar[s], ph ^ 1u, abort_flag)) {
+                if (!mxt_wait(&w_empty[s], ph ^ 1u, abort_flag)) {
                     if (lane == 0) mxt_give_up(abort_flag, status);
                     ok = false;
                     break;
                 }
                 if (mxt_elect()) {
-                    unsigned char* dst = ring + s * STAGE;
-                    if (rank == 0) mbar_expect_tx(&x_full[s], 2 * (uint32_t)x_bytes);
+                    unsigned char* dst = w_ring + s * MXP_W_STAGE;
                     mbar_expect_tx(&w_full[s], w_bytes);
-                    tma_load_2d_pair(dst, &map_x, &x_full[s], c * 128, t0);
-                    tma_load_2d_pair(dst + x_bytes / 2, &map_x, &x_full[s], c * 128 + 64, t0);
-                    dst += x_bytes;
                     const uint8_t* src = src0 + (long)c * MX_CHUNK;
                     if (w_bytes == 0) {
                     } else if (!GATED) {
@@ -252,7 +273,7 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
                 }
                 __syncwarp();
                 ++issued;
-                if (++s == MXP_STAGES) { s = 0; ph ^= 1u; }
+                if (++s == MXP_W_STAGES) { s = 0; ph ^= 1u; }
             }
         }
     } else if (rank == 0) {
@@ -261,33 +282,40 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
         const uint64_t half = (uint64_t)(x_bytes / 2) >> 4;
         int s = 0, i = 0, it = 0;
         uint32_t ph = 0;
+        bool there = false;                                  // what the next instructions read is known to be there
         for (int tile = pair; tile < tiles && ok; tile += pairs, ++i) {
             const int b = i & 1;
             ok = mxt_wait(&acc_empty[b], ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag);
-            tc_fence_after();
             const uint32_t acc = tmem + (uint32_t)(b * 192);
             for (int c = 0; c < chunks && ok; ++c, ++it) {
-                const uint32_t turn = (uint32_t)it & 1u;
-                ok = mxt_wait(&x_full[s], ph, abort_flag);
-                const uint64_t bdesc = smem_desc_sw128(ring_at + (uint32_t)(s * STAGE));
+                const uint64_t bdesc = smem_desc_sw128(ring_at + (uint32_t)(s * x_bytes));
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    ok = ok && mxt_wait(&a_full[2 * turn + h], (uint32_t)(it >> 1) & 1u, abort_flag);
-                    if (!ok) break;
+                    const uint32_t place = 2u * ((uint32_t)it & 1u) + (uint32_t)h;
+                    if (!__all_sync(0xffffffffu, there)) {
+                        ok = (h || mxt_wait(&x_full[s], ph, abort_flag)) && mxt_wait(&a_full[place], (uint32_t)(it >> 1) & 1u, abort_flag);
+                        if (!ok) break;
+                    }
                     tc_fence_after();
+                    if (h == 0) {
+                        there = mxt_test(&a_full[place + 1], (uint32_t)(it >> 1) & 1u);
+                    } else {
+                        const int next = s + 1 == x_stages ? 0 : s + 1;
+                        there = mxt_test(&x_full[next], next ? ph : ph ^ 1u) && mxt_test(&a_full[2u * ((uint32_t)(it + 1) & 1u)], (uint32_t)((it + 1) >> 1) & 1u);
+                    }
                     if (mxt_elect()) {
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            mxp_umma_ts(acc, tmem + 384u + turn * 64u + (uint32_t)(h * 32 + kk * 8), bdesc + (uint64_t)(2 * kk) + (h ? half : 0), idesc,
+                            mxp_umma_ts(acc, tmem + 384u + place * 32u + (uint32_t)(kk * 8), bdesc + (uint64_t)(2 * kk) + (h ? half : 0), idesc,
                                         (c > 0 || h > 0 || kk > 0) ? 1u : 0u);
-                        umma_commit_pair(&a_empty[2 * turn + h]);
-                        if (h) umma_commit_pair(&empty_bar[s]);
+                        umma_commit_pair(&a_empty[place]);
+                        if (h) umma_commit_pair(&x_empty[s]);
                         if (h && c == chunks - 1) umma_commit_pair(&acc_full[b]);
                     }
                     __syncwarp();
                 }
                 if (!ok) break;
-                if (++s == MXP_STAGES) { s = 0; ph ^= 1u; }
+                if (++s == x_stages) { s = 0; ph ^= 1u; }
             }
             if (!ok && lane == 0) mxt_give_up(abort_flag, status);
         }
@@ -295,22 +323,34 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 12 && lane == 0 && *abort_flag) {
-        tma_drain(w_full, MXP_STAGES, issued);
-        if (rank == 0) tma_drain(x_full, MXP_STAGES, issued);
-    }
+    if (warp == 20 && lane == 0 && *abort_flag) tma_drain(x_full, rank == 0 ? x_stages : 0, issued);
+    if (warp == 22 && lane == 0 && *abort_flag) tma_drain(w_full, MXP_W_STAGES, issued);
     __syncthreads();
     cluster_sync_all();                                      // neither leaves while the other's MMAs or copies may reach it
-    if (warp == 13) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if (warp == 21) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// Tokens of a tile: the multiple of 32 up to 192 with which the pairs go round their tiles least often (a chunk takes the same time
+// with any: its hand-overs, rather than its MMAs); `rounds`: how often.
+static int mxp_tokens(int m, int row_tiles, int pairs, long* rounds) {
+    int best = 32;
+    long least = 0;
+    for (int bn = 32; bn <= MXP_BN; bn += 32) {
+        const long r = ((long)row_tiles * ((m + bn - 1) / bn) + pairs - 1) / pairs;
+        if (least == 0 || r < least) best = bn, least = r;
+    }
+    *rounds = least;
+    return best;
 }
 
 template <typename TO, bool GATED>
 static int mxp_launch(const void* x, long ldx, const void* w, void* out, long ldo, int m, int n, int k, FlGate act, int num_sms, int* status,
                       cudaStream_t stream) {
-    const int token_tiles = (m + MXP_BN - 1) / MXP_BN, bn = ((m + token_tiles - 1) / token_tiles + 31) / 32 * 32;
-    const int rows = GATED ? 128 : 256;
+    const int rows = GATED ? 128 : 256, chunks = (k + 127) / 128;
+    long rounds;
+    const int bn = mxp_tokens(m, (n + rows - 1) / rows, num_sms / 2, &rounds);
     const long tiles = (long)((n + rows - 1) / rows) * ((m + bn - 1) / bn);
-    if (tiles > 0x3FFFFFFFl || (long)((k + 127) / 128) * 2 > 0x3FFFFFFFl / (tiles / (num_sms / 2) + 1)) return (int)cudaErrorInvalidValue;
+    if (tiles > 0x3FFFFFFFl || rounds * chunks > 0x3FFFFFFFl) return (int)cudaErrorInvalidValue;
     CUtensorMap map;
     int rc = make_map(&map, x, m, k, ldx, bn / 2);
     if (rc) return rc;
@@ -321,6 +361,7 @@ static int mxp_launch(const void* x, long ldx, const void* w, void* out, long ld
         if (e != cudaSuccess) return (int)e;
         configured = true;
     }
+    const int stages = MXP_X_RING / (bn * 128);
     const long pairs = tiles < num_sms / 2 ? tiles : num_sms / 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(2 * pairs));
@@ -333,16 +374,6 @@ static int mxp_launch(const void* x, long ldx, const void* w, void* out, long ld
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, map, (const uint8_t*)w, (TO*)out, ldo, m, n, k, bn, (m + bn - 1) / bn, (int)tiles, act, status);
-}
-
-// As fl_mxt_product (mxfp4_tc.cu), for many tokens.
-FL_API int fl_mxp_product(const void* x, long ldx, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int gated, int act,
-                          float p0, float p1, int num_sms, int* status, cudaStream_t stream) {
-    const FlGate gate = {act, p0, p1};
-    FL_DISPATCH(out_code, TO, {
-        return gated ? mxp_launch<TO, true>(x, ldx, w, out, ldo, m, n, k, gate, num_sms, status, stream)
-                     : mxp_launch<TO, false>(x, ldx, w, out, ldo, m, n, k, gate, num_sms, status, stream);
-    })
-    return (int)cudaErrorInvalidValue;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, map, (const uint8_t*)w, (TO*)out, ldo, m, n, k, bn,
+                                   stages < MXP_X_STAGES ? stages : MXP_X_STAGES, (m + bn - 1) / bn, (int)tiles, act, status);
 }

@@ -11,6 +11,7 @@
 // tensor memory; then they are the epilogue.  Warp 16 sends for the copies, warp 17 issues the MMAs.  Where there are fewer
 // tiles than SMs a cluster of up to 8 CTAs shares K; its partial sums stay in shared memory, and each CTA adds up its share of the
 // tokens from all of them, in rank order.
+#include "mxfp4_pair.cuh"
 #include "mxfp4_tc.cuh"
 
 #define MXT_BN 128                          // most tokens of a tile
@@ -312,8 +313,8 @@ static int mxt_launch_cluster(void (*kernel)(KArgs...), int threads, int smem, d
     return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-// How many CTAs of a cluster share K: the number of least time, which is returned in `time`, in the time of one row tile's chunk;
-// `per`: what a CTA's chunk takes, `fixed`: what a CTA takes besides.  slots[r]: clusters of r CTAs that the device holds at once.
+// How many CTAs of a cluster share K: the number of least time, which is returned in `time`.  `per`: what a CTA's chunk takes, `fixed`:
+// what a CTA takes besides.  slots[r]: clusters of r CTAs that the device holds at once.
 static int mxt_ranks(long tiles, int chunks, const int* slots, int per, int fixed, long* time = nullptr) {
     int best = 1;
     long least = 0;
@@ -351,16 +352,23 @@ static const int* mxt_slots(void (*kernel)(KArgs...), int threads, int smem, int
 
 template <typename TO, bool GATED>
 static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ldo, int m, int n, int k, bool constant_w, FlGate act,
-                      int* status, cudaStream_t stream) {
+                      int which, int num_sms, int* status, cudaStream_t stream) {
     const int token_tiles = (m + MXT_BN - 1) / MXT_BN;
     const int bn = ((m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
     const int row_tiles = (n + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
     const int tokens_y = (m + bn - 1) / bn, chunks = (k + 127) / 128;
-    if (tokens_y > 65535 || row_tiles > 65535) return (int)cudaErrorInvalidValue;
     static int found[9] = {};
     const int* slots = mxt_slots(mxt_kernel<TO, GATED>, MXT_THREADS, MXT_SMEM, found);
     if (!slots) return (int)cudaGetLastError();
-    const int ranks = mxt_ranks((long)tokens_y * row_tiles, chunks, slots, 1, 8);
+    // Both kernels' times in tenths of a microsecond, as measured: here 1.1 us a chunk, 5 us a tile and 2 us besides, on pairs 0.7 us
+    // a chunk and 6 us.  2048 tokens 4096 -> 12288: 224 us here, 180 on pairs; 1024 tokens 4096 -> 4096: 38 and 51; 512 tokens
+    // 11008 -> 4096 (K shared by clusters): 49 and 63.
+    long time, rounds;
+    const int ranks = mxt_ranks((long)tokens_y * row_tiles, chunks, slots, 11, 50, &time);
+    mxp_tokens(m, row_tiles, num_sms / 2, &rounds);
+    if (which == 2 || (which == 0 && m > MXT_BN && 60 + 7 * rounds * chunks < 20 + time))
+        return mxp_launch<TO, GATED>(x, ldx, w, out, ldo, m, n, k, act, num_sms, status, stream);
+    if (tokens_y > 65535 || row_tiles > 65535) return (int)cudaErrorInvalidValue;
     const int per_rank = (chunks + ranks - 1) / ranks;
     int stages = MXT_RING / (bn * 256 + MXT_W_BYTES);
     if (stages > MXT_MAX_STAGES) stages = MXT_MAX_STAGES;
@@ -373,12 +381,13 @@ static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ld
 
 // x: bfloat16 rows, 16-byte aligned, `ldx` elements apart (a multiple of 8).  n: output features (gated: half of w's rows).
 // constant_w: no kernel before this one in the stream writes w, so its first bytes may be read while that one still runs.
+// which: 0 the kernel that takes less time, 1 the one above, 2 the one on pairs of CTAs (mxfp4_pair.cuh).
 FL_API int fl_mxt_product(const void* x, long ldx, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int gated,
-                          int act, float p0, float p1, int constant_w, int* status, cudaStream_t stream) {
+                          int act, float p0, float p1, int constant_w, int which, int num_sms, int* status, cudaStream_t stream) {
     const FlGate gate = {act, p0, p1};
     FL_DISPATCH(out_code, TO, {
-        return gated ? mxt_launch<TO, true>(x, ldx, w, out, ldo, m, n, k, constant_w != 0, gate, status, stream)
-                     : mxt_launch<TO, false>(x, ldx, w, out, ldo, m, n, k, constant_w != 0, gate, status, stream);
+        return gated ? mxt_launch<TO, true>(x, ldx, w, out, ldo, m, n, k, constant_w != 0, gate, which, num_sms, status, stream)
+                     : mxt_launch<TO, false>(x, ldx, w, out, ldo, m, n, k, constant_w != 0, gate, which, num_sms, status, stream);
     })
     return (int)cudaErrorInvalidValue;
 }
@@ -482,13 +491,16 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
         int s = 0;
         uint32_t ph = 0;
         bool going = ok;
+        bool there = false;                                      // the next stage is known to be there
         for (int c = c_begin; c < c_end && going; ++c) {
-            if (!mxt_wait(&full_bar[s], ph, abort_flag)) {
+            if (!__all_sync(0xffffffffu, there) && !mxt_wait(&full_bar[s], ph, abort_flag)) {
                 if (lane == 0) mxt_give_up(abort_flag, status);
                 going = false;
                 break;
             }
             tc_fence_after();
+            const int next = s + 1 == MXQ_STAGES ? 0 : s + 1;
+            there = mxt_test(&full_bar[next], next ? ph : ph ^ 1u);
             const uint32_t at = ring_at + (uint32_t)(s * MXQ_STAGE), sf = tmem_sf + (uint32_t)(s * MXQ_SF);
             if (mxt_elect()) {
                 // (the stage's columns: its last use's MMAs were done before its copies were sent for)

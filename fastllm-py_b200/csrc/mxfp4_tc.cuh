@@ -35,6 +35,20 @@ __device__ __forceinline__ int mxt_warp() { return __shfl_sync(0xffffffffu, (int
 __device__ __forceinline__ void mxt_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// Whether a barrier's phase is complete, without waiting.  A wait costs an issuing warp some 190 clocks even where the phase is
+// complete long since; asked ahead of the matrix instructions that come before it, the answer is there when they have been issued
+// (the pairs' kernel, mxfp4_pair.cu: 672 clocks for a half chunk whose MMAs take 384).
+__device__ __forceinline__ bool mxt_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // lane 0 waits for its warp
 __device__ __forceinline__ bool mxt_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
     uint32_t ok = 1;

@@ -107,9 +107,7 @@ _DEQUANTIZE = ("mxfp4", "fl_mx_dequantize", [c_void_p, c_void_p, c_int, c_long, 
 _FEW = ("mxfp4", "fl_mx_few", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_float, c_float,
                                c_int, c_int, c_void_p])
 _MANY = ("mxfp4_tc", "fl_mxt_product", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_float,
-                                        c_float, c_int, c_void_p, c_void_p])
-_PAIRS = ("mxfp4_pair", "fl_mxp_product", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_float,
-                                           c_float, c_int, c_void_p, c_void_p])
+                                        c_float, c_int, c_int, c_int, c_void_p, c_void_p])
 _BOTH = ("mxfp4_tc", "fl_mxq_product", [c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_void_p, c_void_p])
 
 
@@ -150,12 +148,10 @@ def dequantize(q: Matrix, out: torch.Tensor) -> None:
     ops._check(_fn(_DEQUANTIZE)(data.data_ptr(), out.data_ptr(), code, pitch, q.rows, q.k, stream), "mxfp4.dequantize")
 
 
-import os
-MANY_ROWS = int(os.environ.get('MXP', '256'))
 FEW_ROWS = 8                                    # most rows that the kernel for few of them takes
 
 
-def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, constant_w) -> None:
+def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, constant_w, kernel) -> None:
     pitch, out_pitch = _activations(x), _rows_of(out, "out")
     m, k = x.shape
     if w.k != k or out.shape != (m, n) or (gated and w.rows % 2):
@@ -165,33 +161,30 @@ def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, consta
     stream = _stream_of(x, data, out)
     if m == 0:
         return
-    if m <= FEW_ROWS:
+    if m <= FEW_ROWS and kernel == 0:
         rc = _fn(_FEW)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
                        constant_w, ops.sm_count(x.device), stream)
-    elif m > MANY_ROWS:
-        rc = _fn(_PAIRS)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
-                         ops.sm_count(x.device), _status(x), stream)
     else:
         rc = _fn(_MANY)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
-                        constant_w, _status(x), stream)
+                        constant_w, kernel, ops.sm_count(x.device), _status(x), stream)
     ops._check(rc, name)
 
 
 def linear(x: torch.Tensor, w: Matrix, out: torch.Tensor, activation: str | None = None, params=(0.0, 0.0),
-           constant_w: bool = False) -> None:
+           constant_w: bool = False, kernel: int = 0) -> None:
     """out[m, n] (bfloat16 or float32) = x[m, k] @ w[n, k]^T; x bfloat16 (16-byte aligned, its row pitch a multiple of 8
     elements), products and sums in float.  `activation` (`ops.ACTIVATIONS`, f(v, 1)) is applied on the way out.  `constant_w`
     says that the kernels just before this one in the stream do not write w (a model's matrix), so that its first bytes may be
-    read while they run."""
-    _times_weights("linear", x, w, out, 0, w.rows, activation, params, constant_w)
+    read while they run.  `kernel`: 0 the one that suits the sizes, 1 the tensor-core kernel on tiles, 2 the one on pairs of CTAs."""
+    _times_weights("linear", x, w, out, 0, w.rows, activation, params, constant_w, kernel)
 
 
 def linear_gated(x: torch.Tensor, w: Matrix, out: torch.Tensor, activation: str = "silu", params=(0.0, 0.0),
-                 constant_w: bool = False) -> None:
+                 constant_w: bool = False, kernel: int = 0) -> None:
     """out[m, i] = act(x @ gate^T) * (x @ up^T) for w = [gate; up] stacked as [2 i, k] (any i: the halves' border may lie
     inside a row tile); both products stay in float until the unit (`ops.ACTIVATIONS`, with its `params`) has been applied.
-    `constant_w` as in `linear`."""
-    _times_weights("linear_gated", x, w, out, 1, w.rows // 2, activation, params, constant_w)
+    `constant_w` and `kernel` as in `linear`."""
+    _times_weights("linear_gated", x, w, out, 1, w.rows // 2, activation, params, constant_w, kernel)
 
 
 def product(a: Matrix, b: Matrix, out: torch.Tensor) -> None:
