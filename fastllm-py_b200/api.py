@@ -4,12 +4,14 @@
     new_ids = model.generate(prompt_ids, max_new_tokens=32, temperature=0.7, seed=1)
 
 `Model.load` and `Model.generate` keep the names and meanings of
-fastllm_py/model.py:150-153 and :500-504 where they apply to one GPU and
-unquantised weights: `dtype`, `max_new_tokens`, `temperature`, `use_graph`,
+fastllm_py/model.py:150-153 and :500-504 where they apply to one GPU: `dtype`, `max_new_tokens`, `temperature`, `use_graph`,
 `stop_ids`, `top_p`, `top_k`, `seed`, `min_p`, `repetition_penalty`,
 `frequency_penalty`, `presence_penalty`; generate returns only the new ids and
-includes the stop id.  Options of the reference that select what this engine
-does not have (device maps over several GPUs, INT4/FP8 quantisation, MoE expert
+includes the stop id.  Where the reference quantises to INT4, `weights="mxfp4"` holds
+the matrices of dense attention and feed-forward layers in microscaled 4-bit
+floating point (rounded when the model is loaded; embedding, head and other
+layers' matrices stay as they are stored).  Options of the reference that select what this engine
+does not have (device maps over several GPUs, FP8 quantisation, MoE expert
 placement) do not exist here.  New: a list of prompts generates as one batch
 through the scheduler, and `Model.from_config` makes a model with seeded random
 weights.
@@ -63,12 +65,15 @@ class Model:
         else:
             plan = arch.make_plan(config, names)
         max_len = engine_config.max_model_len or plan.max_positions
-        ctx = BuildContext(dev, dtype, engine_config.page_size, max_len)
+        ctx = BuildContext(dev, dtype, engine_config.page_size, max_len, engine_config.weights)
         decoder = Decoder(plan, ctx)
         from .native import build as native_build
         from .native.libraries import libraries_for
         head_dims = [p.head_dim for p in decoder.all_parts() if hasattr(p, "head_dim")]
         named = [lib for p in decoder.all_parts() for lib in getattr(p, "native_libraries", ())]
+        if engine_config.weights == "mxfp4":
+            from .native.mxfp4 import LIBRARIES
+            named += LIBRARIES
         # builds that a part wants for its own sizes (a kernel compiled per head size, say) join the same parallel build
         sized = [b for p in decoder.all_parts() if hasattr(p, "native_builds") for b in p.native_builds()]
         native_build.compile_many(libraries_for(engine_config.dtype, head_dims, named) + sized)

@@ -7,7 +7,8 @@ In fastllm-py's manner (scripts/generate.py:16-34):
 prints a load line with the architecture summary, the text (or the token ids),
 and `[n tokens in t s = x tok/s]`.  The positional arguments keep the
 reference's order and meaning; `dtype` is `bfloat16` (default here; the
-reference's fp16/INT4 paths do not exist) or `float32`.  Sampling options carry
+reference's fp16 path does not exist) or `float32`; `--weights mxfp4` stands where the reference
+has INT4.  Sampling options carry
 the names of `Model.generate` (fastllm_py/model.py:500-504).  The tokenizer is
 loaded from the model folder when it has one; without tokenizer files give the
 prompt as token ids with --prompt-ids (or --random-prompt N).
@@ -40,6 +41,8 @@ def main(argv=None) -> int:
     ap.add_argument("prompt", nargs="?", default="The capital of France is")
     ap.add_argument("n_new", nargs="?", type=int, default=32, help="tokens to generate")
     ap.add_argument("dtype", nargs="?", default="bfloat16", choices=["bfloat16", "float32", "bf16", "fp32"])
+    ap.add_argument("--weights", default="stored", choices=["stored", "mxfp4"],
+                    help="mxfp4: the dense layers' matrices in 4 bits (bfloat16 only)")
     ap.add_argument("--prompt-ids", help="comma-separated token ids instead of text")
     ap.add_argument("--random-prompt", type=int, metavar="N", help="N random token ids as the prompt")
     ap.add_argument("--temperature", type=float, default=0.0)
@@ -75,11 +78,12 @@ def main(argv=None) -> int:
     t0 = time.time()
     n_prompt = args.random_prompt or len(ids)
     longest = args.max_model_len
-    model = Model.load(args.model_path, dtype=args.dtype, page_size=args.page_size,
+    model = Model.load(args.model_path, dtype=args.dtype, weights=args.weights, page_size=args.page_size,
                        max_tokens=args.max_tokens or max(4096, 2 * (n_prompt + args.n_new)),
                        max_model_len=longest, cuda_graph=not args.no_graph, max_requests=4)
     cfg = model.cfg
-    print(f"[load {time.time() - t0:.1f}s] {cfg.summary()} dtype={model.engine_config.dtype}")
+    print(f"[load {time.time() - t0:.1f}s] {cfg.summary()} dtype={model.engine_config.dtype}"
+          + ("" if args.weights == "stored" else f" weights={args.weights}"))
     if ids is None:
         import numpy as np
 

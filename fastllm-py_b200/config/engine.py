@@ -21,6 +21,7 @@ def canonical_dtype(name: str) -> str:
 @dataclass
 class EngineConfig:
     dtype: str = "bfloat16"           # activations, cache and matrix inputs; "float32" = true 32-bit everywhere
+    weights: str = "stored"           # "mxfp4": matrices of dense attention and feed-forward layers in 4 bits (bfloat16 only)
     page_size: int = 16               # tokens per cache page
     max_tokens: int | None = None     # cache pool size in tokens (None: sized from free device memory)
     memory_fraction: float = 0.85     # share of free device memory the pool may take when max_tokens is None
@@ -35,6 +36,10 @@ class EngineConfig:
 
     def __post_init__(self):
         self.dtype = canonical_dtype(self.dtype)
+        if self.weights not in ("stored", "mxfp4"):
+            raise ValueError(f"weights must be 'stored' or 'mxfp4', got {self.weights!r}")
+        if self.weights == "mxfp4" and self.dtype != "bfloat16":
+            raise ValueError("weights='mxfp4' takes bfloat16 activations: the 32-bit path keeps its matrices as they are stored")
         if self.page_size < 1:
             raise ValueError("page_size must be >= 1")
         if self.max_requests < 1:

@@ -369,8 +369,8 @@ static int mx_launch_few(const bf16* x, long ldx, const uint8_t* w, TO* out, lon
 }
 
 // x: up to 8 bfloat16 rows with `ldx` elements between them (a multiple of 8, from 16 bytes on).  n: output features (gated: half
-// of w's rows).  act: an FlAct or FL_ACT_NONE; a product that is not gated has f(v, 1).  constant_w: no kernel before this one
-// in the stream writes w, so its first bytes may be read while that one still runs.
+// of w's rows).  act: an FlAct or FL_ACT_NONE; a product that is not gated has f(v, 1).  constant_w: nothing that may still
+// run writes w, so its first bytes may be read while the kernels before this one in the stream run.
 FL_API int fl_mx_few(const void* x, long ldx, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int gated,
                      int act, float p0, float p1, int constant_w, int num_sms, cudaStream_t stream) {
     const FlGate gate = {act, p0, p1};

@@ -380,7 +380,7 @@ static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ld
 }
 
 // x: bfloat16 rows, 16-byte aligned, `ldx` elements apart (a multiple of 8).  n: output features (gated: half of w's rows).
-// constant_w: no kernel before this one in the stream writes w, so its first bytes may be read while that one still runs.
+// constant_w: nothing that may still run writes w, so its first bytes may be read while the kernels before this one run.
 // which: 0 the kernel that takes less time, 1 the one above, 2 the one on pairs of CTAs (mxfp4_pair.cuh).
 FL_API int fl_mxt_product(const void* x, long ldx, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int gated,
                           int act, float p0, float p1, int constant_w, int which, int num_sms, int* status, cudaStream_t stream) {

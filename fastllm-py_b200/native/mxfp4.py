@@ -118,13 +118,21 @@ def _fn(which):
     return fn
 
 
-def _status(t: torch.Tensor) -> int:
-    """Address of the device's status word."""
-    found = _fns.get(t.get_device())
+def _status(device: torch.device) -> int:
+    """Address of the word in which kernels record that they gave up (gemm_tc.status_word)."""
+    found = _fns.get(device.index)
     if found is None:
         from . import gemm_tc
-        found = _fns[t.get_device()] = gemm_tc.status_word(t.device).data_ptr()
+        if torch.cuda.is_current_stream_capturing():
+            raise KernelError("mxfp4: run the product once eagerly (or call mxfp4.reserve) before capturing it")
+        found = _fns[device.index] = gemm_tc.status_word(device).data_ptr()
     return found
+
+
+def reserve(device) -> None:
+    """Make what products on `device` share, once, before one is captured into a graph."""
+    device = torch.device(device)
+    _status(device if device.index is not None else torch.device("cuda", torch.cuda.current_device()))
 
 
 def quantize(x: torch.Tensor, out: Matrix) -> None:
@@ -166,7 +174,7 @@ def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, consta
                        constant_w, ops.sm_count(x.device), stream)
     else:
         rc = _fn(_MANY)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
-                        constant_w, kernel, ops.sm_count(x.device), _status(x), stream)
+                        constant_w, kernel, ops.sm_count(x.device), _status(x.device), stream)
     ops._check(rc, name)
 
 
@@ -174,8 +182,8 @@ def linear(x: torch.Tensor, w: Matrix, out: torch.Tensor, activation: str | None
            constant_w: bool = False, kernel: int = 0) -> None:
     """out[m, n] (bfloat16 or float32) = x[m, k] @ w[n, k]^T; x bfloat16 (16-byte aligned, its row pitch a multiple of 8
     elements), products and sums in float.  `activation` (`ops.ACTIVATIONS`, f(v, 1)) is applied on the way out.  `constant_w`
-    says that the kernels just before this one in the stream do not write w (a model's matrix), so that its first bytes may be
-    read while they run.  `kernel`: 0 the one that suits the sizes, 1 the tensor-core kernel on tiles, 2 the one on pairs of CTAs."""
+    says that nothing that may still be running writes w (a model's matrix, written long since), so that its first bytes may be
+    read while the kernels before this one in the stream run.  `kernel`: 0 the one that suits the sizes, 1 the tensor-core kernel on tiles, 2 the one on pairs of CTAs."""
     _times_weights("linear", x, w, out, 0, w.rows, activation, params, constant_w, kernel)
 
 
@@ -194,4 +202,4 @@ def product(a: Matrix, b: Matrix, out: torch.Tensor) -> None:
         raise KernelError(f"mxfp4.product: {a.shape} x {b.shape}^T -> {tuple(out.shape)}")
     code, x, w = ops.dtype_code(out), a.data, b.data
     stream = _stream_of(x, w, out)
-    ops._check(_fn(_BOTH)(x.data_ptr(), w.data_ptr(), out.data_ptr(), code, out_pitch, a.rows, b.rows, a.k, _status(x), stream), "mxfp4.product")
+    ops._check(_fn(_BOTH)(x.data_ptr(), w.data_ptr(), out.data_ptr(), code, out_pitch, a.rows, b.rows, a.k, _status(x.device), stream), "mxfp4.product")

@@ -111,8 +111,8 @@ class Attention(Part):
         mats = [tensors["q"]] if self.shares_cache else [tensors["q"], tensors["k"], tensors["v"]]
         if len({m.dtype for m in mats}) != 1:
             raise ValueError("attention: q, k and v matrices must be stored in one dtype")
-        self.qkv = Linear(mats)
-        self.o = Linear([tensors["o"]])
+        self.qkv = Linear(mats, self.ctx.weights)
+        self.o = Linear([tensors["o"]], self.ctx.weights)
 
     def forward(self, h, out, step, cache: PagedCacheView):
         n = h.shape[0]

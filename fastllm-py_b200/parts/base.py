@@ -64,6 +64,7 @@ class BuildContext:
     dtype: torch.dtype                 # activation / cache dtype: torch.bfloat16 or torch.float32
     page_size: int
     max_positions: int                 # position tables cover [0, max_positions)
+    weights: str = "stored"            # how the matrices of dense attention and feed-forward parts are held: or "mxfp4"
     shared: dict = field(default_factory=dict)   # objects parts may share (position tables by spec)
 
 

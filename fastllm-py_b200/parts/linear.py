@@ -10,6 +10,9 @@ product serves them all, and picks the kernel by operand types:
     those kernels stream fastest (native/gemm_tc.py: PackedWeight), and lets the
     row-major copy go, unless something else reads that copy too (a tied
     embedding table);
+  * bfloat16 activations and a matrix held in 4 bits (`weights="mxfp4"`: rounded when the Linear is made, the
+    stored matrix let go): the kernels of native/mxfp4.py, whose products are left neither in parts nor to the
+    rotary epilogue;
   * anything with a 32-bit operand: the CUDA-core kernel with float
     accumulation (a weight stored in 32-bit stays 32-bit; the true 32-bit path
     never touches a reduced-precision matrix mode).
@@ -22,6 +25,7 @@ from ..native import ops
 
 
 _gemm_tc_module = None
+_mxfp4_module = None
 
 
 def _gemm_tc():
@@ -33,14 +37,30 @@ def _gemm_tc():
     return _gemm_tc_module
 
 
+def _mxfp4():
+    """native/mxfp4.py, likewise."""
+    global _mxfp4_module
+    if _mxfp4_module is None:
+        from ..native import mxfp4
+        _mxfp4_module = mxfp4
+    return _mxfp4_module
+
+
 class Linear:
-    def __init__(self, weights: list):
-        """`weights`: matrices [out_i, in] of one dtype, stacked along out."""
+    def __init__(self, weights: list, held: str = "stored"):
+        """`weights`: matrices [out_i, in] of one dtype, stacked along out.  `held`: "stored", or "mxfp4"."""
         w = weights[0] if len(weights) == 1 else torch.cat(weights, dim=0)
-        self.weight = w.contiguous()          # row-major; None once the tensor-core copy has replaced it
+        self.weight = w.contiguous()          # row-major; None once the tensor-core or the 4-bit copy has replaced it
         self._set_shape(self.weight)
         self.shared = False
         self._tc = None
+        self._q4 = None
+        if held == "mxfp4":
+            from ..native import mxfp4
+            self._q4 = mxfp4.Matrix.of(self.weight)
+            self.weight = None
+        elif held != "stored":
+            raise ValueError(f"a Linear's matrix is held 'stored' or as 'mxfp4', got {held!r}")
 
     @classmethod
     def sharing(cls, weight: torch.Tensor) -> "Linear":
@@ -49,7 +69,7 @@ class Linear:
         self.weight = weight
         self._set_shape(weight)
         self.shared = True
-        self._tc = None
+        self._tc = self._q4 = None
         return self
 
     def _set_shape(self, w: torch.Tensor) -> None:
@@ -62,6 +82,8 @@ class Linear:
         consumer that adds them as it reads: `out` is then not written.  `side`:
         the partial sums go to the second scratch buffer (reserve with `side` too),
         where they outlive the products that follow in the first."""
+        if self._q4 is not None:
+            return _mxfp4().linear(a, self._q4, out, constant_w=True)
         if a.dtype == torch.bfloat16 and self.dtype == torch.bfloat16:
             return self._tensor_core().forward(a, out, defer, side)
         if self.weight is None:
@@ -73,6 +95,9 @@ class Linear:
     def forward_activated(self, a: torch.Tensor, out: torch.Tensor, activation: str, params=(0.0, 0.0)) -> None:
         """out = f(a @ W^T, 1) for an activation of one argument (`native.ops.ACTIVATIONS`): in the tensor-core
         product's epilogue, else by a kernel of its own."""
+        if self._q4 is not None:
+            _mxfp4().linear(a, self._q4, out, activation, params, constant_w=True)
+            return
         if a.dtype == torch.bfloat16 and self.dtype == torch.bfloat16:
             self._tensor_core().forward(a, out, activation=activation, params=params)
             return
@@ -92,7 +117,9 @@ class Linear:
         (pack it, for bfloat16 products) and size the scratch memory that products of up to
         `max_tokens` rows will take, so that nothing has to grow (and no captured graph goes
         stale) once the engine runs."""
-        if activation_dtype == torch.bfloat16 and self.dtype == torch.bfloat16:
+        if self._q4 is not None:
+            _mxfp4().reserve(self.device)
+        elif activation_dtype == torch.bfloat16 and self.dtype == torch.bfloat16:
             from ..native import gemm_tc
             self._tensor_core()
             gemm_tc.reserve(self.device, self.out_features, self.in_features, max_tokens, side)
@@ -103,7 +130,7 @@ class Linear:
         cache write in its epilogue (rotated queries into `q_out`, rotated keys and values into the
         tokens' cache slots), in one tensor-core kernel.  False (nothing done) when that kernel does
         not apply; the caller then takes `forward` and the rotary kernel."""
-        if a.dtype == torch.bfloat16 and self.dtype == torch.bfloat16:
+        if a.dtype == torch.bfloat16 and self._q4 is None and self.dtype == torch.bfloat16:
             return _gemm_tc().gemm_qkv_rope(a, self._tensor_core().weight, q_out, n_heads, n_kv_heads, head_dim, rot_dim,
                                  cos, sin, positions, slots, cache, page_size)
         return False
@@ -112,6 +139,9 @@ class Linear:
         """For a Linear that stacks a gate and an up matrix: out = f(a gate^T, a up^T) (f = act(g) * u, or the
         clamped swish unit with its `params`) in one tensor-core kernel.  False (nothing done) when that kernel does not apply; the
         caller then takes `forward` and the activation kernel."""
+        if self._q4 is not None:
+            _mxfp4().linear_gated(a, self._q4, out, activation, params, constant_w=True)
+            return True
         if a.dtype == torch.bfloat16 and self.dtype == torch.bfloat16:
             return _gemm_tc().gemm_swiglu(a, self._tensor_core().weight, out, activation, params)
         return False

@@ -37,8 +37,8 @@ class SwiGLU(Part):
     def load(self, tensors):
         if tensors["gate"].dtype != tensors["up"].dtype:
             raise ValueError("swiglu: gate and up matrices must be stored in one dtype")
-        self.gate_up = Linear([tensors["gate"], tensors["up"]])
-        self.down = Linear([tensors["down"]])
+        self.gate_up = Linear([tensors["gate"], tensors["up"]], self.ctx.weights)
+        self.down = Linear([tensors["down"]], self.ctx.weights)
 
     def reserve(self, limits):
         for lin in (self.gate_up, self.down):
@@ -85,8 +85,8 @@ class PlainMLP(Part):
         return {"up": (self.inter, self.hidden), "down": (self.hidden, self.inter)}
 
     def load(self, tensors):
-        self.up = Linear([tensors["up"]])
-        self.down = Linear([tensors["down"]])
+        self.up = Linear([tensors["up"]], self.ctx.weights)
+        self.down = Linear([tensors["down"]], self.ctx.weights)
 
     def reserve(self, limits):
         for lin in (self.up, self.down):

@@ -78,3 +78,13 @@ def test_plain_packing_and_its_values_agree():
     unit = np.repeat(2.0 ** (s - 127.0), 32, axis=1)[:, :200]
     assert np.all(np.abs(want - x) <= 2 * unit)
     assert np.all(np.abs(want - x)[np.abs(x) <= 6 * unit] <= unit[np.abs(x) <= 6 * unit])
+
+
+def test_engine_options():
+    from fastllm_py_b200.config import EngineConfig
+
+    assert EngineConfig().weights == "stored" and EngineConfig(weights="mxfp4").dtype == "bfloat16"
+    with pytest.raises(ValueError, match="bfloat16"):
+        EngineConfig(dtype="float32", weights="mxfp4")
+    with pytest.raises(ValueError, match="weights must be"):
+        EngineConfig(weights="int4")

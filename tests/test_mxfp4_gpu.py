@@ -169,6 +169,75 @@ def test_linear(m, n, k, out_dtype):
     check_sum(out[:, :n], x @ w.T, np.abs(x) @ np.abs(w).T, k, out_dtype)
 
 
+@pytest.mark.parametrize("kernel", [1, 2])
+@pytest.mark.parametrize("m, n, k", [(1, 1, 1), (1, 300, 129), (5, 64, 4096), (16, 257, 40), (33, 130, 300), (97, 513, 72), (128, 256, 128), (129, 384, 1000),
+                                     (192, 700, 256), (193, 129, 520), (385, 2300, 136), (600, 1000, 1928)])
+def test_linear_and_gated_on_every_tensor_core_kernel(m, n, k, kernel):
+    """Each of the two kernels for many rows whatever the rule would choose: tiles of tokens that end early, features that end inside
+    a tile, in a pair's second CTA and before it, a gated unit's halves that meet inside a tile, K of one and of many chunks."""
+    from fastllm_py_b200.native import gemm_tc, mxfp4
+
+    x, data, w = operands(m, 2 * n, k, m + n + k)
+    xs = rows_in(x, torch.bfloat16)
+    for out_dtype, wide in ((torch.bfloat16, 3), (torch.float32, 8)):
+        out = torch.full((m, 2 * n + wide), -5.0, dtype=out_dtype, device=DEV)
+        mxfp4.linear(xs, matrix(data, 2 * n, k), out[:, :2 * n], kernel=kernel)
+        act = torch.full((m, n + wide), -5.0, dtype=out_dtype, device=DEV)
+        mxfp4.linear_gated(xs, matrix(data, 2 * n, k), act[:, :n], kernel=kernel)
+        torch.cuda.synchronize()
+        assert int(gemm_tc.status_word(torch.device(DEV)).item()) == 0
+        assert bool((out[:, 2 * n:] == -5.0).all()) and bool((act[:, n:] == -5.0).all())
+        check_sum(out[:, :2 * n], x @ w.T, np.abs(x) @ np.abs(w).T, k, out_dtype)
+        check_gated(act[:, :n], x, w, "silu", (0, 0), k, out_dtype)
+
+
+@pytest.mark.parametrize("kernel", [1, 2])
+def test_products_after_a_recorded_fault_leave_at_once(kernel):
+    """With a fault in the status word every role gives up at its first look: the launches return and write nothing, and the next
+    launch without it works again."""
+    from fastllm_py_b200.native import gemm_tc, mxfp4
+
+    m, n, k = 300, 700, 520
+    x, data, w = operands(m, n, k, 1)
+    xs, q = rows_in(x, torch.bfloat16), matrix(data, n, k)
+    a = mxfp4.Matrix.of(xs.float())
+    word = gemm_tc.status_word(torch.device(DEV))
+    outs = [torch.full((m, c), 7.0, dtype=torch.bfloat16, device=DEV) for c in (n, n // 2, n)]
+    try:
+        word.fill_(101)
+        mxfp4.linear(xs, q, outs[0], kernel=kernel)
+        mxfp4.linear_gated(xs, q, outs[1], kernel=kernel)
+        mxfp4.product(a, q, outs[2])
+        torch.cuda.synchronize()
+        assert int(word.item()) == 101 and all(bool((o == 7.0).all()) for o in outs)
+    finally:
+        word.zero_()
+    mxfp4.linear(xs, q, outs[0], kernel=kernel)
+    check_sum(outs[0], x @ w.T, np.abs(x) @ np.abs(w).T, k, torch.bfloat16)
+
+
+def test_a_first_product_inside_a_capture():
+    """What is made once per device is not made inside a capture: the product is refused there, and works after `reserve`."""
+    from fastllm_py_b200.native import mxfp4
+    from fastllm_py_b200.native.ops import KernelError
+
+    x, data, w = operands(20, 64, 96, 1)
+    xs, q, out = rows_in(x, torch.bfloat16), matrix(data, 64, 96), torch.empty(20, 64, dtype=torch.bfloat16, device=DEV)
+    kept = mxfp4._fns.pop(0, None)
+    graph = torch.cuda.CUDAGraph()
+    refused = False
+    with torch.cuda.graph(graph):
+        xs.add_(0.0)
+        try:
+            mxfp4.linear(xs, q, out)
+        except KernelError:
+            refused = True
+    mxfp4.reserve(DEV)
+    assert refused and mxfp4._fns[0] == (kept or mxfp4._fns[0])
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        mxfp4.linear(xs, q, out)
+
+
 @pytest.mark.parametrize("m, n, k", [s for s in SIZES if s[1] > 1])
 def test_product_of_two_packed_matrices(m, n, k):
     from fastllm_py_b200.native import mxfp4
