@@ -29,7 +29,7 @@
 // The end of a CTA whose sums of `rows` tokens are written, by all its threads: its share of the tokens from all of the cluster's
 // CTAs, by its first WARPS warps.  Leaves with the cluster's sums no longer needed.
 template <typename TO, bool GATED, int FEAT, int PITCH, int WARPS>
-__device__ __forceinline__ void mxt_join(const float* sums, volatile int* abort_flag, int rows, int ranks, int rank, TO* __restrict__ out,
+__device__ __forceinline__ void mxt_join(float* sums, volatile int* abort_flag, int rows, int ranks, int rank, TO* __restrict__ out,
                                          long ldo, int f0, int n, const FlGate act) {
     const int warp = mxt_warp();
     __syncwarp();
@@ -45,8 +45,10 @@ __device__ __forceinline__ void mxt_join(const float* sums, volatile int* abort_
         // a warp takes a token: V features a lane and 32 V a step, or single ones side by side where rows are not aligned
         if ((((uintptr_t)out | (uintptr_t)(ldo * (long)sizeof(TO))) & (V * sizeof(TO) - 1)) == 0 && (n & (V - 1)) == 0)
             mxt_rows<TO, GATED, FEAT, PITCH, V, WARPS>(sums, first + warp, last, ranks, out, ldo, n - f0, act);
-        else
-            mxt_rows<TO, GATED, FEAT, PITCH, 1, WARPS>(sums, first + warp, last, ranks, out, ldo, n - f0, act);
+        else {
+            if (ranks > 1) mxt_gather<(GATED ? 2 : 1) * FEAT, PITCH, WARPS>(sums, first + warp, last, ranks);
+            mxt_rows<TO, GATED, FEAT, PITCH, 1, WARPS>(sums, first + warp, last, 1, out, ldo, n - f0, act);
+        }
     }
     __syncwarp();
     if (ranks > 1) cluster_sync_all();                                // the others may still read this CTA's sums
@@ -313,14 +315,18 @@ static int mxt_launch_cluster(void (*kernel)(KArgs...), int threads, int smem, d
     return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-// How many CTAs of a cluster share K: the number of least time, which is returned in `time`.  `per`: what a CTA's chunk takes, `fixed`:
-// what a CTA takes besides.  slots[r]: clusters of r CTAs that the device holds at once.
-static int mxt_ranks(long tiles, int chunks, const int* slots, int per, int fixed, long* time = nullptr) {
+// How many CTAs of a cluster share K: the number of least time, which is returned in `time`, in units of 10 ns.  `per`: what a CTA's
+// chunk takes.  A tile takes 5 us besides, and each CTA of a cluster 3.6 ns more for a token, whose sums have to be joined; clusters
+// of a number that is no power of two start later.  128 tokens 4096 -> 4096: 37 us with one CTA a tile, 23.5 with two, 17.3 with four,
+// 17.9 with six, 31.9 with eight (two rounds); 128 x 1000 x 1536 in 4 bits: 8.5, 8.6, 9.1, 11.0 and 11.7.
+// slots[r]: clusters of r CTAs that the device holds at once.
+static int mxt_ranks(long tiles, int chunks, int tokens, const int* slots, int per, long* time = nullptr) {
     int best = 1;
     long least = 0;
     for (int r = 1; r <= 8 && r <= chunks; ++r) {
         if (slots[r] < 1) continue;
-        const long t = (tiles + slots[r] - 1) / slots[r] * ((chunks + r - 1) / r * per + fixed);
+        const long tile = (long)((chunks + r - 1) / r) * per + 500 + (long)r * tokens * 36 / 100 + (r & (r - 1) ? 150 : 0);
+        const long t = (tiles + slots[r] - 1) / slots[r] * tile;
         if (least == 0 || t < least) best = r, least = t;
     }
     if (time) *time = least;
@@ -360,13 +366,13 @@ static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ld
     static int found[9] = {};
     const int* slots = mxt_slots(mxt_kernel<TO, GATED>, MXT_THREADS, MXT_SMEM, found);
     if (!slots) return (int)cudaGetLastError();
-    // Both kernels' times in tenths of a microsecond, as measured: here 1.1 us a chunk, 5 us a tile and 2 us besides, on pairs 0.7 us
-    // a chunk and 6 us.  2048 tokens 4096 -> 12288: 224 us here, 180 on pairs; 1024 tokens 4096 -> 4096: 38 and 51; 512 tokens
+    // Both kernels' times, as measured: here 1.1 us a chunk, what mxt_ranks says and 2 us besides, on pairs 0.7 us
+    // a chunk and 6 us, and 8 more where a pair has one tile, whose epilogue nothing hides.  2048 tokens 4096 -> 12288: 224 us here, 180 on pairs; 1024 tokens 4096 -> 4096: 38 and 51; 512 tokens
     // 11008 -> 4096 (K shared by clusters): 49 and 63.
     long time, rounds;
-    const int ranks = mxt_ranks((long)tokens_y * row_tiles, chunks, slots, 11, 50, &time);
+    const int ranks = mxt_ranks((long)tokens_y * row_tiles, chunks, bn, slots, 110, &time);
     mxp_tokens(m, row_tiles, num_sms / 2, &rounds);
-    if (which == 2 || (which == 0 && m > MXT_BN && 60 + 7 * rounds * chunks < 20 + time))
+    if (which == 2 || (which == 0 && m > MXT_BN && 600 + 70 * rounds * chunks + (rounds == 1 ? 800 : 0) < 200 + time))
         return mxp_launch<TO, GATED>(x, ldx, w, out, ldo, m, n, k, act, num_sms, status, stream);
     if (tokens_y > 65535 || row_tiles > 65535) return (int)cudaErrorInvalidValue;
     const int per_rank = (chunks + ranks - 1) / ranks;
@@ -535,7 +541,7 @@ FL_API int fl_mxq_product(const void* a, const void* w, void* out, int out_code,
         static int found[9] = {};
         const int* slots = mxt_slots(mxq_kernel<TO>, MXT_THREADS, MXQ_SMEM, found);
         if (!slots) return (int)cudaGetLastError();
-        const int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, slots, 1, 8);
+        const int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, m < 128 ? m : 128, slots, 35);
         const int per_rank = (chunks + ranks - 1) / ranks;
         return mxt_launch_cluster(mxq_kernel<TO>, MXT_THREADS, MXQ_SMEM, dim3(ranks, token_tiles, row_tiles), stream, (const uint8_t*)a,
                                   (const uint8_t*)w, (TO*)out, ldo, m, n, chunks, ranks, per_rank, status);

@@ -123,6 +123,25 @@ __device__ __forceinline__ void mxt_rows(const float* sums, int t, int last, int
     }
 }
 
+// The same tokens' sums over the cluster left in this CTA's own rows, which no other CTA reads: for rows that leave an element at a
+// time, since single elements from another CTA take as long as four (261 x 1000 x 1537 in 4 bits: 10.0 us, and 5 of them here).
+template <int WIDTH, int PITCH, int STEP>
+__device__ __forceinline__ void mxt_gather(float* sums, int t, int last, int ranks) {
+#pragma unroll 2
+    for (; t < last; t += STEP)
+#pragma unroll
+        for (int p = 0; p < WIDTH; p += 128) {
+            float* at = sums + t * PITCH + p + (threadIdx.x & 31) * 4;
+            float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+            for (int q = 0; q < ranks; ++q) {
+                const MxtVec<4> x = mxt_get<4>(at, ranks, q);
+                r.x += x.v[0], r.y += x.v[1], r.z += x.v[2], r.w += x.v[3];
+            }
+            *reinterpret_cast<float4*>(at) = r;
+        }
+    __syncwarp();
+}
 __device__ __forceinline__ void mxt_give_up(volatile int* abort_flag, int* status) {
     if (!*abort_flag) {
         *abort_flag = 1;
