@@ -77,24 +77,24 @@ def _stream_of(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor) -> int:
 
 def _rows_of(t: torch.Tensor, what: str) -> int:
     """Elements between the rows of a 2-D tensor whose rows are dense and do not overlap."""
-    if t.dim() != 2:
+    stride = t.stride()
+    if len(stride) == 2 and stride[1] == 1 and stride[0] >= t.shape[1]:
+        return stride[0]
+    if len(stride) != 2:
         raise KernelError(f"mxfp4: {what} is a matrix, got shape {tuple(t.shape)}")
     rows, cols = t.shape
-    pitch, step = t.stride()
-    if step != 1 and cols > 1:
+    if stride[1] != 1 and cols > 1:
         raise KernelError(f"mxfp4: the rows of {what} must be contiguous")
-    if pitch < cols:
-        if rows > 1:
-            raise KernelError(f"mxfp4: the rows of {what} overlap")
-        return cols
-    return pitch
+    if stride[0] < cols and rows > 1:
+        raise KernelError(f"mxfp4: the rows of {what} overlap")
+    return max(stride[0], cols)
 
 
 def _activations(x: torch.Tensor) -> int:
     pitch = _rows_of(x, "x")
     if x.dtype is not torch.bfloat16:
         raise KernelError(f"mxfp4: activations are bfloat16, got {x.dtype}")
-    if x.shape[0] == 1:
+    if pitch % 8 and x.shape[0] == 1:
         pitch = -(-pitch // 8) * 8                               # (a single row has no pitch)
     if pitch % 8 or x.data_ptr() % 16:
         raise KernelError("mxfp4: activations must be 16-byte aligned with a row pitch that is a multiple of 8 elements")
@@ -118,41 +118,38 @@ def _fn(which):
     return fn
 
 
-def _status(device: torch.device) -> int:
-    """Address of the word in which kernels record that they gave up (gemm_tc.status_word)."""
-    found = _fns.get(device.index)
+def _known(t: torch.Tensor):
+    """(address of the word in which kernels record that they gave up, gemm_tc.status_word, and number of SMs) of t's device."""
+    found = _fns.get(t.get_device())
     if found is None:
         from . import gemm_tc
         if torch.cuda.is_current_stream_capturing():
             raise KernelError("mxfp4: run the product once eagerly (or call mxfp4.reserve) before capturing it")
-        found = _fns[device.index] = gemm_tc.status_word(device).data_ptr()
+        found = _fns[t.get_device()] = (gemm_tc.status_word(t.device).data_ptr(), ops.sm_count(t.device))
     return found
 
 
 def reserve(device) -> None:
     """Make what products on `device` share, once, before one is captured into a graph."""
-    device = torch.device(device)
-    _status(device if device.index is not None else torch.device("cuda", torch.cuda.current_device()))
+    _known(torch.empty(0, device=device))
 
 
 def quantize(x: torch.Tensor, out: Matrix) -> None:
     """out = x [rows, k] (float32 or bfloat16) rounded to nearest, ties to even codes; a block's scale is the power of two that
     puts its largest magnitude into [4, 8) (the codes end at 6), a block that holds a NaN or an infinity becomes NaN."""
-    pitch = _rows_of(x, "x")
+    pitch, data = _rows_of(x, "x"), out.data
     if x.shape != out.shape:
         raise KernelError(f"mxfp4.quantize: {tuple(x.shape)} into {out.shape}")
-    code, data = ops.dtype_code(x), out.data
-    stream = _stream_of(x, data, data)
+    code, stream = ops.dtype_code(x), _stream_of(x, data, data)
     ops._check(_fn(_QUANTIZE)(x.data_ptr(), code, pitch, data.data_ptr(), out.rows, out.k, stream), "mxfp4.quantize")
 
 
 def dequantize(q: Matrix, out: torch.Tensor) -> None:
     """out [rows, k] (float32 or bfloat16) = the values that q stands for, exact in both types."""
-    pitch = _rows_of(out, "out")
+    pitch, data = _rows_of(out, "out"), q.data
     if out.shape != q.shape:
         raise KernelError(f"mxfp4.dequantize: {q.shape} into {tuple(out.shape)}")
-    code, data = ops.dtype_code(out), q.data
-    stream = _stream_of(data, out, out)
+    code, stream = ops.dtype_code(out), _stream_of(data, out, out)
     ops._check(_fn(_DEQUANTIZE)(data.data_ptr(), out.data_ptr(), code, pitch, q.rows, q.k, stream), "mxfp4.dequantize")
 
 
@@ -160,21 +157,21 @@ FEW_ROWS = 8                                    # most rows that the kernel for 
 
 
 def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, constant_w, kernel) -> None:
-    pitch, out_pitch = _activations(x), _rows_of(out, "out")
+    pitch, out_pitch, data = _activations(x), _rows_of(out, "out"), w.data
     m, k = x.shape
     if w.k != k or out.shape != (m, n) or (gated and w.rows % 2):
         raise KernelError(f"mxfp4.{name}: {tuple(x.shape)} x {w.shape}^T -> {tuple(out.shape)}")
     act = -1 if activation is None else ops.activation_code(activation)
-    code, data = ops.dtype_code(out), w.data
-    stream = _stream_of(x, data, out)
+    code, stream = ops.dtype_code(out), _stream_of(x, data, out)
     if m == 0:
         return
+    status, sms = _known(x)
     if m <= FEW_ROWS and kernel == 0:
         rc = _fn(_FEW)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
-                       constant_w, ops.sm_count(x.device), stream)
+                       constant_w, sms, stream)
     else:
         rc = _fn(_MANY)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
-                        constant_w, kernel, ops.sm_count(x.device), _status(x.device), stream)
+                        constant_w, kernel, sms, status, stream)
     ops._check(rc, name)
 
 
@@ -202,4 +199,4 @@ def product(a: Matrix, b: Matrix, out: torch.Tensor) -> None:
         raise KernelError(f"mxfp4.product: {a.shape} x {b.shape}^T -> {tuple(out.shape)}")
     code, x, w = ops.dtype_code(out), a.data, b.data
     stream = _stream_of(x, w, out)
-    ops._check(_fn(_BOTH)(x.data_ptr(), w.data_ptr(), out.data_ptr(), code, out_pitch, a.rows, b.rows, a.k, _status(x.device), stream), "mxfp4.product")
+    ops._check(_fn(_BOTH)(x.data_ptr(), w.data_ptr(), out.data_ptr(), code, out_pitch, a.rows, b.rows, a.k, _known(x)[0], stream), "mxfp4.product")
