@@ -1,4 +1,5 @@
-// Products of many rows with a matrix in microscaled 4-bit floating point on pairs of CTAs (cta_group::2): prompts.
+// Products of many rows with a matrix in microscaled 4-bit floating point on pairs of CTAs (cta_group::2): prompts.  First bfloat16 rows;
+// rows in 4 bits themselves at the end.
 //
 // A pair's tile is 256 rows of W x up to 192 tokens.  Each CTA turns its 128 rows of W into bfloat16 in its own tensor memory (as
 // mxfp4_tc.cu does) and loads half of the tokens; the MMA reads both halves, so a CTA moves and converts half of what two CTAs with
@@ -376,4 +377,258 @@ static int mxp_launch(const void* x, long ldx, const void* w, void* out, long ld
     cfg.numAttrs = 1;
     return (int)cudaLaunchKernelEx(&cfg, kernel, map, (const uint8_t*)w, (TO*)out, ldo, m, n, k, bn,
                                    stages < MXP_X_STAGES ? stages : MXP_X_STAGES, (m + bn - 1) / bn, (int)tiles, act, status);
+}
+
+// ---------------------------------------------------------------- both operands in 4 bits
+// A pair's tile is 256 rows of W x 256 tokens, two packed tiles of each: a CTA copies one of W and one of A, in stages of two chunks
+// (256 along K) that lie side by side in the packed form, one copy each, and the other CTA's tokens' scales.  A stage's MMAs take 512
+// clocks and its 35 KB from L2 about as long, where single CTAs with tiles of 256 x 128 read 52 KB for half of the products.  Tensor
+// memory holds one accumulator and the scales of every stage.
+//
+// Warps 0-15, four of them a stage, move the scales (a lane 16 bytes of each block of them; every quarter of the lanes has all); warps
+// 16-23 are the epilogue, in two groups; warp 24 sends for the copies, warp 25 of the leader issues the MMAs.
+#define MXQP_STAGES 5
+#define MXQP_STAGE (4 * MX_CHUNK + 1024)
+#define MXQP_SF 24                                       // columns of a stage's scales: 4 of W and 8 of the tokens for each chunk
+#define MXQP_SMEM (MXQP_STAGES * MXQP_STAGE + 2 * MXP_ROUND + 1024)
+#define MXQP_THREADS (26 * 32)
+
+__device__ __forceinline__ void mxqp_umma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                          uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mxqp_st4(uint32_t taddr, const uint4 v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// A barrier of the epilogue's group `group`, and whether any of its threads came with `flag`.
+__device__ __forceinline__ bool mxqp_vote(bool flag, int group) {
+    uint32_t any;
+    __syncwarp();
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, %2, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"((uint32_t)flag), "r"(2 + group)
+        : "memory");
+    return any != 0;
+}
+
+// tiles: row pairs x token pairs (two packed tiles each).
+template <typename TO>
+__global__ void __launch_bounds__(MXQP_THREADS, 1)
+mxqp_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __restrict__ out, long ldo, int m, int n, int chunks,
+            int token_pairs, int tiles, int* __restrict__ status) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* ring = (unsigned char*)(((uintptr_t)smem_raw + 127) & ~(uintptr_t)127);
+    float* staged = reinterpret_cast<float*>(ring + MXQP_STAGES * MXQP_STAGE);
+    uint64_t* full_bar = (uint64_t*)(staged + 2 * (MXP_ROUND / 4));
+    uint64_t* empty_bar = full_bar + MXQP_STAGES;
+    uint64_t* scales_bar = empty_bar + MXQP_STAGES;              // (the leader's)
+    uint64_t* acc_full = scales_bar + MXQP_STAGES;
+    uint64_t* acc_empty = acc_full + 1;                          // (the leader's)
+    uint32_t* tmem_slot = (uint32_t*)(acc_empty + 1);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    const int warp = mxt_warp(), lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank(), pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+    const int steps = (chunks + 1) / 2;                          // stages of a tile
+    const int last_w = (n - 1) / MX_ROWS, last_a = (m - 1) / MX_ROWS;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < MXQP_STAGES; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+            mbar_init(&scales_bar[s], 8);                        // four warps in each CTA
+        }
+        mbar_init(acc_full, 1);
+        mbar_init(acc_empty, 16);                                // eight warps in each CTA
+        *abort_flag = (*(volatile int*)status != 0) ? 1 : 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 25) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();                                          // both CTAs' barriers exist before anyone signals them
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_sf = tmem + 256u;
+    bool ok = !*abort_flag;
+    int issued = 0;
+    if (warp < 16) {
+        // ---- scales to tensor memory, every fourth stage
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        int it = 0;
+        for (int tile = pair; tile < tiles && ok; tile += pairs)
+            for (int step = 0; step < steps; ++step, ++it) {
+                if ((it & 3) != warp >> 2) continue;
+                const int s = it % MXQP_STAGES;
+                if (!mxt_wait(&full_bar[s], (uint32_t)(it / MXQP_STAGES) & 1u, abort_flag)) {
+                    if (lane == 0) mxt_give_up(abort_flag, status);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();                                // (the stage's columns: its last use's MMAs were done before it was filled again)
+                const unsigned char* stage = ring + s * MXQP_STAGE;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    if (2 * step + c >= chunks) break;
+                    const uint32_t at = tmem_sf + lanes + (uint32_t)(s * MXQP_SF + c * 12);
+                    const uint4 own = *reinterpret_cast<const uint4*>(stage + 2 * MX_CHUNK + c * MX_CHUNK + MX_CODES + lane * 16);
+                    const uint4 peer = *reinterpret_cast<const uint4*>(stage + 4 * MX_CHUNK + c * 512 + lane * 16);
+                    mxqp_st4(at, *reinterpret_cast<const uint4*>(stage + c * MX_CHUNK + MX_CODES + lane * 16));
+                    mxqp_st4(at + 4u, rank ? peer : own);
+                    mxqp_st4(at + 8u, rank ? own : peer);
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_leader(&scales_bar[s]);
+            }
+    } else if (warp < 24) {
+        // ---- epilogue: two groups of four warps, every other 32 tokens
+        const int group = (warp >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
+        float* mine = staged + group * (MXP_ROUND / 4);
+        int i = 0;
+        for (int tile = pair; tile < tiles; tile += pairs, ++i) {
+            if (ok && !mxt_wait(acc_full, (uint32_t)i & 1u, abort_flag)) {
+                if (lane == 0) mxt_give_up(abort_flag, status);
+                ok = false;
+            }
+            if (mxqp_vote(!ok, group)) break;
+            tc_fence_after();
+            const int t0 = tile % token_pairs * 256, f0 = tile / token_pairs * 256 + rank * 128, tokens = min(256, m - t0), left = n - f0;
+            TO* dst = out + (long)t0 * ldo + f0;
+            const bool vec = (((uintptr_t)dst | (uintptr_t)(ldo * (long)sizeof(TO))) & (4 * sizeof(TO) - 1)) == 0 && (n & 3) == 0;
+            bool going = true;
+            for (int t = 32 * group; t < 256 && going; t += 64) {
+                uint32_t v[32];
+                tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)t, v);
+                tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(t + 16), v + 16);
+                tmem_ld_wait();
+                if (t + 64 >= 256) {                             // this group has read its part of the accumulator
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_leader(acc_empty);
+                }
+                if (t >= tokens || left <= 0) continue;          // (the same in the whole group)
+                if (mxqp_vote(false, group)) going = false;      // the last round's rows have left
+#pragma unroll
+                for (int j = 0; j < 32; ++j) mine[j * 128 + r] = __uint_as_float(v[j]);
+                if (mxqp_vote(*abort_flag != 0, group)) going = false;
+                if (!going) break;
+                const int last = min(32, tokens - t);
+                if (vec) mxt_rows<TO, false, 128, 128, 4, 4>(mine, quarter, last, 1, dst + (long)t * ldo, ldo, left, FlGate{FL_ACT_NONE, 0.0f, 0.0f});
+                else mxt_rows<TO, false, 128, 128, 1, 4>(mine, quarter, last, 1, dst + (long)t * ldo, ldo, left, FlGate{FL_ACT_NONE, 0.0f, 0.0f});
+            }
+            if (!going) break;
+        }
+    } else if (warp == 24) {
+        // ---- producer: a tile of W, a tile of A, the other CTA's tokens' scales (tiles that do not exist: the last one again, whose
+        // sums go nowhere)
+        int s = 0;
+        uint32_t ph = 0;
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+            const long tile_bytes = (long)chunks * MX_CHUNK;
+            const int wt = tile / token_pairs * 2 + rank, at = tile % token_pairs * 2;
+            const uint8_t* src_w = w + min(wt, last_w) * tile_bytes;
+            const uint8_t* src_a = a + min(at + rank, last_a) * tile_bytes;
+            const uint8_t* src_p = a + min(at + 1 - rank, last_a) * tile_bytes + MX_CODES;
+            for (int step = 0; step < steps; ++step) {
+                if (!mxt_wait(&empty_bar[s], ph ^ 1u, abort_flag)) {
+                    if (lane == 0) mxt_give_up(abort_flag, status);
+                    ok = false;
+                    break;
+                }
+                if (mxt_elect()) {
+                    unsigned char* dst = ring + s * MXQP_STAGE;
+                    const int two = 2 * step + 1 < chunks ? 2 : 1;
+                    const long at_k = 2l * step * MX_CHUNK;
+                    mbar_expect_tx(&full_bar[s], (uint32_t)(two * (2 * MX_CHUNK + 512)));
+                    mxt_copy(dst, src_w + at_k, (uint32_t)(two * MX_CHUNK), &full_bar[s]);
+                    mxt_copy(dst + 2 * MX_CHUNK, src_a + at_k, (uint32_t)(two * MX_CHUNK), &full_bar[s]);
+                    mxt_copy(dst + 4 * MX_CHUNK, src_p + at_k, 512, &full_bar[s]);
+                    if (two == 2) mxt_copy(dst + 4 * MX_CHUNK + 512, src_p + at_k + MX_CHUNK, 512, &full_bar[s]);
+                }
+                __syncwarp();
+                ++issued;
+                if (++s == MXQP_STAGES) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (rank == 0) {
+        // ---- MMA issuer, for both CTAs.  (A stage's scales are in tensor memory once its copies have come, in either CTA.)
+        const uint32_t idesc[2] = {mxq_idesc(256, 256, 0), mxq_idesc(256, 256, 2)}, ring_at = smem_u32(ring);
+        int s = 0, i = 0;
+        uint32_t ph = 0;
+        bool there = false;                                      // the next stage is known to be there
+        for (int tile = pair; tile < tiles && ok; tile += pairs, ++i) {
+            ok = mxt_wait(acc_empty, ((uint32_t)i & 1u) ^ 1u, abort_flag);
+            for (int step = 0; step < steps && ok; ++step) {
+                if (!__all_sync(0xffffffffu, there)) ok = mxt_wait(&scales_bar[s], ph, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                const int next = s + 1 == MXQP_STAGES ? 0 : s + 1;
+                there = mxt_test(&scales_bar[next], next ? ph : ph ^ 1u);
+                const uint32_t at = ring_at + (uint32_t)(s * MXQP_STAGE), sf = tmem_sf + (uint32_t)(s * MXQP_SF);
+                if (mxt_elect()) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        if (2 * step + c >= chunks) break;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            mxqp_umma(tmem, mxq_desc(at + (uint32_t)(c * MX_CHUNK + h * 4096), 2048),
+                                      mxq_desc(at + (uint32_t)((2 + c) * MX_CHUNK + h * 4096), 2048), idesc[h], sf + (uint32_t)(c * 12),
+                                      sf + (uint32_t)(c * 12 + 4), (step > 0 || c > 0 || h > 0) ? 1u : 0u);
+                    }
+                    umma_commit_pair(&empty_bar[s]);
+                    if (step == steps - 1) umma_commit_pair(acc_full);
+                }
+                __syncwarp();
+                if (++s == MXQP_STAGES) { s = 0; ph ^= 1u; }
+            }
+            if (!ok && lane == 0) mxt_give_up(abort_flag, status);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 24 && lane == 0 && *abort_flag) tma_drain(full_bar, MXQP_STAGES, issued);
+    __syncthreads();
+    cluster_sync_all();                                          // neither leaves while the other's MMAs or copies may reach it
+    if (warp == 25) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+template <typename TO>
+static int mxqp_launch(const void* a, const void* w, void* out, long ldo, int m, int n, int k, int num_sms, int* status, cudaStream_t stream) {
+    const int chunks = (k + 127) / 128, token_pairs = (m + 255) / 256;
+    const long tiles = (long)((n + 255) / 256) * token_pairs, pairs = tiles < num_sms / 2 ? tiles : num_sms / 2;
+    if (tiles > 0x3FFFFFFFl || (tiles / pairs + 1) * ((chunks + 1) / 2) > 0x3FFFFFFFl) return (int)cudaErrorInvalidValue;
+    auto kernel = mxqp_kernel<TO>;
+    static bool configured = false;
+    if (!configured) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MXQP_SMEM);
+        if (e != cudaSuccess) return (int)e;
+        configured = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * pairs));
+    cfg.blockDim = dim3(MXQP_THREADS);
+    cfg.dynamicSmemBytes = MXQP_SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, (const uint8_t*)a, (const uint8_t*)w, (TO*)out, ldo, m, n, chunks, token_pairs, (int)tiles, status);
 }

@@ -408,17 +408,8 @@ FL_API int fl_mxt_product(const void* x, long ldx, const void* w, void* out, int
 #define MXQ_SF 12                                              // columns of a stage's scales
 #define MXQ_SMEM (MXQ_STAGES * MXQ_STAGE + 1024)
 
-// no swizzle: `lead` bytes between core matrices along K, 128 between those of neighbouring groups of 8 rows
-__device__ __forceinline__ uint64_t mxq_desc(uint32_t saddr, uint32_t lead) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
-}
 __device__ __forceinline__ void mxq_copy_scales(uint32_t taddr, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-// float accumulator; A and B e2m1 with a scale 2^(s - 127) for 32 elements, which of the four bytes of a scale column `id` (0 or 2) and
-// the next one are
-__device__ __forceinline__ uint32_t mxq_idesc(int n, int id) {
-    return (uint32_t)id << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | 1u << 23 | (uint32_t)(128 >> 4) << 24 | (uint32_t)id << 29;
 }
 __device__ __forceinline__ void mxq_umma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                          uint32_t accumulate) {
@@ -493,7 +484,7 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
         }
     } else if (warp == MXT_WARPS + 1) {
         const int bn = (rows + 15) / 16 * 16;
-        const uint32_t idesc[2] = {mxq_idesc(bn, 0), mxq_idesc(bn, 2)}, ring_at = smem_u32(ring);
+        const uint32_t idesc[2] = {mxq_idesc(128, bn, 0), mxq_idesc(128, bn, 2)}, ring_at = smem_u32(ring);
         int s = 0;
         uint32_t ph = 0;
         bool going = ok;
@@ -532,16 +523,21 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
     if (warp == MXT_WARPS + 1) tmem_dealloc(tmem_d, 512);
 }
 
-// a [m, k] and w [n, k] packed.
-FL_API int fl_mxq_product(const void* a, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int* status,
-                          cudaStream_t stream) {
+// a [m, k] and w [n, k] packed.  which: 0 the kernel that takes less time, 1 the one above, 2 the one on pairs of CTAs
+// (mxfp4_pair.cuh).
+FL_API int fl_mxq_product(const void* a, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int which, int num_sms,
+                          int* status, cudaStream_t stream) {
     const int chunks = (k + 127) / 128, token_tiles = (m + 127) / 128, row_tiles = (n + 255) / 256;
-    if (token_tiles > 65535 || row_tiles > 65535) return (int)cudaErrorInvalidValue;
     FL_DISPATCH(out_code, TO, {
         static int found[9] = {};
         const int* slots = mxt_slots(mxq_kernel<TO>, MXT_THREADS, MXQ_SMEM, found);
         if (!slots) return (int)cudaGetLastError();
-        const int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, m < 128 ? m : 128, slots, 35);
+        long time;
+        const int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, m < 128 ? m : 128, slots, 35, &time);
+        const long rounds = ((long)row_tiles * ((token_tiles + 1) / 2) + num_sms / 2 - 1) / (num_sms / 2);
+        if (which == 2 || (which == 0 && m > 128 && 600 + rounds * (chunks * 17 + 200) < 200 + time))
+            return mxqp_launch<TO>(a, w, out, ldo, m, n, k, num_sms, status, stream);
+        if (token_tiles > 65535 || row_tiles > 65535) return (int)cudaErrorInvalidValue;
         const int per_rank = (chunks + ranks - 1) / ranks;
         return mxt_launch_cluster(mxq_kernel<TO>, MXT_THREADS, MXQ_SMEM, dim3(ranks, token_tiles, row_tiles), stream, (const uint8_t*)a,
                                   (const uint8_t*)w, (TO*)out, ldo, m, n, chunks, ranks, per_rank, status);

@@ -154,3 +154,14 @@ __device__ __forceinline__ void mxt_copy(void* dst, const void* src, uint32_t by
                  "r"(bytes), "r"(smem_u32(bar))
                  : "memory");
 }
+
+// ------------------------------------------------------------------ both operands in 4 bits
+// A tile's codes as an operand of the block-scaled matrix instruction: no swizzle: `lead` bytes between core matrices along K, 128 between those of neighbouring groups of 8 rows
+__device__ __forceinline__ uint64_t mxq_desc(uint32_t saddr, uint32_t lead) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+// float accumulator; A and B e2m1 with a scale 2^(s - 127) for 32 elements, which of the four bytes of a scale column `id` (0 or 2) and
+// the next one are
+__device__ __forceinline__ uint32_t mxq_idesc(int m, int n, int id) {
+    return (uint32_t)id << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | 1u << 23 | (uint32_t)(m >> 4) << 24 | (uint32_t)id << 29;
+}

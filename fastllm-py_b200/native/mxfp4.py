@@ -108,7 +108,7 @@ _FEW = ("mxfp4", "fl_mx_few", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_lo
                                c_int, c_int, c_void_p])
 _MANY = ("mxfp4_tc", "fl_mxt_product", [c_void_p, c_long, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_float,
                                         c_float, c_int, c_int, c_int, c_void_p, c_void_p])
-_BOTH = ("mxfp4_tc", "fl_mxq_product", [c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_void_p, c_void_p])
+_BOTH = ("mxfp4_tc", "fl_mxq_product", [c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p])
 
 
 def _fn(which):
@@ -192,11 +192,14 @@ def linear_gated(x: torch.Tensor, w: Matrix, out: torch.Tensor, activation: str 
     _times_weights("linear_gated", x, w, out, 1, w.rows // 2, activation, params, constant_w, kernel)
 
 
-def product(a: Matrix, b: Matrix, out: torch.Tensor) -> None:
-    """out[m, n] (bfloat16 or float32) = a[m, k] @ b[n, k]^T, both in 4 bits; sums in float."""
+def product(a: Matrix, b: Matrix, out: torch.Tensor, kernel: int = 0) -> None:
+    """out[m, n] (bfloat16 or float32) = a[m, k] @ b[n, k]^T, both in 4 bits; sums in float.  `kernel`: 0 the one that suits the
+    sizes, 1 the one on tiles, 2 the one on pairs of CTAs."""
     out_pitch = _rows_of(out, "out")
     if b.k != a.k or out.shape != (a.rows, b.rows):
         raise KernelError(f"mxfp4.product: {a.shape} x {b.shape}^T -> {tuple(out.shape)}")
     code, x, w = ops.dtype_code(out), a.data, b.data
     stream = _stream_of(x, w, out)
-    ops._check(_fn(_BOTH)(x.data_ptr(), w.data_ptr(), out.data_ptr(), code, out_pitch, a.rows, b.rows, a.k, _known(x)[0], stream), "mxfp4.product")
+    status, sms = _known(x)
+    ops._check(_fn(_BOTH)(x.data_ptr(), w.data_ptr(), out.data_ptr(), code, out_pitch, a.rows, b.rows, a.k, kernel, sms, status, stream),
+               "mxfp4.product")

@@ -246,9 +246,9 @@ def test_product_of_two_packed_matrices(m, n, k):
     a_data = plain.pack((rng.standard_normal((m, k)) * np.exp(rng.standard_normal(k))).astype(np.float32))
     _, data, w = operands(1, n, k, m + n)
     a = plain.values(a_data, m, k)
-    for out_dtype in (torch.bfloat16, torch.float32):
+    for out_dtype, kernel in ((torch.bfloat16, 0), (torch.float32, 1), (torch.bfloat16, 2), (torch.float32, 2)):
         out = torch.full((m, n + 8), -5.0, dtype=out_dtype, device=DEV)
-        mxfp4.product(matrix(a_data, m, k), matrix(data, n, k), out[:, :n])
+        mxfp4.product(matrix(a_data, m, k), matrix(data, n, k), out[:, :n], kernel=kernel)
         torch.cuda.synchronize()
         assert bool((out[:, n:] == -5.0).all())
         check_sum(out[:, :n], a @ w.T, np.abs(a) @ np.abs(w).T, k, out_dtype)
