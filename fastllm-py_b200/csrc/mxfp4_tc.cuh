@@ -35,9 +35,8 @@ __device__ __forceinline__ int mxt_warp() { return __shfl_sync(0xffffffffu, (int
 __device__ __forceinline__ void mxt_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// Whether a barrier's phase is complete, without waiting.  A wait costs an issuing warp some 190 clocks even where the phase is
-// complete long since; asked ahead of the matrix instructions that come before it, the answer is there when they have been issued
-// (the pairs' kernel, mxfp4_pair.cu: 672 clocks for a half chunk whose MMAs take 384).
+// Whether a barrier's phase is complete, without waiting.  The warps that issue matrix instructions ask for the next ones' barriers
+// before they issue: the answer is there when they have.
 __device__ __forceinline__ bool mxt_test(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -49,11 +48,16 @@ __device__ __forceinline__ bool mxt_test(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// lane 0 waits for its warp
+// A whole warp waits for a barrier's phase (limits as mbar_wait's).  All lanes ask, over and over: a wait by one lane, which may be put
+// to sleep, and a shuffle of the outcome took 190 clocks even where the phase was complete, and these kernels hand over from warp to
+// warp several times a chunk (4096 x 8192 x 22016 in 4 bits: 384 us so, 313 this way; 64 tokens 22016 -> 8192: 40.8 and 36.8).
 __device__ __forceinline__ bool mxt_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-    uint32_t ok = 1;
-    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag) ? 1u : 0u;
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+    if (__all_sync(0xffffffffu, mxt_test(bar, parity))) return true;
+    const uint64_t t0 = global_ns();
+    for (uint32_t spins = 1;; ++spins) {
+        if (__all_sync(0xffffffffu, mxt_test(bar, parity))) return true;
+        if ((spins & 255u) == 0 && __any_sync(0xffffffffu, *abort_flag || global_ns() - t0 > TC_WAIT_LIMIT_NS)) return false;
+    }
 }
 // Tokens t, t + STEP, .. of the float sums [token][PITCH] (FEAT features, of a gated unit then their up values), added up over the cluster's CTAs in rank order, through the
 // activation and out; `n`: how many features there are from the tile's first on.
