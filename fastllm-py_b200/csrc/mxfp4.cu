@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const T* __restrict__ 
     const long tile = blockIdx.x >> 4;
     const int u = blockIdx.x & 15;
     uint8_t* dst = data + (tile * chunks + chunk) * MX_CHUNK;
-    if (VEC) {
+    if constexpr (VEC) {
         const int r = mx_row_of(u, lane >> 2);
         const long row = tile * MX_ROWS + r;
         float v[4][8];
@@ -89,33 +89,33 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const T* __restrict__ 
             *reinterpret_cast<uint32_t*>(dst + b * 2048 + r * 16 + t * 4) = s == 255 ? 0 : word;
         }
         if (t == 0) *reinterpret_cast<uint32_t*>(dst + mx_scale_at(r)) = scales;
-        return;
-    }
+    } else {
 #pragma unroll 2
-    for (int i = 0; i < 8; ++i) {
-        const int r = mx_row_of(u, i);
-        const long row = tile * MX_ROWS + r;
-        float v[4];
+        for (int i = 0; i < 8; ++i) {
+            const int r = mx_row_of(u, i);
+            const long row = tile * MX_ROWS + r;
+            float v[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int c = chunk * 128 + b * 32 + lane;
-            v[b] = row < m && c < k ? to_f32<T>(x[row * ld + c]) : 0.0f;
-        }
-        uint32_t scales = 0, mine = 0;
+            for (int b = 0; b < 4; ++b) {
+                const int c = chunk * 128 + b * 32 + lane;
+                v[b] = row < m && c < k ? to_f32<T>(x[row * ld + c]) : 0.0f;
+            }
+            uint32_t scales = 0, mine = 0;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int s = mx_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7FFFFFFFu));
-            scales |= (uint32_t)s << (8 * b);
-            // the lane's code where its word has it, the eight lanes of a word added up
-            uint32_t word = s == 255 ? 0 : mx_one_code(v[b] * mx_inverse(s)) << (4 * ((lane & 1) * 4 + (lane >> 1 & 3)));
-            word |= __shfl_xor_sync(0xffffffffu, word, 1);
-            word |= __shfl_xor_sync(0xffffffffu, word, 2);
-            word |= __shfl_xor_sync(0xffffffffu, word, 4);
-            word = __shfl_sync(0xffffffffu, word, (lane & 3) * 8);
-            if (lane >> 2 == b) mine = word;                          // lanes 4 b .. 4 b + 3 hold the block's words
+            for (int b = 0; b < 4; ++b) {
+                const int s = mx_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7FFFFFFFu));
+                scales |= (uint32_t)s << (8 * b);
+                // the lane's code where its word has it, the eight lanes of a word added up
+                uint32_t word = s == 255 ? 0 : mx_one_code(v[b] * mx_inverse(s)) << (4 * ((lane & 1) * 4 + (lane >> 1 & 3)));
+                word |= __shfl_xor_sync(0xffffffffu, word, 1);
+                word |= __shfl_xor_sync(0xffffffffu, word, 2);
+                word |= __shfl_xor_sync(0xffffffffu, word, 4);
+                word = __shfl_sync(0xffffffffu, word, (lane & 3) * 8);
+                if (lane >> 2 == b) mine = word;                          // lanes 4 b .. 4 b + 3 hold the block's words
+            }
+            if (lane < 16) *reinterpret_cast<uint32_t*>(dst + (lane >> 2) * 2048 + r * 16 + (lane & 3) * 4) = mine;
+            else if (lane == 16) *reinterpret_cast<uint32_t*>(dst + mx_scale_at(r)) = scales;
         }
-        if (lane < 16) *reinterpret_cast<uint32_t*>(dst + (lane >> 2) * 2048 + r * 16 + (lane & 3) * 4) = mine;
-        else if (lane == 16) *reinterpret_cast<uint32_t*>(dst + mx_scale_at(r)) = scales;
     }
 }
 
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __res
     uint32_t word[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) word[b] = *reinterpret_cast<const uint32_t*>(src + b * 2048 + r * 16 + t * 4);
-    if (VEC) {
+    if constexpr (VEC) {
         const long row = tile * MX_ROWS + r;
         const bool large = __any_sync(0xffffffffu, (scales & 0x80808080u & ((scales & 0x7F7F7F7Fu) + 0x7F7F7F7Fu)) != 0);
         if (row >= m) return;
@@ -181,18 +181,18 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __res
                     if (c + i < k) dst[i] = v[i];
             }
         }
-        return;
-    }
-    const int place = 4 * ((lane & 1) * 4 + (lane >> 1 & 3));         // of element lane % 8 in its word
+    } else {
+        const int place = 4 * ((lane & 1) * 4 + (lane >> 1 & 3));         // of element lane % 8 in its word
 #pragma unroll 2
-    for (int i = 0; i < 8; ++i) {
-        const long row = tile * MX_ROWS + mx_row_of(u, i);
-        const uint32_t sc = __shfl_sync(0xffffffffu, scales, 4 * i);
+        for (int i = 0; i < 8; ++i) {
+            const long row = tile * MX_ROWS + mx_row_of(u, i);
+            const uint32_t sc = __shfl_sync(0xffffffffu, scales, 4 * i);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const uint32_t code = __shfl_sync(0xffffffffu, word[b], 4 * i + (lane >> 3)) >> place;
-            const int c = chunk * 128 + b * 32 + lane;
-            if (row < m && c < k) out[row * ld + c] = from_f32<T>(mx_value(code, 0) * mx_scale((int)(sc >> (8 * b)) & 255));
+            for (int b = 0; b < 4; ++b) {
+                const uint32_t code = __shfl_sync(0xffffffffu, word[b], 4 * i + (lane >> 3)) >> place;
+                const int c = chunk * 128 + b * 32 + lane;
+                if (row < m && c < k) out[row * ld + c] = from_f32<T>(mx_value(code, 0) * mx_scale((int)(sc >> (8 * b)) & 255));
+            }
         }
     }
 }
@@ -217,8 +217,8 @@ FL_API int fl_mx_dequantize(const void* data, void* out, int code, long ld, int 
 // one instruction does not matter as long as both operands agree, and a lane's 8 consecutive elements of a token are the partners of
 // one word of codes.  The warps' sums meet in shared memory and are added in order.
 //
-// LB warps fit an SM.  With 24 a warp has registers for one chunk: its rows are loaded anew for the next one as soon as their codes
-// have been read, and its tokens at the end.  With 16 the next codes are on their way during the whole chunk.
+// LB warps fit an SM.  With 20 and more a warp has registers for one chunk: its rows are loaded anew for the next one as soon as
+// their codes have been read, and its tokens at the end.  With 16 the next codes are on their way during the whole chunk.
 __device__ __forceinline__ void mx_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -375,16 +375,19 @@ FL_API int fl_mx_few(const void* x, long ldx, const void* w, void* out, int out_
                      int act, float p0, float p1, int constant_w, int num_sms, cudaStream_t stream) {
     const FlGate gate = {act, p0, p1};
     if (m > 8) return (int)cudaErrorInvalidValue;
-    // Warps of a CTA: as many as keep an SM's 24 (or 16) busy with the CTAs that there are.  One token, 4096 -> 12288: 13.6 us with 16
-    // warps, 10.2 with 8, 16.6 with 4; 11008 -> 4096: 9.5, 20.7 and 24.4; 4096 -> 102400: 98, 65 and 60.
+    // Warps of a CTA, and CTAs an SM, by how many CTAs there are: all of them at once, as far as that goes, and then as many registers a
+    // thread as that leaves.  One token, in us, with 16 warps an SM in CTAs of 16 and 8, with 24 in CTAs of 8, with 20 in CTAs of 4:
+    // 128 CTAs (11008 -> 4096) 9.5, 18, 21, 24; 256 (22016 -> 8192) 38, 36, 45, 72; 384 (4096 -> 12288) 13.3, 12.7, 10.6, 15.5; 688
+    // (4096 -> the gated 2 x 11008) 24.9, 22.8, 19.2, 17.1.
     const int ctas = gated ? (n + 15) / 16 : (n + 31) / 32;
     FL_DISPATCH(out_code, TO, {
 #define MX_FEW(WARPS, LB)                                                                                                              \
     return gated ? mx_launch_few<TO, WARPS, true, LB>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, constant_w != 0, gate, stream) \
                  : mx_launch_few<TO, WARPS, false, LB>((const bf16*)x, ldx, (const uint8_t*)w, (TO*)out, ldo, m, n, k, constant_w != 0, gate, stream)
         if (ctas <= num_sms) MX_FEW(16, 16);
+        if (ctas <= 2 * num_sms) MX_FEW(8, 16);
         if (ctas <= 3 * num_sms) MX_FEW(8, 24);
-        MX_FEW(4, 24);
+        MX_FEW(4, 20);
     })
     return (int)cudaErrorInvalidValue;
 }
