@@ -16,6 +16,13 @@
 #define MX_ROWS 128
 #define MX_CODES 8192
 #define MX_CHUNK 8704
+#define MX_DEVICES 64
+
+// The current device's index, for what a launcher asks or sets once on each (a function's attributes are a device's own); -1: none.
+static inline int mx_device() {
+    int device;
+    return cudaGetDevice(&device) == cudaSuccess && device < MX_DEVICES ? device : -1;
+}
 
 __device__ __forceinline__ long mx_scale_at(int r) { return MX_CODES + (r & 31) * 16 + (r >> 5) * 4; }
 __device__ __forceinline__ float mx_scale(int s) {          // 2^(s - 127)

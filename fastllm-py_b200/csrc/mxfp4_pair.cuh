@@ -165,6 +165,7 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
                     const uint4 qb = *reinterpret_cast<const uint4*>(stage + h * 4096 + 2048 + r * 16);
                     const uint32_t sa = stage[scale_at], sb = stage[scale_at + 1];
                     const bool large = __any_sync(0xffffffffu, max(sa, sb) > 128u);
+                    __syncwarp();
                     if (lane == 0) mxt_arrive(&w_empty[s]);
                     uint32_t v[32];
                     if (!large) {
@@ -356,11 +357,13 @@ static int mxp_launch(const void* x, long ldx, const void* w, void* out, long ld
     int rc = make_map(&map, x, m, k, ldx, bn / 2);
     if (rc) return rc;
     auto kernel = mxp_kernel<TO, GATED>;
-    static bool configured = false;
-    if (!configured) {
+    static bool configured[MX_DEVICES];
+    const int device = mx_device();
+    if (device < 0) return (int)cudaErrorInvalidDevice;
+    if (!configured[device]) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MXP_SMEM);
         if (e != cudaSuccess) return (int)e;
-        configured = true;
+        configured[device] = true;
     }
     const int stages = MXP_X_RING / (bn * 128);
     const long pairs = tiles < num_sms / 2 ? tiles : num_sms / 2;
@@ -613,11 +616,13 @@ static int mxqp_launch(const void* a, const void* w, void* out, long ldo, int m,
     const long tiles = (long)((n + 255) / 256) * token_pairs, pairs = tiles < num_sms / 2 ? tiles : num_sms / 2;
     if (tiles > 0x3FFFFFFFl || (tiles / pairs + 1) * ((chunks + 1) / 2) > 0x3FFFFFFFl) return (int)cudaErrorInvalidValue;
     auto kernel = mxqp_kernel<TO>;
-    static bool configured = false;
-    if (!configured) {
+    static bool configured[MX_DEVICES];
+    const int device = mx_device();
+    if (device < 0) return (int)cudaErrorInvalidDevice;
+    if (!configured[device]) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MXQP_SMEM);
         if (e != cudaSuccess) return (int)e;
-        configured = true;
+        configured[device] = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(2 * pairs));

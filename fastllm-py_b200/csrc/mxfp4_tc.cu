@@ -332,9 +332,19 @@ static int mxt_ranks(long tiles, int chunks, int tokens, const int* slots, int p
     if (time) *time = least;
     return best;
 }
-// Asked of the driver at a kernel's first launch (the current device's; all that the library runs on are alike).
+static int mxt_failed() {
+    const cudaError_t e = cudaGetLastError();
+    return (int)(e == cudaSuccess ? cudaErrorInvalidDevice : e);
+}
+// Asked of the driver at a kernel's first launch on a device, which is also when the kernel gets its shared memory there.
+struct MxtSlots {
+    int of[MX_DEVICES][9];                  // [device][0]: asked
+};
 template <typename... KArgs>
-static const int* mxt_slots(void (*kernel)(KArgs...), int threads, int smem, int (&slots)[9]) {
+static const int* mxt_slots(void (*kernel)(KArgs...), int threads, int smem, MxtSlots& found) {
+    const int device = mx_device();
+    if (device < 0) return nullptr;
+    int* slots = found.of[device];
     if (slots[0]) return slots;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
         cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
@@ -363,18 +373,19 @@ static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ld
     const int bn = ((m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
     const int row_tiles = (n + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
     const int tokens_y = (m + bn - 1) / bn, chunks = (k + 127) / 128;
-    static int found[9] = {};
+    static MxtSlots found;
     const int* slots = mxt_slots(mxt_kernel<TO, GATED>, MXT_THREADS, MXT_SMEM, found);
-    if (!slots) return (int)cudaGetLastError();
+    if (!slots) return mxt_failed();
     // Both kernels' times, as measured: here 1.1 us a chunk, what mxt_ranks says and 2 us besides, on pairs 0.7 us
     // a chunk and 6 us, and 8 more where a pair has one tile, whose epilogue nothing hides.  2048 tokens 4096 -> 12288: 224 us here, 180 on pairs; 1024 tokens 4096 -> 4096: 38 and 51; 512 tokens
     // 11008 -> 4096 (K shared by clusters): 49 and 63.
     long time, rounds;
     const int ranks = mxt_ranks((long)tokens_y * row_tiles, chunks, bn, slots, 110, &time);
     mxp_tokens(m, row_tiles, num_sms / 2, &rounds);
-    if (which == 2 || (which == 0 && m > MXT_BN && 600 + 70 * rounds * chunks + (rounds == 1 ? 800 : 0) < 200 + time))
+    const bool fits = tokens_y <= 65535 && row_tiles <= 65535;       // a grid's y and z; pairs walk over any number of tiles
+    if (which == 2 || (which == 0 && (!fits || (m > MXT_BN && 600 + 70 * rounds * chunks + (rounds == 1 ? 800 : 0) < 200 + time))))
         return mxp_launch<TO, GATED>(x, ldx, w, out, ldo, m, n, k, act, num_sms, status, stream);
-    if (tokens_y > 65535 || row_tiles > 65535) return (int)cudaErrorInvalidValue;
+    if (!fits) return (int)cudaErrorInvalidValue;
     const int per_rank = (chunks + ranks - 1) / ranks;
     int stages = MXT_RING / (bn * 256 + MXT_W_BYTES);
     if (stages > MXT_MAX_STAGES) stages = MXT_MAX_STAGES;
@@ -529,15 +540,16 @@ FL_API int fl_mxq_product(const void* a, const void* w, void* out, int out_code,
                           int* status, cudaStream_t stream) {
     const int chunks = (k + 127) / 128, token_tiles = (m + 127) / 128, row_tiles = (n + 255) / 256;
     FL_DISPATCH(out_code, TO, {
-        static int found[9] = {};
+        static MxtSlots found;
         const int* slots = mxt_slots(mxq_kernel<TO>, MXT_THREADS, MXQ_SMEM, found);
-        if (!slots) return (int)cudaGetLastError();
+        if (!slots) return mxt_failed();
         long time;
         const int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, m < 128 ? m : 128, slots, 35, &time);
         const long rounds = ((long)row_tiles * ((token_tiles + 1) / 2) + num_sms / 2 - 1) / (num_sms / 2);
-        if (which == 2 || (which == 0 && m > 128 && 600 + rounds * (chunks * 17 + 200) < 200 + time))
+        const bool fits = token_tiles <= 65535 && row_tiles <= 65535;
+        if (which == 2 || (which == 0 && (!fits || (m > 128 && 600 + rounds * (chunks * 17 + 200) < 200 + time))))
             return mxqp_launch<TO>(a, w, out, ldo, m, n, k, num_sms, status, stream);
-        if (token_tiles > 65535 || row_tiles > 65535) return (int)cudaErrorInvalidValue;
+        if (!fits) return (int)cudaErrorInvalidValue;
         const int per_rank = (chunks + ranks - 1) / ranks;
         return mxt_launch_cluster(mxq_kernel<TO>, MXT_THREADS, MXQ_SMEM, dim3(ranks, token_tiles, row_tiles), stream, (const uint8_t*)a,
                                   (const uint8_t*)w, (TO*)out, ldo, m, n, chunks, ranks, per_rank, status);

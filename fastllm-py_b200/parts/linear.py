@@ -58,6 +58,7 @@ class Linear:
         if held == "mxfp4":
             from ..native import mxfp4
             self._q4 = mxfp4.Matrix.of(self.weight)
+            torch.cuda.current_stream().synchronize()       # products read it as constant: none may begin beside the rounding
             self.weight = None
         elif held != "stored":
             raise ValueError(f"a Linear's matrix is held 'stored' or as 'mxfp4', got {held!r}")

@@ -460,3 +460,83 @@ def test_long_rows_and_many_tokens():
     got = torch.cat([out[:150], out[-150:]])
     check_sum(got, x @ w.T, np.abs(x) @ np.abs(w).T, k, torch.bfloat16)
     assert bool((out[150:-150] == 0).all())
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 65536 * 256 + 5, 24), (9, 65536 * 256 + 5, 24), (65536 * 128 + 5, 8, 8)])
+def test_more_tiles_than_a_grid_has_places(m, n, k):
+    """65536 tiles and a few rows more, of W or of tokens: zeros but for the last rows, whose sums come out where they belong."""
+    from fastllm_py_b200.native import mxfp4
+
+    rng = np.random.default_rng(m)
+    rows = n % 128 or 128
+    last = plain.pack((rng.standard_normal((rows, k)) / np.sqrt(k)).astype(np.float32))
+    q = mxfp4.Matrix.empty(n, k, DEV)
+    q.data.zero_()
+    q.data[-1].copy_(torch.from_numpy(np.ascontiguousarray(last)).to(DEV)[0])
+    w = plain.values(last, rows, k)
+    some = bf16(rng.standard_normal((130, k)))
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=DEV)
+    take = min(m, 130)
+    x[-take:] = torch.from_numpy(some[:take]).to(DEV).to(torch.bfloat16)
+    out = torch.full((m, n), -5.0, dtype=torch.bfloat16, device=DEV)
+    mxfp4.linear(x, q, out)
+    check_sum(out[-take:, n - rows:], some[:take] @ w.T, np.abs(some[:take]) @ np.abs(w).T, k, torch.bfloat16)
+    assert not bool(out[:, :n - rows].any()) and not bool(out[:m - take].any())
+    a = mxfp4.Matrix.of(x)
+    av = torch.empty(m, k, device=DEV)
+    mxfp4.dequantize(a, av)
+    av = av[-take:].double().cpu().numpy()
+    out.fill_(-5.0)
+    mxfp4.product(a, q, out)
+    check_sum(out[-take:, n - rows:], av @ w.T, np.abs(av) @ np.abs(w).T, k, torch.bfloat16)
+    assert not bool(out[:, :n - rows].any()) and not bool(out[:m - take].any())
+
+
+def test_a_layer_multiplies_as_soon_as_it_is_made():
+    """Two layers made one after the other and used at once: their matrices are there before a product reads them as constant."""
+    from fastllm_py_b200.parts.linear import Linear
+
+    rng = np.random.default_rng(5)
+    x = bf16(rng.standard_normal((3, 4096)))
+    xs = rows_in(x, torch.bfloat16)
+    ws = [bf16(rng.standard_normal((2048, 4096)) / 64) for _ in range(2)]
+    layers = [Linear([torch.from_numpy(w).to(DEV).to(torch.bfloat16)], "mxfp4") for w in ws]
+    outs = [torch.empty(3, 2048, dtype=torch.bfloat16, device=DEV) for _ in ws]
+    for layer, out in zip(layers, outs):
+        layer.forward(xs, out)
+    for w, out in zip(ws, outs):
+        v = plain.values(plain.pack(w.astype(np.float32)), 2048, 4096)
+        check_sum(out, x @ v.T, np.abs(x) @ np.abs(v).T, 4096, torch.bfloat16)
+
+
+def test_two_captured_products_replayed_at_the_same_time():
+    """Graphs of the same calls on different outputs, replayed on two streams: nothing but the operands is shared."""
+    from fastllm_py_b200.native import mxfp4
+
+    m, n, k = 40, 520, 2048
+    x, data, w = operands(m, 2 * n, k, 3)
+    xs, q = rows_in(x, torch.bfloat16), matrix(data, 2 * n, k)
+    a = mxfp4.Matrix.of(xs)
+    mxfp4.reserve(DEV)
+    graphs, outs = [], []
+    for _ in range(2):
+        out = [torch.empty(m, 2 * n, dtype=torch.float32, device=DEV) for _ in range(2)] + [torch.empty(m, n, dtype=torch.float32, device=DEV)]
+        mxfp4.linear(xs, q, out[0]), mxfp4.product(a, q, out[1]), mxfp4.linear_gated(xs, q, out[2])
+        outs.append((out, [o.clone() for o in out]))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            mxfp4.linear(xs, q, out[0]), mxfp4.product(a, q, out[1]), mxfp4.linear_gated(xs, q, out[2])
+        graphs.append(g)
+    for out, _ in outs:
+        for o in out:
+            o.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for out, want in outs:
+        assert all(torch.equal(o, v) for o, v in zip(out, want))
+    check_sum(outs[0][0][0], x @ w.T, np.abs(x) @ np.abs(w).T, k, torch.float32)
