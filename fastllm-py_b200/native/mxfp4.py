@@ -13,7 +13,7 @@ points, its scales are exact, and the tensor cores of sm_100a multiply it as it 
     mxfp4.linear_gated(x, q, out)             # out = act(x gate^T) * (x up^T), q = [gate; up]
     mxfp4.product(a, q, out)                  # out = a q^T, both in 4 bits
 
-Everything launches on the current stream of the current device and allocates nothing.
+Everything launches on the current stream of the current device and allocates nothing.  No output may overlap an operand.
 """
 from __future__ import annotations
 
@@ -25,18 +25,20 @@ from . import ops
 from .ops import KernelError
 
 ROWS, CHUNK_K, CHUNK_BYTES = 128, 128, 8704      # a tile's rows, a chunk's elements along K and its bytes (csrc/mxfp4.cu)
+MOST_ROWS, MOST_K = 2**31 - 1024, 2**26 - 1024   # rows are counted in 32 bits, to the end of their tile; a grid holds 65535 x 8 chunks
 LIBRARIES = ["mxfp4", "mxfp4_tc", "gemm_tcgen05"]
 
 
 class Matrix:
     """A matrix [rows, k] in the packed form: uint8 [ceil(rows / 128), ceil(k / 128), 8704] (csrc/mxfp4.cu says how a chunk
-    lies).  Codes behind k are zero; rows behind the last are not read for any result."""
+    lies).  Codes behind k are zero, and so are the scales of whole blocks there; rows behind the last are not read for any
+    result."""
 
     __slots__ = ("data", "rows", "k", "shape")
 
     def __init__(self, data: torch.Tensor, rows: int, k: int):
-        if rows < 1 or k < 1:
-            raise KernelError(f"mxfp4: a matrix has rows and columns, got {rows} x {k}")
+        if not (1 <= rows <= MOST_ROWS and 1 <= k <= MOST_K):
+            raise KernelError(f"mxfp4: a matrix has 1 to {MOST_ROWS} rows and 1 to {MOST_K} columns, got {rows} x {k}")
         if data.dtype is not torch.uint8 or data.shape != (-(-rows // ROWS), -(-k // CHUNK_K), CHUNK_BYTES) or not data.is_contiguous():
             raise KernelError(f"mxfp4: [{rows}, {k}] packed is a contiguous uint8 tensor "
                               f"{(-(-rows // ROWS), -(-k // CHUNK_K), CHUNK_BYTES)}, got {data.dtype} {tuple(data.shape)}")
@@ -51,6 +53,8 @@ class Matrix:
     @classmethod
     def of(cls, x: torch.Tensor) -> "Matrix":
         """x [rows, k] rounded to the format."""
+        if x.dim() != 2:
+            raise KernelError(f"mxfp4: x is a matrix, got shape {tuple(x.shape)}")
         q = cls.empty(x.shape[0], x.shape[1], x.device)
         quantize(x, q)
         return q
@@ -161,6 +165,12 @@ def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, consta
     m, k = x.shape
     if w.k != k or out.shape != (m, n) or (gated and w.rows % 2):
         raise KernelError(f"mxfp4.{name}: {tuple(x.shape)} x {w.shape}^T -> {tuple(out.shape)}")
+    if kernel not in (0, 1, 2):
+        raise KernelError(f"mxfp4.{name}: there is no kernel {kernel}")
+    if m > MOST_ROWS:
+        raise KernelError(f"mxfp4.{name}: {m} rows, at most {MOST_ROWS}")
+    if x.data_ptr() == out.data_ptr() and m > 0:
+        raise KernelError(f"mxfp4.{name}: out lies on x, which the kernels read while they write")
     act = -1 if activation is None else ops.activation_code(activation)
     code, stream = ops.dtype_code(out), _stream_of(x, data, out)
     if m == 0:
@@ -180,7 +190,8 @@ def linear(x: torch.Tensor, w: Matrix, out: torch.Tensor, activation: str | None
     """out[m, n] (bfloat16 or float32) = x[m, k] @ w[n, k]^T; x bfloat16 (16-byte aligned, its row pitch a multiple of 8
     elements), products and sums in float.  `activation` (`ops.ACTIVATIONS`, f(v, 1)) is applied on the way out.  `constant_w`
     says that nothing that may still be running writes w (a model's matrix, written long since), so that its first bytes may be
-    read while the kernels before this one in the stream run.  `kernel`: 0 the one that suits the sizes, 1 the tensor-core kernel on tiles, 2 the one on pairs of CTAs."""
+    read while the kernels before this one in the stream run.  `kernel`: 0 the one that suits the sizes, 1 the tensor-core kernel on
+    tiles, 2 the one on pairs of CTAs."""
     _times_weights("linear", x, w, out, 0, w.rows, activation, params, constant_w, kernel)
 
 
@@ -198,6 +209,8 @@ def product(a: Matrix, b: Matrix, out: torch.Tensor, kernel: int = 0) -> None:
     out_pitch = _rows_of(out, "out")
     if b.k != a.k or out.shape != (a.rows, b.rows):
         raise KernelError(f"mxfp4.product: {a.shape} x {b.shape}^T -> {tuple(out.shape)}")
+    if kernel not in (0, 1, 2):
+        raise KernelError(f"mxfp4.product: there is no kernel {kernel}")
     code, x, w = ops.dtype_code(out), a.data, b.data
     stream = _stream_of(x, w, out)
     status, sms = _known(x)

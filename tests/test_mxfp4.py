@@ -30,6 +30,33 @@ def test_a_matrix_takes_its_packed_shape_only(rows, k):
             mxfp4.Matrix(q.data, r, c)
 
 
+def test_sizes_that_the_kernels_cannot_count_are_refused():
+    for rows, k in ((2**31 - 1023, 1), (1, 2**26 - 1023), (2**32 + 1, 128)):
+        with pytest.raises(KernelError, match="1 to"):
+            mxfp4.Matrix(torch.empty(1, dtype=torch.uint8).expand(-(-rows // 128), -(-k // 128), 8704), rows, k)
+    long = torch.empty(2**31 - 1023, 8, dtype=torch.bfloat16, device="meta")
+    with pytest.raises(KernelError, match="rows, at most"):
+        mxfp4.linear(long, empty(8, 8), torch.empty(2**31 - 1023, 8, dtype=torch.bfloat16, device="meta"))
+
+
+def test_a_matrix_of_something_else_than_rows_is_refused():
+    for x in (torch.zeros(96), torch.zeros(2, 3, 96)):
+        with pytest.raises(KernelError, match="is a matrix"):
+            mxfp4.Matrix.of(x)
+
+
+def test_kernels_that_do_not_exist_and_outputs_on_an_operand_are_refused():
+    x, w, a = torch.zeros(5, 64, dtype=torch.bfloat16), empty(64, 64), empty(5, 64)
+    for kernel in (-1, 3):
+        for call in (lambda: mxfp4.linear(x, w, torch.zeros(5, 64), kernel=kernel), lambda: mxfp4.linear_gated(x, w, torch.zeros(5, 32), kernel=kernel),
+                     lambda: mxfp4.product(a, w, torch.zeros(5, 64), kernel=kernel)):
+            with pytest.raises(KernelError, match="there is no kernel"):
+                call()
+    for call in (lambda: mxfp4.linear(x, w, x), lambda: mxfp4.linear_gated(x, w, x[:, :32])):
+        with pytest.raises(KernelError, match="out lies on x"):
+            call()
+
+
 def test_wrappers_refuse_what_the_kernels_do_not_take():
     bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731
     w, a = empty(64, 96), empty(5, 96)
