@@ -77,8 +77,8 @@ __device__ __forceinline__ bool mxp_epilogue(uint32_t tmem_acc, float* staged, u
         if (mxp_vote(*abort_flag != 0)) return false;     // (a half's readers have all come here before it is written again)
         if (n <= 0) continue;
         const int last = min(32, tokens - t);
-        if (vec) mxt_rows<TO, GATED, FEAT, 128, V, 4>(half, quarter, last, 1, out + (long)t * ldo, ldo, n, act);
-        else mxt_rows<TO, GATED, FEAT, 128, 1, 4>(half, quarter, last, 1, out + (long)t * ldo, ldo, n, act);
+        if (vec) mxt_rows<TO, GATED, FEAT, 128, V, 4>(MxtSums{half, half, 1, 0, 0, 0}, quarter, last, out + (long)t * ldo, ldo, n, act);
+        else mxt_rows<TO, GATED, FEAT, 128, 1, 4>(MxtSums{half, half, 1, 0, 0, 0}, quarter, last, out + (long)t * ldo, ldo, n, act);
     }
     return true;
 }
@@ -530,8 +530,8 @@ mxqp_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __
                 if (mxqp_vote(*abort_flag != 0, group)) going = false;
                 if (!going) break;
                 const int last = min(32, tokens - t);
-                if (vec) mxt_rows<TO, false, 128, 128, 4, 4>(mine, quarter, last, 1, dst + (long)t * ldo, ldo, left, FlGate{FL_ACT_NONE, 0.0f, 0.0f});
-                else mxt_rows<TO, false, 128, 128, 1, 4>(mine, quarter, last, 1, dst + (long)t * ldo, ldo, left, FlGate{FL_ACT_NONE, 0.0f, 0.0f});
+                if (vec) mxt_rows<TO, false, 128, 128, 4, 4>(MxtSums{mine, mine, 1, 0, 0, 0}, quarter, last, dst + (long)t * ldo, ldo, left, FlGate{FL_ACT_NONE, 0.0f, 0.0f});
+                else mxt_rows<TO, false, 128, 128, 1, 4>(MxtSums{mine, mine, 1, 0, 0, 0}, quarter, last, dst + (long)t * ldo, ldo, left, FlGate{FL_ACT_NONE, 0.0f, 0.0f});
             }
             if (!going) break;
         }

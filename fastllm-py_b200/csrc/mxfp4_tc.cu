@@ -7,18 +7,25 @@
 //
 // A CTA takes two tiles of 128 rows of W (of a gated unit: a gate tile and the up tile of the same features) and up to 128
 // tokens, K in stages of a chunk (128): one copy a row tile, two boxes of the tokens.  Warps 0-15 turn the codes into bfloat16, a
-// thread one row of a chunk (warps 0-7 of every other one, 8-15 of those between), and write them to one of the two places in
-// tensor memory; then they are the epilogue.  Warp 16 sends for the copies, warp 17 issues the MMAs.  Where there are fewer
-// tiles than SMs a cluster of up to 8 CTAs shares K; its partial sums stay in shared memory, and each CTA adds up its share of the
-// tokens from all of them, in rank order.
+// thread one row of a chunk (warps 0-7 of every other one, 8-15 of those between), and write them to one of the two or
+// three places in tensor memory; then they are the epilogue.  Warp 16 sends for the copies, warp 17 issues the MMAs.  Where there are
+// fewer tiles than SMs a cluster of up to 8 CTAs shares K; each CTA is sent the others' sums of its share of the tokens, and adds them
+// up in rank order.
+//
+// What bounds it: the conversion.  A word of 8 codes takes 9 instructions of the integer units, which take two clocks of a quarter of
+// the SM each, and 8 multiplications: a chunk of 256 rows 600 clocks at the least, and 1050 with what the warps wait for one
+// another; 16 MMAs take 620 clocks with 16 tokens, 820 with 64 and 1140 with 128.  64 tokens 22016 -> 8192: 35.1 us, 2.7 TB/s
+// of codes, 0.66 PFLOP/s; 16 tokens 30.9; 128 tokens 44, 1.05 PFLOP/s.
 #include "mxfp4_pair.cuh"
 #include "mxfp4_tc.cuh"
 
 #define MXT_BN 128                          // most tokens of a tile
-#define MXT_A 2                             // places of 2 x 64 columns in tensor memory
+#define MXT_A 3                             // most places of 2 x 64 columns in tensor memory
 #define MXT_W_BYTES (2 * (MX_CODES + 1024)) // two row tiles of a chunk: codes, the scales of the one or two packed tiles they lie in
-#define MXT_RING (208 * 1024)               // the epilogue's sums take its place
+#define MXT_RING (224 * 1024)               // the epilogue's sums take its place: a CTA's own and what the others of its cluster send it
 #define MXT_MAX_STAGES 10
+#define MXT_FEW_ROWS 8                      // what fl_mx_few takes
+#define MXT_FEW (-1)
 #define MXT_PITCH 256                       // floats between the tokens of the sums
 // (No other kernel that takes tensor memory fits an SM beside this much shared memory: an allocation never waits for a CTA that
 // waits for its predecessor in the stream.)
@@ -26,62 +33,73 @@
 #define MXT_WARPS 16                        // that convert, and of the epilogue
 #define MXT_THREADS ((MXT_WARPS + 2) * 32)
 
-// The end of a CTA whose sums of `rows` tokens are written, by all its threads: its share of the tokens from all of the cluster's
-// CTAs, by its first WARPS warps.  Leaves with the cluster's sums no longer needed.
-template <typename TO, bool GATED, int FEAT, int PITCH, int WARPS>
-__device__ __forceinline__ void mxt_join(float* sums, volatile int* abort_flag, int rows, int ranks, int rank, TO* __restrict__ out,
-                                         long ldo, int f0, int n, const FlGate act) {
-    const int warp = mxt_warp();
+// What the kernels with accumulators in tensor memory end with, by the whole CTA: the accumulators (valid where `any`, else zero)
+// as float sums [token][2 x 128 rows] in shared memory, where the ring was (every copy has been read by an MMA that is done).  `ok`:
+// of the first MXT_WARPS warps, whether the accumulators may be waited for.
+//
+// Of a cluster each CTA takes a share of the tokens; the others send it their sums of them, one copy each, to behind its own, where its
+// ring is free too once its MMAs are done: the first meeting of the cluster, arrived at before the accumulators are read.  The second is
+// arrived at when a CTA has all that it was sent, so the senders' sums have been read, and is waited for behind the output.  (With the
+// sums fetched from the other CTAs by loads, 64 tokens 4096 -> 4096 took 11.6 us, 5.5 of them here.)  A CTA that gave up sends
+// what it has: the status word tells that the results are not valid.
+template <typename TO, bool GATED>
+__device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, int acc_cols, uint64_t* acc_bar, uint64_t* sent_bar, volatile int* abort_flag, int* status,
+                                           bool ok, bool any, int rows, int ranks, int rank, TO* __restrict__ out, long ldo, int f0, int n,
+                                           const FlGate act) {
+    constexpr int FEAT = GATED ? 128 : 256, V = 4;
+    const int warp = mxt_warp(), lane = threadIdx.x & 31;
+    const int share = (rows + ranks - 1) / ranks, first = min(rows, rank * share), last = min(rows, first + share);
+    float* parts = sums + rows * MXT_PITCH;
+    if (warp < MXT_WARPS && ok && !mxt_wait(acc_bar, 0, abort_flag)) {
+        if (lane == 0) mxt_give_up(abort_flag, status);
+        ok = false;
+    }
     __syncwarp();
+    if (ranks > 1) mxt_cluster_arrive();
+    if (warp < MXT_WARPS && ok) {
+        tc_fence_after();
+        const int tile = warp >> 2 & 1, f = tile * 128 + (threadIdx.x & 127);
+        const uint32_t src = tmem_d + (uint32_t)(tile * acc_cols) + ((uint32_t)((warp & 3) * 32) << 16);
+        for (int c = (warp >> 3) * 16; c < rows; c += 32) {
+            uint32_t v[16];
+            tmem_ld16(src + (uint32_t)c, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (c + j < rows) sums[(c + j) * MXT_PITCH + f] = any ? __uint_as_float(v[j]) : 0.0f;
+        }
+    }
     tc_fence_before();
-    if (ranks > 1) cluster_sync_all();
-    else __syncthreads();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
     tc_fence_after();
-    // (a CTA of the cluster that gave up leaves its sums as they are: the status word tells that the results are not valid)
-    if (warp < WARPS && !*abort_flag) {
-        const int share = (rows + ranks - 1) / ranks, first = rank * share, last = min(rows, first + share);
-        constexpr int V = FEAT >= 128 ? 4 : 2;
+    if (ranks > 1) {
+        mxt_cluster_wait();
+        if (warp == MXT_WARPS && mxt_elect()) {
+            if (last > first) mbar_expect_tx(sent_bar, (uint32_t)((ranks - 1) * (last - first) * MXT_PITCH * 4));
+            for (int i = 1; i < ranks; ++i) {
+                const int to = rank + i < ranks ? rank + i : rank + i - ranks, t0 = to * share, tokens = min(share, rows - t0);
+                if (tokens > 0)
+                    mxt_push(parts + (rank - (rank > to)) * tokens * MXT_PITCH, sums + t0 * MXT_PITCH, (uint32_t)(tokens * MXT_PITCH * 4), sent_bar, to);
+            }
+        }
+        // (a CTA that gave up waits for what is on its way to it all the same)
+        if (warp < MXT_WARPS && last > first && !mxt_wait(sent_bar, 0, nullptr) && lane == 0) mxt_give_up(abort_flag, status);
+        __syncwarp();
+        mxt_cluster_arrive();
+    }
+    if (warp < MXT_WARPS && !*abort_flag) {
+        const MxtSums from = {sums, parts, ranks, rank, first, (last - first) * MXT_PITCH};
         out += f0;
         // a warp takes a token: V features a lane and 32 V a step, or single ones side by side where rows are not aligned
         if ((((uintptr_t)out | (uintptr_t)(ldo * (long)sizeof(TO))) & (V * sizeof(TO) - 1)) == 0 && (n & (V - 1)) == 0)
-            mxt_rows<TO, GATED, FEAT, PITCH, V, WARPS>(sums, first + warp, last, ranks, out, ldo, n - f0, act);
-        else {
-            if (ranks > 1) mxt_gather<(GATED ? 2 : 1) * FEAT, PITCH, WARPS>(sums, first + warp, last, ranks);
-            mxt_rows<TO, GATED, FEAT, PITCH, 1, WARPS>(sums, first + warp, last, 1, out, ldo, n - f0, act);
-        }
+            mxt_rows<TO, GATED, FEAT, MXT_PITCH, V, MXT_WARPS>(from, first + warp, last, out, ldo, n - f0, act);
+        else
+            mxt_rows<TO, GATED, FEAT, MXT_PITCH, 1, MXT_WARPS>(from, first + warp, last, out, ldo, n - f0, act);
     }
     __syncwarp();
-    if (ranks > 1) cluster_sync_all();                                // the others may still read this CTA's sums
+    if (ranks > 1) mxt_cluster_wait();
     else __syncthreads();
-}
-
-// What the kernels with accumulators in tensor memory end with, by the whole CTA: the accumulators (valid where `any`, else zero)
-// as float sums [token][2 x 128 rows] in shared memory, where the ring was (every copy has been read by an MMA that is done), then
-// mxt_join.  `ok`: of the first MXT_WARPS warps, whether the accumulators may be waited for.
-template <typename TO, bool GATED>
-__device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, uint64_t* acc_bar, volatile int* abort_flag, int* status, bool ok,
-                                           bool any, int rows, int ranks, int rank, TO* __restrict__ out, long ldo, int f0, int n,
-                                           const FlGate act) {
-    const int warp = mxt_warp(), lane = threadIdx.x & 31;
-    if (warp < MXT_WARPS) {
-        if (ok && !mxt_wait(acc_bar, 0, abort_flag)) {
-            if (lane == 0) mxt_give_up(abort_flag, status);
-            ok = false;
-        }
-        if (ok) {
-            tc_fence_after();
-            const int tile = warp >> 2 & 1, f = tile * 128 + (threadIdx.x & 127);
-            const uint32_t src = tmem_d + (uint32_t)(tile * 128) + ((uint32_t)((warp & 3) * 32) << 16);
-            for (int c = (warp >> 3) * 16; c < rows; c += 32) {
-                uint32_t v[16];
-                tmem_ld16(src + (uint32_t)c, v);
-                tmem_ld_wait();
-#pragma unroll
-                for (int j = 0; j < 16; ++j) sums[(c + j) * MXT_PITCH + f] = any ? __uint_as_float(v[j]) : 0.0f;
-            }
-        }
-    }
-    mxt_join<TO, GATED, GATED ? 128 : 256, MXT_PITCH, MXT_WARPS>(sums, abort_flag, rows, ranks, rank, out, ldo, f0, n, act);
 }
 
 // The copies of a CTA's chunks c_begin .. c_end - 1, by one warp; returns how many stages were sent for.  A stage: bn x 128 elements
@@ -158,7 +176,8 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
     uint64_t* a_full = empty_bar + MXT_MAX_STAGES;
     uint64_t* a_empty = a_full + MXT_A;
     uint64_t* acc_bar = a_empty + MXT_A;
-    uint32_t* tmem_slot = (uint32_t*)(acc_bar + 1);
+    uint64_t* sent_bar = acc_bar + 1;
+    uint32_t* tmem_slot = (uint32_t*)(sent_bar + 1);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     const int warp = mxt_warp(), lane = threadIdx.x & 31;
     const int rank = blockIdx.x;
@@ -182,6 +201,7 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
             mbar_init(&a_empty[s], 1);
         }
         mbar_init(acc_bar, 1);
+        mbar_init(sent_bar, 1);
         *abort_flag = (*(volatile int*)status != 0) ? 1 : 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -193,7 +213,10 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_d = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_a = tmem_d + 256;   // accumulators of 128 columns each, then the ring of A
+    // two accumulators, then the places of A.  Up to 64 tokens leave room for three: a chunk's conversion then does not wait for the MMAs
+    // of the last but one, which end about when it begins.
+    const int acc_cols = bn <= 64 ? 64 : 128, places = bn <= 64 ? 3 : 2;
+    const uint32_t tmem_d = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_a = tmem_d + (uint32_t)(2 * acc_cols);
     pdl_trigger();
     int issued = 0;
     bool ok = !*abort_flag;
@@ -205,8 +228,8 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
         const int rr = (tile ? off : 0) + r;                     // the row's place in the packed tiles
         const int codes_at = x_bytes + tile * (MX_CODES + 1024) + r * 16;
         const int scale_at = x_bytes + tile * (MX_CODES + 1024) + (rr >> 7) * 512 + mx_scale_at(rr & 127);
-        const uint32_t dst = tmem_a + (uint32_t)(turn * 128 + tile * 64) + ((uint32_t)((warp & 3) * 32) << 16);
-        int s = turn;
+        const uint32_t lanes = tmem_a + (uint32_t)(tile * 64) + ((uint32_t)((warp & 3) * 32) << 16);
+        int s = turn, place = turn;
         uint32_t ph = 0, pa = 0;
         if (s >= stages) s -= stages, ph ^= 1u;
         for (int c = c_begin + turn; c < c_end && ok; c += 2) {
@@ -235,12 +258,13 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
                 }
             };
             if (here) two(0);
-            if (!mxt_wait(&a_empty[turn], pa ^ 1u, abort_flag)) {
+            if (!mxt_wait(&a_empty[place], pa ^ 1u, abort_flag)) {
                 if (lane == 0) mxt_give_up(abort_flag, status);
                 ok = false;
                 break;
             }
             tc_fence_after();
+            const uint32_t dst = lanes + (uint32_t)(place * 128);
             if (here) {
                 mxt_tmem_st16(dst, v);
                 mxt_tmem_st16(dst + 16u, v + 16);
@@ -251,8 +275,8 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mxt_arrive(&a_full[turn]);
-            pa ^= 1u;
+            if (lane == 0) mxt_arrive(&a_full[place]);
+            if ((place += 2) >= places) place -= places, pa ^= 1u;
             s += 2;
             if (s >= stages) s -= stages, ph ^= 1u;
         }
@@ -263,33 +287,37 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
         // ---- MMA issuer
         const uint32_t idesc = instr_desc_bf16(128, bn), ring_at = smem_u32(ring);
         int s = 0;
-        uint32_t ph = 0, turn = 0, pa = 0;
+        uint32_t place = 0, pa = 0;
+        bool there = false;                                      // the next chunk is known to be there
         for (int c = c_begin; c < c_end && ok; ++c) {
-            if (!mxt_wait(&full_bar[s], ph, abort_flag) || !mxt_wait(&a_full[turn], pa, abort_flag)) {
+            // (the tokens are there too: the converting warps had waited for the stage's barrier)
+            if (!__all_sync(0xffffffffu, there) && !mxt_wait(&a_full[place], pa, abort_flag)) {
                 if (lane == 0) mxt_give_up(abort_flag, status);
                 ok = false;
                 break;
             }
             tc_fence_after();
+            const uint32_t next = place + 1 == (uint32_t)places ? 0 : place + 1;
+            there = mxt_test(&a_full[next], next ? pa : pa ^ 1u);
             const uint64_t bdesc = smem_desc_sw128(ring_at + (uint32_t)(s * stage_bytes));
             const uint64_t half = (uint64_t)(x_bytes / 2) >> 4;
             if (mxt_elect()) {
                 for (int tile = 0; tile < tiles; ++tile)
 #pragma unroll
                     for (int kk = 0; kk < 8; ++kk)
-                        mxt_umma_ts(tmem_d + (uint32_t)(tile * 128), tmem_a + turn * 128u + (uint32_t)(tile * 64 + kk * 8),
+                        mxt_umma_ts(tmem_d + (uint32_t)(tile * acc_cols), tmem_a + place * 128u + (uint32_t)(tile * 64 + kk * 8),
                                     bdesc + (uint64_t)(2 * (kk & 3)) + (kk >= 4 ? half : 0), idesc, (c > c_begin || kk > 0) ? 1u : 0u);
-                umma_commit(&a_empty[turn]);
+                umma_commit(&a_empty[place]);
                 umma_commit(&empty_bar[s]);
             }
             __syncwarp();
-            if (++s == stages) { s = 0; ph ^= 1u; }
-            turn ^= 1u;
-            pa ^= turn ^ 1u;
+            if (++s == stages) s = 0;
+            place = next;
+            if (next == 0) pa ^= 1u;
         }
         if (ok && mxt_elect()) umma_commit(acc_bar);
     }
-    mxt_finish<TO, GATED>(reinterpret_cast<float*>(ring), tmem_d, acc_bar, abort_flag, status, ok, c_end > c_begin, min(bn, m - t0), ranks, rank,
+    mxt_finish<TO, GATED>(reinterpret_cast<float*>(ring), tmem_d, acc_cols, acc_bar, sent_bar, abort_flag, status, ok, c_end > c_begin, min(bn, m - t0), ranks, rank,
                           out + (long)t0 * ldo, ldo, f0, n, act);
     if (warp == MXT_WARPS && lane == 0 && *abort_flag) tma_drain(full_bar, stages, issued);
     __syncthreads();
@@ -315,21 +343,23 @@ static int mxt_launch_cluster(void (*kernel)(KArgs...), int threads, int smem, d
     return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-// How many CTAs of a cluster share K: the number of least time, which is returned in `time`, in units of 10 ns.  `per`: what a CTA's
-// chunk takes.  A tile takes 5 us besides, and each CTA of a cluster 3.6 ns more for a token, whose sums have to be joined; clusters
-// of a number that is no power of two start later.  128 tokens 4096 -> 4096: 37 us with one CTA a tile, 23.5 with two, 17.3 with four,
-// 17.9 with six, 31.9 with eight (two rounds); 128 x 1000 x 1536 in 4 bits: 8.5, 8.6, 9.1, 11.0 and 11.7.
-// slots[r]: clusters of r CTAs that the device holds at once.
-static int mxt_ranks(long tiles, int chunks, int tokens, const int* slots, int per, long* time = nullptr) {
+// What a kernel takes, in ns: `launch`, and for each round of the device's clusters of `ranks` CTAs a chunk's time for each of a CTA's,
+// and a tile's beginning and end: `tile`, more for each token, and for each whose sums it is sent.
+struct MxtTimes {
+    int launch, chunk, tile, token, sent;
+};
+// The clusters' size of least time for tiles of `bn` tokens, which it returns in `time`.  slots[r]: clusters of r CTAs that the device
+// holds at once.
+static int mxt_ranks(long tiles, int chunks, int bn, const int* slots, const MxtTimes& t, long* time) {
     int best = 1;
-    long least = 0;
+    *time = 0;
     for (int r = 1; r <= 8 && r <= chunks; ++r) {
-        if (slots[r] < 1) continue;
-        const long tile = (long)((chunks + r - 1) / r) * per + 500 + (long)r * tokens * 36 / 100 + (r & (r - 1) ? 150 : 0);
-        const long t = (tiles + slots[r] - 1) / slots[r] * tile;
-        if (least == 0 || t < least) best = r, least = t;
+        const int sent = (r - 1) * ((bn + r - 1) / r);
+        if (slots[r] < 1 || (bn + sent) * MXT_PITCH * 4 > MXT_RING) continue;
+        const long round = (long)((chunks + r - 1) / r) * t.chunk + t.tile + t.token * bn + t.sent * sent;
+        const long all = (tiles + slots[r] - 1) / slots[r] * round + t.launch;
+        if (*time == 0 || all < *time) best = r, *time = all;
     }
-    if (time) *time = least;
     return best;
 }
 static int mxt_failed() {
@@ -369,21 +399,33 @@ static const int* mxt_slots(void (*kernel)(KArgs...), int threads, int smem, Mxt
 template <typename TO, bool GATED>
 static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ldo, int m, int n, int k, bool constant_w, FlGate act,
                       int which, int num_sms, int* status, cudaStream_t stream) {
-    const int token_tiles = (m + MXT_BN - 1) / MXT_BN;
-    const int bn = ((m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
-    const int row_tiles = (n + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
-    const int tokens_y = (m + bn - 1) / bn, chunks = (k + 127) / 128;
+    const int row_tiles = (n + (GATED ? 127 : 255)) / (GATED ? 128 : 256), chunks = (k + 127) / 128;
     static MxtSlots found;
     const int* slots = mxt_slots(mxt_kernel<TO, GATED>, MXT_THREADS, MXT_SMEM, found);
     if (!slots) return mxt_failed();
-    // Both kernels' times, as measured: here 1.1 us a chunk, what mxt_ranks says and 2 us besides, on pairs 0.7 us
-    // a chunk and 6 us, and 8 more where a pair has one tile, whose epilogue nothing hides.  2048 tokens 4096 -> 12288: 224 us here, 180 on pairs; 1024 tokens 4096 -> 4096: 38 and 51; 512 tokens
-    // 11008 -> 4096 (K shared by clusters): 49 and 63.
-    long time, rounds;
-    const int ranks = mxt_ranks((long)tokens_y * row_tiles, chunks, bn, slots, 110, &time);
-    mxp_tokens(m, row_tiles, num_sms / 2, &rounds);
+    // Tokens of a tile and CTAs of a cluster, by what the kernel takes (fitted to 190 measured products, 16 to 517 tokens, K 1024 to 22016,
+    // 1536 to 12288 features, within 4% on average): a chunk a little more than half a us whatever the tokens, so as many of them
+    // as there are, unless the tiles are too few for the SMs.  128 tokens 11008 -> 4096: 64 a tile with four CTAs 22.1 us, 128 with four
+    // 28.1; 22016 -> 8192: 128 with four 44.7, 64 with two 63.1; 517 tokens 4096 -> 4096: 64 with one 26.9, 112 with one 34.1.
+    int bn = 0, ranks = 1;
+    long time = 0, rounds;
+    for (int most = MXT_BN; most >= 64; most -= 32) {
+        const int even = (m + most - 1) / most, tokens = ((m + even - 1) / even + 15) / 16 * 16;
+        if (tokens == bn) continue;
+        long t;
+        const MxtTimes times = {300, tokens <= 64 ? 560 + tokens * 3 / 2 : 580 + tokens * 2, 3800, 24, 22};
+        const int r = mxt_ranks((long)((m + tokens - 1) / tokens) * row_tiles, chunks, tokens, slots, times, &t);
+        if (bn == 0 || t < time) bn = tokens, ranks = r, time = t;
+    }
+    const int tokens_y = (m + bn - 1) / bn;
+    // The kernel for few rows takes 0.19 ns for 1000 elements of W: one token 22016 -> 8192: 35.7 us, 29.7 here; 4096 -> the gated 2 x
+    // 11008: 16.5, 22 here.
+    if (which == 0 && m <= MXT_FEW_ROWS && 1500 + (long)n * (GATED ? 2 : 1) * k / 1000 * 19 / 100 < time) return MXT_FEW;
+    // On pairs of CTAs: a chunk 525 ns with any tokens, and the last tile's epilogue.  517 tokens 22016 -> 8192: 193 us, 217 here; 256
+    // tokens 22016 -> 8192: 100 and 84; 2048 tokens 4096 -> 12288: 178 and 224.
+    const int pair_bn = mxp_tokens(m, row_tiles, num_sms / 2, &rounds);
     const bool fits = tokens_y <= 65535 && row_tiles <= 65535;       // a grid's y and z; pairs walk over any number of tiles
-    if (which == 2 || (which == 0 && (!fits || (m > MXT_BN && 600 + 70 * rounds * chunks + (rounds == 1 ? 800 : 0) < 200 + time))))
+    if (which == 2 || (which == 0 && (!fits || 5000 + 525 * rounds * chunks + 42 * pair_bn < time)))
         return mxp_launch<TO, GATED>(x, ldx, w, out, ldo, m, n, k, act, num_sms, status, stream);
     if (!fits) return (int)cudaErrorInvalidValue;
     const int per_rank = (chunks + ranks - 1) / ranks;
@@ -398,7 +440,8 @@ static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ld
 
 // x: bfloat16 rows, 16-byte aligned, `ldx` elements apart (a multiple of 8).  n: output features (gated: half of w's rows).
 // constant_w: nothing that may still run writes w, so its first bytes may be read while the kernels before this one run.
-// which: 0 the kernel that takes less time, 1 the one above, 2 the one on pairs of CTAs (mxfp4_pair.cuh).
+// which: 0 the kernel that takes less time, 1 the one above, 2 the one on pairs of CTAs (mxfp4_pair.cuh).  MXT_FEW: nothing has been
+// launched, the kernel for few rows (fl_mx_few) takes less.
 FL_API int fl_mxt_product(const void* x, long ldx, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int gated,
                           int act, float p0, float p1, int constant_w, int which, int num_sms, int* status, cudaStream_t stream) {
     const FlGate gate = {act, p0, p1};
@@ -417,7 +460,8 @@ FL_API int fl_mxt_product(const void* x, long ldx, const void* w, void* out, int
 #define MXQ_STAGE (3 * MX_CHUNK)
 #define MXQ_STAGES 8
 #define MXQ_SF 12                                              // columns of a stage's scales
-#define MXQ_SMEM (MXQ_STAGES * MXQ_STAGE + 1024)
+#define MXQ_SMEM MXT_SMEM
+static_assert(MXQ_STAGES * MXQ_STAGE <= MXT_RING, "the stages lie in the ring");
 
 __device__ __forceinline__ void mxq_copy_scales(uint32_t taddr, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
@@ -438,10 +482,11 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
            int ranks, int per_rank, int* __restrict__ status) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* ring = (unsigned char*)(((uintptr_t)smem_raw + 127) & ~(uintptr_t)127);
-    uint64_t* full_bar = (uint64_t*)(ring + MXQ_STAGES * MXQ_STAGE);
+    uint64_t* full_bar = (uint64_t*)(ring + MXT_RING);
     uint64_t* empty_bar = full_bar + MXQ_STAGES;
     uint64_t* acc_bar = empty_bar + MXQ_STAGES;
-    uint32_t* tmem_slot = (uint32_t*)(acc_bar + 1);
+    uint64_t* sent_bar = acc_bar + 1;
+    uint32_t* tmem_slot = (uint32_t*)(sent_bar + 1);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     const int warp = mxt_warp(), lane = threadIdx.x & 31;
     const int rank = blockIdx.x;
@@ -455,6 +500,7 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
             mbar_init(&empty_bar[s], 1);
         }
         mbar_init(acc_bar, 1);
+        mbar_init(sent_bar, 1);
         *abort_flag = (*(volatile int*)status != 0) ? 1 : 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -527,7 +573,7 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
         }
         if (going && mxt_elect()) umma_commit(acc_bar);
     }
-    mxt_finish<TO, false>(reinterpret_cast<float*>(ring), tmem_d, acc_bar, abort_flag, status, ok, c_end > c_begin, rows, ranks, rank,
+    mxt_finish<TO, false>(reinterpret_cast<float*>(ring), tmem_d, 128, acc_bar, sent_bar, abort_flag, status, ok, c_end > c_begin, rows, ranks, rank,
                           out + (long)t0 * ldo, ldo, f0, n, FlGate{FL_ACT_NONE, 0.0f, 0.0f});
     if (warp == MXT_WARPS && lane == 0 && *abort_flag) tma_drain(full_bar, MXQ_STAGES, issued);
     __syncthreads();
@@ -543,11 +589,14 @@ FL_API int fl_mxq_product(const void* a, const void* w, void* out, int out_code,
         static MxtSlots found;
         const int* slots = mxt_slots(mxq_kernel<TO>, MXT_THREADS, MXQ_SMEM, found);
         if (!slots) return mxt_failed();
+        // 15.6 us for 128 tokens 11008 -> 4096 with four CTAs, 17.6 with three, 21.5 with two, 33.2 with one; 9.3 for 16 tokens
+        // 4096 -> 12288 with two, 13.0 with four.  On pairs 25.2 us for 517 tokens 4096 -> 12288, 32.6 here; 21.6 for 192 tokens 11008 ->
+        // 4096, 16.4 here.
         long time;
-        const int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, m < 128 ? m : 128, slots, 35, &time);
+        const int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, m < 128 ? m : 128, slots, MxtTimes{500, 334, 2700, 17, 29}, &time);
         const long rounds = ((long)row_tiles * ((token_tiles + 1) / 2) + num_sms / 2 - 1) / (num_sms / 2);
         const bool fits = token_tiles <= 65535 && row_tiles <= 65535;
-        if (which == 2 || (which == 0 && (!fits || (m > 128 && 600 + rounds * (chunks * 17 + 200) < 200 + time))))
+        if (which == 2 || (which == 0 && (!fits || (m > 128 && 6000 + rounds * (chunks * 170 + 2000) < time))))
             return mxqp_launch<TO>(a, w, out, ldo, m, n, k, num_sms, status, stream);
         if (!fits) return (int)cudaErrorInvalidValue;
         const int per_rank = (chunks + ranks - 1) / ranks;

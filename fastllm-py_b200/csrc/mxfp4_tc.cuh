@@ -48,7 +48,7 @@ __device__ __forceinline__ bool mxt_test(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// A whole warp waits for a barrier's phase (limits as mbar_wait's).  All lanes ask, over and over: a wait by one lane, which may be put
+// A whole warp waits for a barrier's phase (limits as mbar_wait's; without a flag to the end).  All lanes ask, over and over: a wait by one lane, which may be put
 // to sleep, and a shuffle of the outcome took 190 clocks even where the phase was complete, and these kernels hand over from warp to
 // warp several times a chunk (4096 x 8192 x 22016 in 4 bits: 384 us so, 313 this way; 64 tokens 22016 -> 8192: 40.8 and 36.8).
 __device__ __forceinline__ bool mxt_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
@@ -56,39 +56,29 @@ __device__ __forceinline__ bool mxt_wait(uint64_t* bar, uint32_t parity, volatil
     const uint64_t t0 = global_ns();
     for (uint32_t spins = 1;; ++spins) {
         if (__all_sync(0xffffffffu, mxt_test(bar, parity))) return true;
-        if ((spins & 255u) == 0 && __any_sync(0xffffffffu, *abort_flag || global_ns() - t0 > TC_WAIT_LIMIT_NS)) return false;
+        if ((spins & 255u) == 0 && __any_sync(0xffffffffu, (abort_flag && *abort_flag) || global_ns() - t0 > TC_WAIT_LIMIT_NS)) return false;
     }
 }
-// Tokens t, t + STEP, .. of the float sums [token][PITCH] (FEAT features, of a gated unit then their up values), added up over the cluster's CTAs in rank order, through the
-// activation and out; `n`: how many features there are from the tile's first on.
-template <int V> struct MxtVec { float v[V]; };
-template <int V> __device__ __forceinline__ MxtVec<V> mxt_get(const float* sums, int ranks, int rank) {
-    MxtVec<V> r;
-    if (ranks == 1) {
-        if (V == 4) {
-            const float4 x = *reinterpret_cast<const float4*>(sums);
-            r.v[V > 3 ? 3 : 0] = x.w, r.v[V > 2 ? 2 : 0] = x.z, r.v[V > 1 ? 1 : 0] = x.y, r.v[0] = x.x;
-        } else {
+// Where the sums of a CTA's tokens are: [token][PITCH] floats of its own, and behind `parts` the other CTAs' of its cluster, in rank
+// order, `stride` floats between them, from token `first` on.
+struct MxtSums {
+    const float* own;
+    const float* parts;
+    int ranks, rank, first, stride;
+};
+// Tokens t, t + STEP, .. (FEAT features, of a gated unit then their up values), added up in rank order, through the activation and out;
+// `n`: how many features there are from the tile's first on.
+template <int V> __device__ __forceinline__ void mxt_add(const float* from, float* to) {
+    if (V == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(from);
+        to[0] += x.x, to[V > 1 ? 1 : 0] += x.y, to[V > 2 ? 2 : 0] += x.z, to[V > 3 ? 3 : 0] += x.w;
+    } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) r.v[i] = sums[i];
-        }
-        return r;
+        for (int i = 0; i < V; ++i) to[i] += from[i];
     }
-    uint32_t at;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(sums)), "r"(rank));
-    if (V == 4)
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(r.v[0]), "=f"(r.v[V > 1 ? 1 : 0]), "=f"(r.v[V > 2 ? 2 : 0]), "=f"(r.v[V > 3 ? 3 : 0])
-                     : "r"(at)
-                     : "memory");
-    else if (V == 2)
-        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(r.v[0]), "=f"(r.v[V > 1 ? 1 : 0]) : "r"(at) : "memory");
-    else
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r.v[0]) : "r"(at) : "memory");
-    return r;
 }
 template <typename TO, bool GATED, int FEAT, int PITCH, int V, int STEP>
-__device__ __forceinline__ void mxt_rows(const float* sums, int t, int last, int ranks, TO* out, long ldo, int n, const FlGate act) {
+__device__ __forceinline__ void mxt_rows(const MxtSums sums, int t, int last, TO* out, long ldo, int n, const FlGate act) {
     constexpr int PARTS = FEAT / (32 * V);                            // steps of 32 V features
     const int f0 = (threadIdx.x & 31) * V;
 #pragma unroll 2
@@ -96,20 +86,18 @@ __device__ __forceinline__ void mxt_rows(const float* sums, int t, int last, int
         float g[PARTS * V], u[PARTS * V];
 #pragma unroll
         for (int i = 0; i < PARTS * V; ++i) g[i] = 0.0f, u[i] = GATED ? 0.0f : 1.0f;
-        const float* row = sums + t * PITCH + f0;
+        const float* own = sums.own + t * PITCH + f0;
+        const float* part = sums.parts + (t - sums.first) * PITCH + f0;
 #pragma unroll 4
-        for (int q = 0; q < ranks; ++q)
+        for (int q = 0; q < sums.ranks; ++q) {
+            const float* row = q == sums.rank ? own : part;
+            part += q == sums.rank ? 0 : sums.stride;
 #pragma unroll
             for (int p = 0; p < PARTS; ++p) {
-                const MxtVec<V> x = mxt_get<V>(row + p * 32 * V, ranks, q);
-#pragma unroll
-                for (int i = 0; i < V; ++i) g[p * V + i] += x.v[i];
-                if (GATED) {
-                    const MxtVec<V> y = mxt_get<V>(row + FEAT + p * 32 * V, ranks, q);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) u[p * V + i] += y.v[i];
-                }
+                mxt_add<V>(row + p * 32 * V, g + p * V);
+                if (GATED) mxt_add<V>(row + FEAT + p * 32 * V, u + p * V);
             }
+        }
         if (act.act != FL_ACT_NONE) gated_act(g, u, act);
         TO* dst = out + (long)t * ldo + f0;
 #pragma unroll
@@ -127,25 +115,6 @@ __device__ __forceinline__ void mxt_rows(const float* sums, int t, int last, int
     }
 }
 
-// The same tokens' sums over the cluster left in this CTA's own rows, which no other CTA reads: for rows that leave an element at a
-// time, since single elements from another CTA take as long as four (261 x 1000 x 1537 in 4 bits: 10.0 us, and 5 of them here).
-template <int WIDTH, int PITCH, int STEP>
-__device__ __forceinline__ void mxt_gather(float* sums, int t, int last, int ranks) {
-#pragma unroll 2
-    for (; t < last; t += STEP)
-#pragma unroll
-        for (int p = 0; p < WIDTH; p += 128) {
-            float* at = sums + t * PITCH + p + (threadIdx.x & 31) * 4;
-            float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-            for (int q = 0; q < ranks; ++q) {
-                const MxtVec<4> x = mxt_get<4>(at, ranks, q);
-                r.x += x.v[0], r.y += x.v[1], r.z += x.v[2], r.w += x.v[3];
-            }
-            *reinterpret_cast<float4*>(at) = r;
-        }
-    __syncwarp();
-}
 __device__ __forceinline__ void mxt_give_up(volatile int* abort_flag, int* status) {
     if (!*abort_flag) {
         *abort_flag = 1;
@@ -158,6 +127,18 @@ __device__ __forceinline__ void mxt_copy(void* dst, const void* src, uint32_t by
                  "r"(bytes), "r"(smem_u32(bar))
                  : "memory");
 }
+
+// Shared memory to the same place of CTA `rank` of the cluster, and to its barrier.
+__device__ __forceinline__ void mxt_push(void* dst, const void* src, uint32_t bytes, uint64_t* bar, int rank) {
+    uint32_t to, signal;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(dst)), "r"(rank));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(signal) : "r"(smem_u32(bar)), "r"(rank));
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "r"(smem_u32(src)),
+                 "r"(bytes), "r"(signal)
+                 : "memory");
+}
+__device__ __forceinline__ void mxt_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void mxt_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // ------------------------------------------------------------------ both operands in 4 bits
 // A tile's codes as an operand of the block-scaled matrix instruction: no swizzle: `lead` bytes between core matrices along K, 128 between those of neighbouring groups of 8 rows

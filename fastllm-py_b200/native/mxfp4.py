@@ -157,7 +157,9 @@ def dequantize(q: Matrix, out: torch.Tensor) -> None:
     ops._check(_fn(_DEQUANTIZE)(data.data_ptr(), out.data_ptr(), code, pitch, q.rows, q.k, stream), "mxfp4.dequantize")
 
 
-FEW_ROWS = 8                                    # most rows that the kernel for few of them takes
+# The kernel for few rows takes up to 8 of them, and no more time than those on the tensor cores with matrices of up to 2^26 values
+# (one row, 4096 -> 12288: 10.1 and 13.9 us); with larger ones their launcher says which does (LESS: fl_mx_few, csrc/mxfp4_tc.cu).
+FEW_ROWS, FEW_VALUES, LESS = 8, 1 << 26, -1
 
 
 def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, constant_w, kernel) -> None:
@@ -176,12 +178,13 @@ def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, consta
     if m == 0:
         return
     status, sms = _known(x)
-    if m <= FEW_ROWS and kernel == 0:
-        rc = _fn(_FEW)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
-                       constant_w, sms, stream)
-    else:
+    rc = LESS
+    if kernel or m > FEW_ROWS or w.rows * k > FEW_VALUES:
         rc = _fn(_MANY)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
                         constant_w, kernel, sms, status, stream)
+    if rc == LESS:
+        rc = _fn(_FEW)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
+                       constant_w, sms, stream)
     ops._check(rc, name)
 
 

@@ -540,3 +540,32 @@ def test_two_captured_products_replayed_at_the_same_time():
     for out, want in outs:
         assert all(torch.equal(o, v) for o, v in zip(out, want))
     check_sum(outs[0][0][0], x @ w.T, np.abs(x) @ np.abs(w).T, k, torch.float32)
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 4096, 20000), (8, 4096, 20000), (2, 40000, 2048), (7, 40000, 2048)])
+def test_few_rows_with_a_large_matrix(m, n, k):
+    """Matrices of more than 2^26 values, for which one or the other kernel takes less: a plain product and a gated one of each, at
+    chosen features against 64 bits and as a whole against the other kernel."""
+    from fastllm_py_b200.native import mxfp4
+
+    g = torch.Generator(device=DEV).manual_seed(m + n)
+    x = torch.randn(m, k, generator=g, device=DEV).to(torch.bfloat16)
+    q = mxfp4.Matrix.of(torch.randn(n, k, generator=g, device=DEV) / k ** 0.5)
+    some = torch.arange(0, n, 997, device=DEV)
+    w = torch.empty(n, k, dtype=torch.bfloat16, device=DEV)
+    mxfp4.dequantize(q, w)
+    xs, ws = x.double().cpu().numpy(), w[some].double().cpu().numpy()
+    outs = [torch.empty(m, n, dtype=torch.float32, device=DEV) for _ in range(2)]
+    units = [torch.empty(m, n // 2, dtype=torch.float32, device=DEV) for _ in range(2)]
+    for kernel in (0, 1):
+        mxfp4.linear(x, q, outs[kernel], kernel=kernel)
+        mxfp4.linear_gated(x, q, units[kernel], kernel=kernel)
+    check_sum(outs[0][:, some], xs @ ws.T, np.abs(xs) @ np.abs(ws).T, k, torch.float32)
+    # the other kernel's sums differ by twice what either may be off
+    off = 2 * (k / 16 + 64) * 2.0 ** -23 * (x.abs().double() @ w.abs().double().T)
+    assert bool(((outs[0].double() - outs[1].double()).abs() <= off).all())
+    gate, up = outs[0].double().split(n // 2, dim=1)
+    eg, eu = off.split(n // 2, dim=1)
+    # silu's slope is at most 1.1, its value at most |g|; its own evaluation in float is within 2^-18, twice
+    unit = up * gate * torch.sigmoid(gate)
+    assert bool(((units[0].double() - units[1].double()).abs() <= 1.1 * eg * up.abs() + gate.abs() * eu + eg * eu + 2.0 ** -17 * unit.abs()).all())
