@@ -3,14 +3,18 @@
 //
 // A pair's tile is 256 rows of W x up to 192 tokens.  Each CTA turns its 128 rows of W into bfloat16 in its own tensor memory (as
 // mxfp4_tc.cu does) and loads half of the tokens; the MMA reads both halves, so a CTA moves and converts half of what two CTAs with
-// tiles of 256 x 128 would.  Tensor memory holds two accumulators of 192 columns and four places of 32 columns for W (64 elements
-// along K): the next tile's
-// MMAs run while the epilogue's warps empty the last one's accumulator, 32 tokens a round through shared memory.  (With 256 tokens
-// there is room for one accumulator.)  Persistent: a pair walks over its tiles.
+// tiles of 256 x 128 would.  Tensor memory holds two accumulators of 192 columns and two places of 64 columns for a chunk of W: the
+// next tile's MMAs run while the epilogue's warps empty the last one's accumulator, 32 tokens a round through shared memory.  (With 256
+// tokens there is room for one accumulator.)  Persistent: a pair walks over its tiles.
 //
-// Warps 0-15 convert, four of them half of a chunk of 128 along K, a thread one row (with eight warps a chunk took 1300 clocks, mostly
-// waiting; its MMAs take 770); warps 16-19 are the epilogue; warps 20 and 22 send for the tokens and the codes, warp 21 of the pair's
-// even CTA (the leader) issues the MMAs.
+// Warps 0-15 convert, four of them half of a chunk of 128 along K, a thread one row; warps 16-19 are the epilogue; warps 20 and 22 send
+// for the tokens and the codes, warp 21 of the pair's even CTA (the leader) issues the MMAs.
+//
+// What bounds it: a chunk's way through wait, conversion, store to tensor memory and arrival, 1850 clocks of a warp for every other one;
+// MMAs alone take 660 a chunk with 128 tokens, 770 with 192.  The issuing warp has few instructions to spare: with a barrier for each
+// half of a chunk and one for its tokens a chunk took 1070 clocks, however small; it now waits for one, at which a converting
+// warp arrives when it has seen the tokens too.  256 tokens 22016 -> 8192: 100 us, 86 so; 2048 tokens 11008 -> 4096: 172 and 146 (1.26
+// PFLOP/s), 4096 -> the gated 2 x 11008 270 (1.37 PFLOP/s, what the power limit leaves of the rate).
 #pragma once
 
 #include "mxfp4_tc.cuh"
@@ -98,8 +102,8 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
     uint64_t* w_full = x_empty + MXP_X_STAGES;
     uint64_t* w_empty = w_full + MXP_W_STAGES;
     uint64_t* a_full = w_empty + MXP_W_STAGES;                                      // (the leader's)
-    uint64_t* a_empty = a_full + 4;
-    uint64_t* acc_full = a_empty + 4;
+    uint64_t* a_empty = a_full + 2;
+    uint64_t* acc_full = a_empty + 2;
     uint64_t* acc_empty = acc_full + 2;                                             // (the leader's)
     uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
@@ -117,8 +121,8 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
             mbar_init(&w_full[s], 1);
             mbar_init(&w_empty[s], 8);
         }
-        for (int p = 0; p < 4; ++p) {
-            mbar_init(&a_full[p], 8);                        // four warps in each CTA
+        for (int p = 0; p < 2; ++p) {
+            mbar_init(&a_full[p], 16);                       // eight warps in each CTA
             mbar_init(&a_empty[p], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -138,16 +142,17 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
     __syncthreads();
     cluster_sync_all();                                      // both CTAs' barriers exist before anyone signals them
     tc_fence_after();
-    // accumulator b at 192 b, place p of W at 384 + 32 p.  (Launched in plain stream order, as every kernel with cta_group::2.)
+    // accumulator b at 192 b, place p of W at 384 + 64 p.  (Launched in plain stream order, as every kernel with cta_group::2.)
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     bool ok = !*abort_flag;
     int issued = 0;
     if (warp < 16) {
         // ---- codes to bfloat16
-        const int turn = warp >> 3, h = warp >> 2 & 1, r = threadIdx.x & 127;       // every other chunk, one half; place 2 turn + h
+        const int turn = warp >> 3, h = warp >> 2 & 1, r = threadIdx.x & 127;       // every other chunk, one half
         const uint32_t dst = tmem + 384u + (uint32_t)(turn * 64 + h * 32) + ((uint32_t)((warp & 3) * 32) << 16);
-        int s = 0, it = 0;                                   // stage of the chunk, chunks so far
-        uint32_t ph = 0, pa = 0;
+        int s = 0, x = 0, it = 0;                            // stages of the chunk's codes and tokens, chunks so far
+        uint32_t ph = 0, xph = 0, pa = 0;
+        const bool looks = rank == 0 && (warp & 7) == 0;     // for the tokens: the MMAs then need one barrier
         for (int tile = pair; tile < tiles && ok; tile += pairs) {
             const int f0 = tile / token_tiles * (2 * FEAT) + rank * FEAT;
             // where the row's scales are: the gate rows lie in one packed tile, the up rows in one or two
@@ -175,7 +180,7 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
                         mx_block_large(qa, sa, v);
                         mx_block_large(qb, sb, v + 16);
                     }
-                    if (!mxt_wait(&a_empty[2 * turn + h], pa ^ 1u, abort_flag)) {
+                    if ((looks && !mxt_wait(&x_full[x], xph, abort_flag)) || !mxt_wait(&a_empty[turn], pa ^ 1u, abort_flag)) {
                         if (lane == 0) mxt_give_up(abort_flag, status);
                         ok = false;
                         break;
@@ -186,9 +191,13 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_leader(&a_full[2 * turn + h]);
+                    if (lane == 0) {
+                        if (rank == 0) mxt_arrive(&a_full[turn]);
+                        else mbar_arrive_leader(&a_full[turn]);
+                    }
                     pa ^= 1u;
                 }
+                if (++x == x_stages) { x = 0; xph ^= 1u; }
                 if (++s == MXP_W_STAGES) { s = 0; ph ^= 1u; }
             }
         }
@@ -282,42 +291,34 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
         // ---- MMA issuer, for both CTAs
         const uint32_t idesc = instr_desc_bf16(256, bn), ring_at = smem_u32(ring);
         const uint64_t half = (uint64_t)(x_bytes / 2) >> 4;
-        int s = 0, i = 0, it = 0;
-        uint32_t ph = 0;
-        bool there = false;                                  // what the next instructions read is known to be there
+        int s = 0, i = 0;
+        uint32_t turn = 0, pa = 0;
+        bool there = false;                                  // the next chunk is known to be there, its tokens too
         for (int tile = pair; tile < tiles && ok; tile += pairs, ++i) {
             const int b = i & 1;
             ok = mxt_wait(&acc_empty[b], ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag);
             const uint32_t acc = tmem + (uint32_t)(b * 192);
-            for (int c = 0; c < chunks && ok; ++c, ++it) {
-                const uint64_t bdesc = smem_desc_sw128(ring_at + (uint32_t)(s * x_bytes));
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t place = 2u * ((uint32_t)it & 1u) + (uint32_t)h;
-                    if (!__all_sync(0xffffffffu, there)) {
-                        ok = (h || mxt_wait(&x_full[s], ph, abort_flag)) && mxt_wait(&a_full[place], (uint32_t)(it >> 1) & 1u, abort_flag);
-                        if (!ok) break;
-                    }
-                    tc_fence_after();
-                    if (h == 0) {
-                        there = mxt_test(&a_full[place + 1], (uint32_t)(it >> 1) & 1u);
-                    } else {
-                        const int next = s + 1 == x_stages ? 0 : s + 1;
-                        there = mxt_test(&x_full[next], next ? ph : ph ^ 1u) && mxt_test(&a_full[2u * ((uint32_t)(it + 1) & 1u)], (uint32_t)((it + 1) >> 1) & 1u);
-                    }
-                    if (mxt_elect()) {
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            mxp_umma_ts(acc, tmem + 384u + place * 32u + (uint32_t)(kk * 8), bdesc + (uint64_t)(2 * kk) + (h ? half : 0), idesc,
-                                        (c > 0 || h > 0 || kk > 0) ? 1u : 0u);
-                        umma_commit_pair(&a_empty[place]);
-                        if (h) umma_commit_pair(&x_empty[s]);
-                        if (h && c == chunks - 1) umma_commit_pair(&acc_full[b]);
-                    }
-                    __syncwarp();
+            for (int c = 0; c < chunks && ok; ++c) {
+                if (!__all_sync(0xffffffffu, there) && !mxt_wait(&a_full[turn], pa, abort_flag)) {
+                    ok = false;
+                    break;
                 }
-                if (!ok) break;
-                if (++s == x_stages) { s = 0; ph ^= 1u; }
+                tc_fence_after();
+                there = mxt_test(&a_full[turn ^ 1u], turn ? pa ^ 1u : pa);
+                if (mxt_elect()) {
+                    const uint64_t bdesc = smem_desc_sw128(ring_at + (uint32_t)(s * x_bytes));
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk)
+                        mxp_umma_ts(acc, tmem + 384u + turn * 64u + (uint32_t)(kk * 8), bdesc + (uint64_t)(2 * (kk & 3)) + (kk >= 4 ? half : 0), idesc,
+                                    (c > 0 || kk > 0) ? 1u : 0u);
+                    umma_commit_pair(&a_empty[turn]);
+                    umma_commit_pair(&x_empty[s]);
+                    if (c == chunks - 1) umma_commit_pair(&acc_full[b]);
+                }
+                __syncwarp();
+                if (++s == x_stages) s = 0;
+                pa ^= turn;
+                turn ^= 1u;
             }
             if (!ok && lane == 0) mxt_give_up(abort_flag, status);
         }
@@ -332,16 +333,17 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
     if (warp == 21) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-// Tokens of a tile: the multiple of 32 up to 192 with which the pairs go round their tiles least often (a chunk takes the same time
-// with any: its hand-overs, rather than its MMAs); `rounds`: how often.
+// What a chunk takes, in ns: the conversion and its hand-overs up to 160 tokens, with 192 the MMAs (K 22016: 86 us with 64 and with 128
+// tokens a tile, 104 with 192; 2048 tokens 4096 -> 12288 with 192 in eight rounds 162, with 160 in nine 168).
+static int mxp_chunk(int bn) { return bn <= 160 ? 455 : 510; }
+// Tokens of a tile: the multiple of 32 up to 192 with which the pairs take the least time for all their rounds; `rounds`: how many.
 static int mxp_tokens(int m, int row_tiles, int pairs, long* rounds) {
     int best = 32;
     long least = 0;
     for (int bn = 32; bn <= MXP_BN; bn += 32) {
         const long r = ((long)row_tiles * ((m + bn - 1) / bn) + pairs - 1) / pairs;
-        if (least == 0 || r < least) best = bn, least = r;
+        if (least == 0 || r * mxp_chunk(bn) < least) best = bn, least = r * mxp_chunk(bn), *rounds = r;
     }
-    *rounds = least;
     return best;
 }
 
