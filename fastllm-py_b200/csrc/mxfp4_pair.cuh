@@ -42,6 +42,25 @@ __device__ __forceinline__ void mxp_umma_ts(uint32_t tmem_d, uint32_t tmem_a, ui
         "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// The packed form as a tensor of 8-byte elements [chunks][4 pieces][256], for copies of 64 rows' codes of a chunk: a gated unit's rows.
+// (As single copies of 1024 bytes they are eight a chunk: 2048 tokens, 4096 -> the gated 2 x 11008 306 us, and 292 with tensors.)
+static int mxp_map_codes(CUtensorMap* map, const void* w, long rows, int chunks) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return (int)cudaErrorNotSupported;
+    cuuint64_t dims[3] = {256, 4, (cuuint64_t)((rows + MX_ROWS - 1) / MX_ROWS * chunks)};
+    cuuint64_t strides[2] = {2048, MX_CHUNK};
+    cuuint32_t box[3] = {128, 4, 1}, elem[3] = {1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_INT64, 3, const_cast<void*>(w), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+// 64 rows' codes of a chunk, from the tile's row 0 or 64 on
+__device__ __forceinline__ void mxp_copy_codes(void* dst, const CUtensorMap* map, uint64_t* bar, int row, int chunk) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(row * 2), "r"(0), "r"(chunk)
+        : "memory");
+}
 // A barrier of the four epilogue warps, and whether any thread came with `flag`: they leave together or not at all.
 __device__ __forceinline__ bool mxp_vote(bool flag) {
     uint32_t any;
@@ -90,7 +109,7 @@ __device__ __forceinline__ bool mxp_epilogue(uint32_t tmem_acc, float* staged, u
 // row_tiles x token_tiles tiles; bn: tokens of a tile, a multiple of 32.
 template <typename TO, bool GATED>
 __global__ void __launch_bounds__(MXP_THREADS, 1)
-mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ w, TO* __restrict__ out, long ldo, int m, int n, int k,
+mxp_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const uint8_t* __restrict__ w, TO* __restrict__ out, long ldo, int m, int n, int k,
            int bn, int x_stages, int token_tiles, int tiles, FlGate act, int* __restrict__ status) {
     constexpr int FEAT = GATED ? 64 : 128;
     extern __shared__ unsigned char smem_raw[];
@@ -150,6 +169,8 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
         // ---- codes to bfloat16
         const int turn = warp >> 3, h = warp >> 2 & 1, r = threadIdx.x & 127;       // every other chunk, one half
         const uint32_t dst = tmem + 384u + (uint32_t)(turn * 64 + h * 32) + ((uint32_t)((warp & 3) * 32) << 16);
+        // (a gated unit's 64 gate rows lie before its up rows)
+        const int codes_at = GATED ? (r >> 6) * 4096 + h * 2048 + (r & 63) * 16 : h * 4096 + r * 16;
         int s = 0, x = 0, it = 0;                            // stages of the chunk's codes and tokens, chunks so far
         uint32_t ph = 0, xph = 0, pa = 0;
         const bool looks = rank == 0 && (warp & 7) == 0;     // for the tokens: the MMAs then need one barrier
@@ -166,8 +187,8 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
                         break;
                     }
                     const unsigned char* stage = w_ring + s * MXP_W_STAGE;
-                    const uint4 qa = *reinterpret_cast<const uint4*>(stage + h * 4096 + r * 16);
-                    const uint4 qb = *reinterpret_cast<const uint4*>(stage + h * 4096 + 2048 + r * 16);
+                    const uint4 qa = *reinterpret_cast<const uint4*>(stage + codes_at);
+                    const uint4 qb = *reinterpret_cast<const uint4*>(stage + codes_at + (GATED ? 1024 : 2048));
                     const uint32_t sa = stage[scale_at], sb = stage[scale_at + 1];
                     const bool large = __any_sync(0xffffffffu, max(sa, sb) > 128u);
                     __syncwarp();
@@ -269,15 +290,17 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
                     } else if (!GATED) {
                         mxt_copy(dst, src, MX_CHUNK, &w_full[s]);
                     } else {
-                        for (int b = 0; b < 4; ++b) mxt_copy(dst + b * 2048, src + b * 2048 + off0 * 16, 1024, &w_full[s]);
+                        mxp_copy_codes(dst, &map_w, &w_full[s], off0, (int)(f0 / MX_ROWS) * chunks + c);
                         mxt_copy(dst + MX_CODES, src + MX_CODES, 512, &w_full[s]);
                         src = src1 + (long)c * MX_CHUNK;
-                        for (int b = 0; b < 4; ++b) mxt_copy(dst + b * 2048 + 1024, src + b * 2048 + off1 * 16, (uint32_t)first * 16, &w_full[s]);
+                        if ((off1 & 63) == 0) mxp_copy_codes(dst + 4096, &map_w, &w_full[s], off1, (int)(row1 / MX_ROWS) * chunks + c);
+                        else
+                            for (int b = 0; b < 4; ++b) mxt_copy(dst + 4096 + b * 1024, src + b * 2048 + off1 * 16, (uint32_t)first * 16, &w_full[s]);
                         mxt_copy(dst + MX_CODES + 512, src + MX_CODES, 512, &w_full[s]);
                         if (rest) {
                             src += tile_bytes;
                             for (int b = 0; b < 4; ++b)
-                                mxt_copy(dst + b * 2048 + 1024 + first * 16, src + b * 2048, (uint32_t)rest * 16, &w_full[s]);
+                                mxt_copy(dst + 4096 + b * 1024 + first * 16, src + b * 2048, (uint32_t)rest * 16, &w_full[s]);
                             mxt_copy(dst + MX_CODES + 1024, src + MX_CODES, 512, &w_full[s]);
                         }
                     }
@@ -358,6 +381,8 @@ static int mxp_launch(const void* x, long ldx, const void* w, void* out, long ld
     CUtensorMap map;
     int rc = make_map(&map, x, m, k, ldx, bn / 2);
     if (rc) return rc;
+    CUtensorMap map_w = map;                                 // (unused where W comes in whole chunks)
+    if (GATED && (rc = mxp_map_codes(&map_w, w, 2l * n, chunks))) return rc;
     auto kernel = mxp_kernel<TO, GATED>;
     static bool configured[MX_DEVICES];
     const int device = mx_device();
@@ -380,7 +405,7 @@ static int mxp_launch(const void* x, long ldx, const void* w, void* out, long ld
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, map, (const uint8_t*)w, (TO*)out, ldo, m, n, k, bn,
+    return (int)cudaLaunchKernelEx(&cfg, kernel, map, map_w, (const uint8_t*)w, (TO*)out, ldo, m, n, k, bn,
                                    stages < MXP_X_STAGES ? stages : MXP_X_STAGES, (m + bn - 1) / bn, (int)tiles, act, status);
 }
 
