@@ -455,11 +455,16 @@ FL_API int fl_mxt_product(const void* x, long ldx, const void* w, void* out, int
 // ---------------------------------------------------------------- both operands in 4 bits
 // out[t, f] = sum_k A[t, k] W[f, k] on the block-scaled matrix instruction: codes in shared memory as they lie in the packed form (a
 // row's 16 bytes of a block are a line of an 8 x 16-byte core matrix; core matrices 128 bytes apart along the rows, 2048 along
-// K), the scales copied from there to tensor memory, 4 columns for 128 rows x 4 blocks.  A stage is a chunk of 128 along K of two
-// tiles of W's rows and of one of A's: three copies.
-#define MXQ_STAGE (3 * MX_CHUNK)
-#define MXQ_STAGES 8
-#define MXQ_SF 12                                              // columns of a stage's scales
+// K), the scales copied from there to tensor memory, 4 columns for 128 rows x 4 blocks.  A stage is two chunks of 128 along K, side by
+// side in the packed form, of two tiles of W's rows and of one of A's: three copies.
+//
+// What bounds it: few rows the bytes (64 x 8192 x 22016 21.2 us, 4.5 TB/s), small products the way in and out (16 x 256 x 128 takes
+// 2.8 us, 261 x 1537 x 1000 8.4, 4.5 of them after its last stage).  A stage takes 0.56 us, its MMAs 0.27: the rest is the
+// issuing warp's, which has three instructions for the scales of each chunk.  (Stages of one chunk: 0.33 us, and 128 x 4096 x 11008
+// 15.5 us in place of 14.1.)
+#define MXQ_STAGE (6 * MX_CHUNK)
+#define MXQ_STAGES 4
+#define MXQ_SF 24                                              // columns of a stage's scales: 12 for each chunk
 #define MXQ_SMEM MXT_SMEM
 static_assert(MXQ_STAGES * MXQ_STAGE <= MXT_RING, "the stages lie in the ring");
 
@@ -492,7 +497,7 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
     const int rank = blockIdx.x;
     const int t0 = blockIdx.y * 128, f0 = blockIdx.z * 256;
     const int rows = min(128, m - t0), tiles = n - f0 > 128 ? 2 : 1;
-    const int c_begin = rank * per_rank, c_end = min(chunks, c_begin + per_rank);
+    const int c_begin = rank * per_rank, c_end = min((chunks + 1) / 2, c_begin + per_rank);       // stages along K
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < MXQ_STAGES; ++s) {
@@ -530,10 +535,11 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
             }
             if (mxt_elect()) {
                 unsigned char* dst = ring + s * MXQ_STAGE;
-                mbar_expect_tx(&full_bar[s], (uint32_t)((tiles + 1) * MX_CHUNK));
-                mxt_copy(dst, src_a + (long)c * MX_CHUNK, MX_CHUNK, &full_bar[s]);
+                const uint32_t bytes = 2 * c + 1 < chunks ? 2 * MX_CHUNK : MX_CHUNK;
+                mbar_expect_tx(&full_bar[s], (uint32_t)(tiles + 1) * bytes);
+                mxt_copy(dst, src_a + 2l * c * MX_CHUNK, bytes, &full_bar[s]);
                 for (int t = 0; t < tiles; ++t)
-                    mxt_copy(dst + (1 + t) * MX_CHUNK, src_w + ((long)t * chunks + c) * MX_CHUNK, MX_CHUNK, &full_bar[s]);
+                    mxt_copy(dst + (1 + t) * 2 * MX_CHUNK, src_w + ((long)t * chunks + 2 * c) * MX_CHUNK, bytes, &full_bar[s]);
             }
             __syncwarp();
             ++issued;
@@ -558,14 +564,18 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
             const uint32_t at = ring_at + (uint32_t)(s * MXQ_STAGE), sf = tmem_sf + (uint32_t)(s * MXQ_SF);
             if (mxt_elect()) {
                 // (the stage's columns: its last use's MMAs were done before its copies were sent for)
-                for (int t = 0; t <= tiles; ++t)
-                    mxq_copy_scales(sf + (uint32_t)(4 * t), mxq_desc(at + (uint32_t)(t * MX_CHUNK + MX_CODES), 128));
-                for (int t = 0; t < tiles; ++t)
+                const int two = 2 * c + 1 < chunks ? 2 : 1;
+                for (int i = 0; i < two; ++i) {
+                    const uint32_t from = at + (uint32_t)(i * MX_CHUNK), to = sf + (uint32_t)(12 * i);
+                    for (int t = 0; t <= tiles; ++t)
+                        mxq_copy_scales(to + (uint32_t)(4 * t), mxq_desc(from + (uint32_t)(t * 2 * MX_CHUNK + MX_CODES), 128));
+                    for (int t = 0; t < tiles; ++t)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        mxq_umma(tmem_d + (uint32_t)(t * 128), mxq_desc(at + (uint32_t)((1 + t) * MX_CHUNK + h * 4096), 2048),
-                                 mxq_desc(at + (uint32_t)(h * 4096), 2048), idesc[h], sf + (uint32_t)(4 + 4 * t), sf,
-                                 (c > c_begin || h > 0) ? 1u : 0u);
+                        for (int h = 0; h < 2; ++h)
+                            mxq_umma(tmem_d + (uint32_t)(t * 128), mxq_desc(from + (uint32_t)((1 + t) * 2 * MX_CHUNK + h * 4096), 2048),
+                                     mxq_desc(from + (uint32_t)(h * 4096), 2048), idesc[h], to + (uint32_t)(4 + 4 * t), to,
+                                     (c > c_begin || i > 0 || h > 0) ? 1u : 0u);
+                }
                 umma_commit(&empty_bar[s]);
             }
             __syncwarp();
@@ -584,22 +594,22 @@ mxq_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __r
 // (mxfp4_pair.cuh).
 FL_API int fl_mxq_product(const void* a, const void* w, void* out, int out_code, long ldo, int m, int n, int k, int which, int num_sms,
                           int* status, cudaStream_t stream) {
-    const int chunks = (k + 127) / 128, token_tiles = (m + 127) / 128, row_tiles = (n + 255) / 256;
+    const int chunks = (k + 127) / 128, stages = (chunks + 1) / 2, token_tiles = (m + 127) / 128, row_tiles = (n + 255) / 256;
     FL_DISPATCH(out_code, TO, {
         static MxtSlots found;
         const int* slots = mxt_slots(mxq_kernel<TO>, MXT_THREADS, MXQ_SMEM, found);
         if (!slots) return mxt_failed();
-        // 15.6 us for 128 tokens 11008 -> 4096 with four CTAs, 17.6 with three, 21.5 with two, 33.2 with one; 9.3 for 16 tokens
-        // 4096 -> 12288 with two, 13.0 with four.  On pairs 25.2 us for 517 tokens 4096 -> 12288, 32.6 here; 21.6 for 192 tokens 11008 ->
-        // 4096, 16.4 here.
+        // 14.1 us for 128 tokens 11008 -> 4096 with four CTAs, 16.2 with three, 19.0 with two, 28.0 with one; 8.5 for 16 tokens
+        // 4096 -> 12288 with two, 12.4 with four.  On pairs 24.9 us for 517 tokens 4096 -> 12288, 28.8 here; 21.7 for 192 tokens 11008 ->
+        // 4096, 14.8 here.
         long time;
-        const int ranks = mxt_ranks((long)token_tiles * row_tiles, chunks, m < 128 ? m : 128, slots, MxtTimes{500, 334, 2700, 17, 29}, &time);
+        const int ranks = mxt_ranks((long)token_tiles * row_tiles, stages, m < 128 ? m : 128, slots, MxtTimes{340, 564, 2800, 16, 31}, &time);
         const long rounds = ((long)row_tiles * ((token_tiles + 1) / 2) + num_sms / 2 - 1) / (num_sms / 2);
         const bool fits = token_tiles <= 65535 && row_tiles <= 65535;
         if (which == 2 || (which == 0 && (!fits || (m > 128 && 6000 + rounds * (chunks * 170 + 2000) < time))))
             return mxqp_launch<TO>(a, w, out, ldo, m, n, k, num_sms, status, stream);
         if (!fits) return (int)cudaErrorInvalidValue;
-        const int per_rank = (chunks + ranks - 1) / ranks;
+        const int per_rank = (stages + ranks - 1) / ranks;
         return mxt_launch_cluster(mxq_kernel<TO>, MXT_THREADS, MXQ_SMEM, dim3(ranks, token_tiles, row_tiles), stream, (const uint8_t*)a,
                                   (const uint8_t*)w, (TO*)out, ldo, m, n, chunks, ranks, per_rank, status);
     })
