@@ -48,15 +48,17 @@ __device__ __forceinline__ bool mxt_test(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// A whole warp waits for a barrier's phase (limits as mbar_wait's; without a flag to the end).  All lanes ask, over and over: a wait by one lane, which may be put
-// to sleep, and a shuffle of the outcome took 190 clocks even where the phase was complete, and these kernels hand over from warp to
-// warp several times a chunk (4096 x 8192 x 22016 in 4 bits: 384 us so, 313 this way; 64 tokens 22016 -> 8192: 40.8 and 36.8).
+// A whole warp waits for a barrier's phase (limits as mbar_wait's; without a flag to the end).  All lanes ask, first without being put
+// to sleep: a wait by one lane and a shuffle of the outcome took 190 clocks even where the phase was complete, and these kernels
+// hand over from warp to warp several times a chunk (4096 x 8192 x 22016 in 4 bits: 384 us so, 313 this way; 64 tokens 22016 -> 8192:
+// 40.8 and 36.8).  Where it is not they may be: asking over and over takes issue slots from the others (40 x 4096 x 12288 in 4 bits
+// 9.6 us, and 9.0 so).
 __device__ __forceinline__ bool mxt_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
     if (__all_sync(0xffffffffu, mxt_test(bar, parity))) return true;
     const uint64_t t0 = global_ns();
     for (uint32_t spins = 1;; ++spins) {
-        if (__all_sync(0xffffffffu, mxt_test(bar, parity))) return true;
-        if ((spins & 255u) == 0 && __any_sync(0xffffffffu, (abort_flag && *abort_flag) || global_ns() - t0 > TC_WAIT_LIMIT_NS)) return false;
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity) != 0)) return true;
+        if ((spins & 15u) == 0 && __any_sync(0xffffffffu, (abort_flag && *abort_flag) || global_ns() - t0 > TC_WAIT_LIMIT_NS)) return false;
     }
 }
 // Where the sums of a CTA's tokens are: [token][PITCH] floats of its own, and behind `parts` the other CTAs' of its cluster, in rank
