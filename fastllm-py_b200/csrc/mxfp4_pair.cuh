@@ -174,6 +174,8 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
         int s = 0, x = 0, it = 0;                            // stages of the chunk's codes and tokens, chunks so far
         uint32_t ph = 0, xph = 0, pa = 0;
         const bool looks = rank == 0 && (warp & 7) == 0;     // for the tokens: the MMAs then need one barrier
+        // (a stage of the tokens may have been the other group's before: a turn ago this one waited for the MMAs of four chunks back, and
+        // there are more stages than that)
         for (int tile = pair; tile < tiles && ok; tile += pairs) {
             const int f0 = tile / token_tiles * (2 * FEAT) + rank * FEAT;
             // where the row's scales are: the gate rows lie in one packed tile, the up rows in one or two
@@ -393,6 +395,7 @@ static int mxp_launch(const void* x, long ldx, const void* w, void* out, long ld
         configured[device] = true;
     }
     const int stages = MXP_X_RING / (bn * 128);
+    static_assert(MXP_X_RING / (MXP_BN * 128) >= 5 && MXP_X_STAGES >= 5 && MXP_W_STAGES % 2 == 0, "as the converting warps' waits need");
     const long pairs = tiles < num_sms / 2 ? tiles : num_sms / 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(2 * pairs));
@@ -502,7 +505,10 @@ mxqp_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __
             for (int step = 0; step < steps; ++step, ++it) {
                 if ((it & 3) != warp >> 2) continue;
                 const int s = it % MXQP_STAGES;
-                if (!mxt_wait(&full_bar[s], (uint32_t)(it / MXQP_STAGES) & 1u, abort_flag)) {
+                const uint32_t ph = (uint32_t)(it / MXQP_STAGES) & 1u;
+                // (The stage's use before was another group's, and copies land in any order: unless its MMAs are known to be done, this
+                // use's parity may be that of a phase before it.  Those of this use need this group, so that barrier is not passed twice.)
+                if (!mxt_wait(&empty_bar[s], ph ^ 1u, abort_flag) || !mxt_wait(&full_bar[s], ph, abort_flag)) {
                     if (lane == 0) mxt_give_up(abort_flag, status);
                     ok = false;
                     break;

@@ -229,6 +229,8 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
         const int codes_at = x_bytes + tile * (MX_CODES + 1024) + r * 16;
         const int scale_at = x_bytes + tile * (MX_CODES + 1024) + (rr >> 7) * 512 + mx_scale_at(rr & 127);
         const uint32_t lanes = tmem_a + (uint32_t)(tile * 64) + ((uint32_t)((warp & 3) * 32) << 16);
+        // (a stage's or a place's use before may have been the other group's: this one has waited, a turn ago, for the MMAs of four or five
+        // chunks back, and there are at least as many stages as that)
         int s = turn, place = turn;
         uint32_t ph = 0, pa = 0;
         if (s >= stages) s -= stages, ph ^= 1u;
@@ -429,8 +431,9 @@ static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ld
         return mxp_launch<TO, GATED>(x, ldx, w, out, ldo, m, n, k, act, num_sms, status, stream);
     if (!fits) return (int)cudaErrorInvalidValue;
     const int per_rank = (chunks + ranks - 1) / ranks;
-    int stages = MXT_RING / (bn * 256 + MXT_W_BYTES);
+    int stages = MXT_RING / (bn * 256 + MXT_W_BYTES);               // (up to 64 tokens six at the least, else four)
     if (stages > MXT_MAX_STAGES) stages = MXT_MAX_STAGES;
+    static_assert(MXT_RING / (64 * 256 + MXT_W_BYTES) >= 5 && MXT_RING / (MXT_BN * 256 + MXT_W_BYTES) >= 4, "as the converting warps' waits need");
     CUtensorMap map;
     int rc = make_map(&map, x, m, k, ldx, bn);
     if (rc) return rc;

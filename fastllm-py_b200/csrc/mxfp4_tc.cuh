@@ -48,6 +48,8 @@ __device__ __forceinline__ bool mxt_test(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+// (A wait names a phase by its parity, so whoever waits has to know that the phase before the one it means is over: because it waited
+// for that itself, or because something that it waited for came after it.)
 // A whole warp waits for a barrier's phase (limits as mbar_wait's; without a flag to the end).  All lanes ask, first without being put
 // to sleep: a wait by one lane and a shuffle of the outcome took 190 clocks even where the phase was complete, and these kernels
 // hand over from warp to warp several times a chunk (4096 x 8192 x 22016 in 4 bits: 384 us so, 313 this way; 64 tokens 22016 -> 8192:

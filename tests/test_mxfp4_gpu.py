@@ -569,3 +569,30 @@ def test_few_rows_with_a_large_matrix(m, n, k):
     # silu's slope is at most 1.1, its value at most |g|; its own evaluation in float is within 2^-18, twice
     unit = up * gate * torch.sigmoid(gate)
     assert bool(((units[0].double() - units[1].double()).abs() <= 1.1 * eg * up.abs() + gate.abs() * eu + eg * eu + 2.0 ** -17 * unit.abs()).all())
+
+
+@pytest.mark.parametrize("name, kernel, m, n, k", [("linear", 1, 64, 4096, 11008), ("linear", 1, 128, 4096, 5504), ("linear", 1, 96, 2304, 8192), ("linear", 2, 600, 4096, 5504),
+                                                   ("linear_gated", 1, 40, 2048, 8192), ("linear_gated", 2, 900, 2048, 5504), ("product", 1, 100, 4096, 11008),
+                                                   ("product", 2, 1024, 8192, 5504), ("product", 2, 4096, 8192, 11008)])
+def test_the_same_sums_every_time(name, kernel, m, n, k):
+    """Many launches of a large product, with the operands in and out of the L2: bits are the same, and no warp has given up.  (Copies
+    land in any order, and warps that share a ring's stages must not take one phase of a barrier for another.)"""
+    from fastllm_py_b200.native import gemm_tc, mxfp4
+
+    g = torch.Generator(device=DEV).manual_seed(k)
+    x = torch.randn(m, k, generator=g, device=DEV).to(torch.bfloat16)
+    gated = name == "linear_gated"
+    q = mxfp4.Matrix.of(torch.randn(2 * n if gated else n, k, generator=g, device=DEV) / k ** 0.5)
+    first = mxfp4.Matrix.of(x) if name == "product" else x
+    outs = [torch.full((m, n), -5.0, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    flush = torch.empty(160 << 20, dtype=torch.uint8, device=DEV)
+    call = getattr(mxfp4, name)
+    call(first, q, outs[0], kernel=kernel)
+    differ = torch.zeros((), dtype=torch.int64, device=DEV)
+    for i in range(150):
+        if i % 3 == 0:
+            flush.fill_(i)
+        call(first, q, outs[1], kernel=kernel)
+        differ += (outs[0] != outs[1]).sum()
+    assert int(gemm_tc.status_word(torch.device(DEV)).item()) == 0 and int(differ) == 0
+    assert not bool((outs[0] == -5.0).all())
