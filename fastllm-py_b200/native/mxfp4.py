@@ -65,18 +65,20 @@ class Matrix:
 
 
 _device = torch._C._cuda_getDevice               # the current device's index
+_raw_stream = ops._raw_stream
 
 
-def _stream_of(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor) -> int:
-    """The current stream of the device that all three are on, which has to be the current one."""
+def _stream_of(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor | None = None) -> int:
+    """The current stream of the device that all are on, which has to be the current one."""
     index = a.get_device()
-    if index < 0 or b.get_device() != index or c.get_device() != index:
-        if all(t.is_cuda for t in (a, b, c)):
-            raise KernelError(f"mxfp4: operands on {a.device}, {b.device} and {c.device}")
+    if index < 0 or b.get_device() != index or (c is not None and c.get_device() != index):
+        tensors = [t for t in (a, b, c) if t is not None]
+        if all(t.is_cuda for t in tensors):
+            raise KernelError(f"mxfp4: operands on {', '.join(str(t.device) for t in tensors)}")
         raise KernelError("the engine's kernels run on a CUDA device only; got a CPU tensor")
     if index != _device():
         raise KernelError(f"mxfp4: operands on {a.device}, the current device is cuda:{_device()}")
-    return ops._raw_stream(index)
+    return _raw_stream(index)
 
 
 def _rows_of(t: torch.Tensor, what: str) -> int:
@@ -144,8 +146,10 @@ def quantize(x: torch.Tensor, out: Matrix) -> None:
     pitch, data = _rows_of(x, "x"), out.data
     if x.shape != out.shape:
         raise KernelError(f"mxfp4.quantize: {tuple(x.shape)} into {out.shape}")
-    code, stream = ops.dtype_code(x), _stream_of(x, data, data)
-    ops._check(_fn(_QUANTIZE)(x.data_ptr(), code, pitch, data.data_ptr(), out.rows, out.k, stream), "mxfp4.quantize")
+    code, stream = ops.dtype_code(x), _stream_of(x, data)
+    rc = (_fns.get("fl_mx_quantize") or _fn(_QUANTIZE))(x.data_ptr(), code, pitch, data.data_ptr(), out.rows, out.k, stream)
+    if rc:
+        ops._check(rc, "mxfp4.quantize")
 
 
 def dequantize(q: Matrix, out: torch.Tensor) -> None:
@@ -153,8 +157,10 @@ def dequantize(q: Matrix, out: torch.Tensor) -> None:
     pitch, data = _rows_of(out, "out"), q.data
     if out.shape != q.shape:
         raise KernelError(f"mxfp4.dequantize: {q.shape} into {tuple(out.shape)}")
-    code, stream = ops.dtype_code(out), _stream_of(data, out, out)
-    ops._check(_fn(_DEQUANTIZE)(data.data_ptr(), out.data_ptr(), code, pitch, q.rows, q.k, stream), "mxfp4.dequantize")
+    code, stream = ops.dtype_code(out), _stream_of(data, out)
+    rc = (_fns.get("fl_mx_dequantize") or _fn(_DEQUANTIZE))(data.data_ptr(), out.data_ptr(), code, pitch, q.rows, q.k, stream)
+    if rc:
+        ops._check(rc, "mxfp4.dequantize")
 
 
 # The kernel for few rows takes up to 8 of them, and no more time than those on the tensor cores with matrices of up to 2^26 values
@@ -167,11 +173,12 @@ def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, consta
     m, k = x.shape
     if w.k != k or out.shape != (m, n) or (gated and w.rows % 2):
         raise KernelError(f"mxfp4.{name}: {tuple(x.shape)} x {w.shape}^T -> {tuple(out.shape)}")
-    if kernel not in (0, 1, 2):
+    if kernel and kernel not in (1, 2):
         raise KernelError(f"mxfp4.{name}: there is no kernel {kernel}")
     if m > MOST_ROWS:
         raise KernelError(f"mxfp4.{name}: {m} rows, at most {MOST_ROWS}")
-    if x.data_ptr() == out.data_ptr() and m > 0:
+    from_x, to = x.data_ptr(), out.data_ptr()
+    if from_x == to and m > 0:
         raise KernelError(f"mxfp4.{name}: out lies on x, which the kernels read while they write")
     act = -1 if activation is None else ops.activation_code(activation)
     code, stream = ops.dtype_code(out), _stream_of(x, data, out)
@@ -180,12 +187,12 @@ def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, consta
     status, sms = _known(x)
     rc = LESS
     if kernel or m > FEW_ROWS or w.rows * k > FEW_VALUES:
-        rc = _fn(_MANY)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
-                        constant_w, kernel, sms, status, stream)
+        rc = _fn(_MANY)(from_x, pitch, data.data_ptr(), to, code, out_pitch, m, n, k, gated, act, params[0], params[1], constant_w, kernel,
+                        sms, status, stream)
     if rc == LESS:
-        rc = _fn(_FEW)(x.data_ptr(), pitch, data.data_ptr(), out.data_ptr(), code, out_pitch, m, n, k, gated, act, params[0], params[1],
-                       constant_w, sms, stream)
-    ops._check(rc, name)
+        rc = _fn(_FEW)(from_x, pitch, data.data_ptr(), to, code, out_pitch, m, n, k, gated, act, params[0], params[1], constant_w, sms, stream)
+    if rc:
+        ops._check(rc, name)
 
 
 def linear(x: torch.Tensor, w: Matrix, out: torch.Tensor, activation: str | None = None, params=(0.0, 0.0),
