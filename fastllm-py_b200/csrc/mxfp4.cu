@@ -10,41 +10,39 @@
 // Bound by memory: k (2 or 4) bytes of a row in, 17 k / 32 out.  A warp takes 8 rows of a chunk, 4 lanes a row: a lane's 8
 // elements of each of the four blocks are loaded before the first is used.  The rows are two neighbours in each quarter of the
 // tile: their scales are 32 bytes side by side, as two rows' codes of a block are, so that every 32-byte sector is written whole.
-// Rows that do not begin on 16 bytes are read an element a lane instead, a block a warp.
+// Rows that do not begin on 16 bytes go through shared memory, an element a lane.  bfloat16 [2048, 11008] 10.4 us (5.5 TB/s), float
+// [5503, 4096] 17.2 (5.9 TB/s).
 __device__ __forceinline__ int mx_row_of(int unit, int i) { return 2 * unit + (i & 1) + 32 * (i >> 1); }      // unit 0 .. 15, i 0 .. 7
 
-template <typename T> __device__ __forceinline__ void mx_load8(const T* src, int n, float (&v)[8]) {           // zeros behind n
-    if (n >= 8) {
-        if (sizeof(T) == 2) {
-            const uint4 r = *reinterpret_cast<const uint4*>(src);
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+// 8 elements of a row from element c on, zeros behind k
+__device__ __forceinline__ uint4 mx_tokens8(const bf16* row, int c, int k) {
+    if (c + 8 <= k) return *reinterpret_cast<const uint4*>(row + c);
+    uint32_t v[4] = {};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-            }
-        } else {
-            const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        }
-        return;
-    }
+    for (int i = 0; i < 8; ++i)
+        if (c + i < k) v[i >> 1] |= (uint32_t)__bfloat16_as_ushort(row[c + i]) << (16 * (i & 1));
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+struct MxFloat8 {
+    float4 a, b;
+};
+__device__ __forceinline__ MxFloat8 mx_tokens8(const float* row, int c, int k) {
+    if (c + 8 <= k) return {reinterpret_cast<const float4*>(row + c)[0], reinterpret_cast<const float4*>(row + c)[1]};
+    float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32<T>(src[i]) : 0.0f;
+    for (int i = 0; i < 8; ++i) v[i] = c + i < k ? row[c + i] : 0.0f;
+    return {make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7])};
 }
-__device__ __forceinline__ uint32_t mx_one_code(float v) {
-    uint32_t code;
-    asm("{\n\t.reg .b8 q;\n\tcvt.rn.satfinite.e2m1x2.f32 q, %2, %1;\n\tcvt.u32.u8 %0, q;\n\t}" : "=r"(code) : "f"(v), "f"(0.0f));
-    return code;
-}
+// 8 rows of a chunk in a warp's shared memory, elements between rows so that 16 bytes of four lanes a row meet no bank twice
+template <typename T> constexpr int MX_PITCH = sizeof(T) == 2 ? 160 : 132;
 // a word of codes: a conversion makes a byte of two neighbouring nibbles
-__device__ __forceinline__ uint32_t mx_word(const float (&v)[8], float inv) {
+__device__ __forceinline__ uint32_t mx_word(const float (&v)[8]) {
     uint32_t word;
     asm("{\n\t.reg .b8 a, b, c, d;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
         : "=r"(word)
-        : "f"(v[0] * inv), "f"(v[2] * inv), "f"(v[4] * inv), "f"(v[6] * inv), "f"(v[1] * inv), "f"(v[3] * inv), "f"(v[5] * inv), "f"(v[7] * inv));
+        : "f"(v[0]), "f"(v[2]), "f"(v[4]), "f"(v[6]), "f"(v[1]), "f"(v[3]), "f"(v[5]), "f"(v[7]));
     return word;
 }
 // the scale byte of a block whose largest magnitude has these bits (magnitudes compare as integers do, a NaN above all)
@@ -53,6 +51,37 @@ __device__ __forceinline__ int mx_scale_byte(uint32_t top) {
     return e == 255 ? 255 : max(e - 2, 0);
 }
 __device__ __forceinline__ float mx_inverse(int s) { return __uint_as_float((uint32_t)(254 - min(s, 253)) << 23); }   // 2^(127 - s)
+// A lane's 8 elements of a block that 4 lanes have: their largest magnitude's scale byte, and the word of codes.  bfloat16 pairs are
+// compared as pairs of 16-bit integers, and multiplied as pairs: with a power of two that is exact but for what is far below a code.
+__device__ __forceinline__ uint32_t mx_codes(const uint4& x, int& s) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    s = mx_scale_byte(max(top, top << 16));
+    const uint32_t inv = (uint32_t)(254 - min(s, 253)) * 0x00800080u;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t y = mx_mul(w[i], inv);
+        v[2 * i] = __uint_as_float(y << 16);
+        v[2 * i + 1] = __uint_as_float(y & 0xFFFF0000u);
+    }
+    return mx_word(v);
+}
+__device__ __forceinline__ uint32_t mx_codes(const MxFloat8& x, int& s) {
+    float v[8] = {x.a.x, x.a.y, x.a.z, x.a.w, x.b.x, x.b.y, x.b.z, x.b.w};
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    s = mx_scale_byte(top);
+    const float inv = mx_inverse(s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= inv;
+    return mx_word(v);
+}
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ data, int m,
@@ -65,58 +94,36 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const T* __restrict__ 
     const long tile = blockIdx.x >> 4;
     const int u = blockIdx.x & 15;
     uint8_t* dst = data + (tile * chunks + chunk) * MX_CHUNK;
+    const int r = mx_row_of(u, lane >> 2);
+    const long row = tile * MX_ROWS + r;
+    decltype(mx_tokens8(x, 0, 0)) v[4];
     if constexpr (VEC) {
-        const int r = mx_row_of(u, lane >> 2);
-        const long row = tile * MX_ROWS + r;
-        float v[4][8];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int c = chunk * 128 + b * 32 + t * 8;
-            mx_load8(x + row * ld + c, row < m ? k - c : 0, v[b]);
-        }
-        uint32_t scales = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[b][i]) & 0x7FFFFFFFu);
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int s = mx_scale_byte(top);
-            scales |= (uint32_t)s << (8 * b);
-            const float inv = mx_inverse(s);
-            const uint32_t word = mx_word(v[b], inv);
-            *reinterpret_cast<uint32_t*>(dst + b * 2048 + r * 16 + t * 4) = s == 255 ? 0 : word;
-        }
-        if (t == 0) *reinterpret_cast<uint32_t*>(dst + mx_scale_at(r)) = scales;
+        for (int b = 0; b < 4; ++b) v[b] = mx_tokens8(x + row * ld, row < m ? chunk * 128 + b * 32 + t * 8 : k, k);
     } else {
-#pragma unroll 2
-        for (int i = 0; i < 8; ++i) {
-            const int r = mx_row_of(u, i);
-            const long row = tile * MX_ROWS + r;
-            float v[4];
+        __shared__ __align__(16) T staged[8][8 * MX_PITCH<T>];
+        T* mine = staged[threadIdx.x >> 5];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
+                const long from = tile * MX_ROWS + mx_row_of(u, i);
                 const int c = chunk * 128 + b * 32 + lane;
-                v[b] = row < m && c < k ? to_f32<T>(x[row * ld + c]) : 0.0f;
+                mine[i * MX_PITCH<T> + b * 32 + lane] = from < m && c < k ? x[from * ld + c] : from_f32<T>(0.0f);
             }
-            uint32_t scales = 0, mine = 0;
+        __syncwarp();
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const int s = mx_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7FFFFFFFu));
-                scales |= (uint32_t)s << (8 * b);
-                // the lane's code where its word has it, the eight lanes of a word added up
-                uint32_t word = s == 255 ? 0 : mx_one_code(v[b] * mx_inverse(s)) << (4 * ((lane & 1) * 4 + (lane >> 1 & 3)));
-                word |= __shfl_xor_sync(0xffffffffu, word, 1);
-                word |= __shfl_xor_sync(0xffffffffu, word, 2);
-                word |= __shfl_xor_sync(0xffffffffu, word, 4);
-                word = __shfl_sync(0xffffffffu, word, (lane & 3) * 8);
-                if (lane >> 2 == b) mine = word;                          // lanes 4 b .. 4 b + 3 hold the block's words
-            }
-            if (lane < 16) *reinterpret_cast<uint32_t*>(dst + (lane >> 2) * 2048 + r * 16 + (lane & 3) * 4) = mine;
-            else if (lane == 16) *reinterpret_cast<uint32_t*>(dst + mx_scale_at(r)) = scales;
-        }
+        for (int b = 0; b < 4; ++b) v[b] = mx_tokens8(mine + (lane >> 2) * MX_PITCH<T>, b * 32 + t * 8, 128);
     }
+    uint32_t scales = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        int s;
+        const uint32_t word = mx_codes(v[b], s);
+        scales |= (uint32_t)s << (8 * b);
+        *reinterpret_cast<uint32_t*>(dst + b * 2048 + r * 16 + t * 4) = s == 255 ? 0 : word;
+    }
+    if (t == 0) *reinterpret_cast<uint32_t*>(dst + mx_scale_at(r)) = scales;
 }
 
 FL_API int fl_mx_quantize(const void* x, int code, long ld, void* data, int m, int k, cudaStream_t stream) {
@@ -131,8 +138,8 @@ FL_API int fl_mx_quantize(const void* x, int code, long ld, void* data, int m, i
     return (int)cudaErrorInvalidValue;
 }
 
-// Back: the same division of the work; rows that do not begin on 16 bytes are written an element a lane, the words of a row
-// handed round by shuffles.
+// Back: the same division of the work, and the same way for rows that do not begin on 16 bytes.  [2048, 11008] to bfloat16 11.4 us (5.0
+// TB/s), [5503, 4096] to float 18.0 (5.7 TB/s).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __restrict__ data, T* __restrict__ out, long ld, int m,
                                                             int k, int chunks) {
@@ -145,54 +152,60 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __res
     const int u = blockIdx.x & 15, r = mx_row_of(u, lane >> 2);
     const uint8_t* src = data + (tile * chunks + chunk) * MX_CHUNK;
     const uint32_t scales = *reinterpret_cast<const uint32_t*>(src + mx_scale_at(r));
-    uint32_t word[4];
+    // 16 bytes of output a lane and store, side by side: 8 bfloat16 of a word, or 4 floats of each of two words
+    constexpr int WORDS = sizeof(T) / 2, N = 16 / sizeof(T);
+    uint32_t word[4][WORDS];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) word[b] = *reinterpret_cast<const uint32_t*>(src + b * 2048 + r * 16 + t * 4);
-    if constexpr (VEC) {
-        const long row = tile * MX_ROWS + r;
-        const bool large = __any_sync(0xffffffffu, (scales & 0x80808080u & ((scales & 0x7F7F7F7Fu) + 0x7F7F7F7Fu)) != 0);
-        if (row >= m) return;
+    for (int b = 0; b < 4; ++b)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int c = chunk * 128 + b * 32 + t * 8;
-            const uint32_t s = scales >> (8 * b) & 255u;
+        for (int j = 0; j < WORDS; ++j)
+            word[b][j] = *reinterpret_cast<const uint32_t*>(src + b * 2048 + r * 16 + (WORDS == 1 ? t : 2 * j + (t >> 1)) * 4);
+    __shared__ __align__(16) T staged[VEC ? 1 : 8][VEC ? 8 : 8 * MX_PITCH<T>];
+    T* mine = staged[VEC ? 0 : threadIdx.x >> 5];
+    const long row = tile * MX_ROWS + r;
+    const bool large = __any_sync(0xffffffffu, (scales & 0x80808080u & ((scales & 0x7F7F7F7Fu) + 0x7F7F7F7Fu)) != 0);
+    if (VEC && row >= m) return;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const uint32_t s = scales >> (8 * b) & 255u;
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) {
             uint32_t w[4];                                            // in bfloat16, which has all that float has of these values
-            mx_pairs(word[b], large ? mx_factor_large(s) : mx_factor(s), w);
+            mx_pairs(WORDS == 1 ? word[b][j] : word[b][j] >> (8 * (t & 1)), large ? mx_factor_large(s) : mx_factor(s), w);
             if (large)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = mx_mul(w[i], mx_factor_rest(s));
-            __align__(16) T v[8];
+            __align__(16) T v[N];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < N / 2; ++i) {
                 if (sizeof(T) == 2) {
                     reinterpret_cast<uint32_t*>(v)[i] = w[i];
                 } else {
-                    reinterpret_cast<uint32_t*>(v)[(sizeof(T) / 2) * i] = w[i] << 16;
-                    reinterpret_cast<uint32_t*>(v)[(sizeof(T) / 2) * i + sizeof(T) / 4] = w[i] & 0xFFFF0000u;
+                    reinterpret_cast<uint32_t*>(v)[2 * i] = w[i] << 16;
+                    reinterpret_cast<uint32_t*>(v)[2 * i + 1] = w[i] & 0xFFFF0000u;
                 }
             }
-            T* dst = out + row * ld + c;
-            if (c + 8 <= k) {
-#pragma unroll
-                for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(v)[i];
+            const int at = b * 32 + (j * 4 + t) * N, c = chunk * 128 + at;
+            if (!VEC) {
+                *reinterpret_cast<uint4*>(mine + (lane >> 2) * MX_PITCH<T> + at) = *reinterpret_cast<const uint4*>(v);
+            } else if (c + N <= k) {
+                *reinterpret_cast<uint4*>(out + row * ld + c) = *reinterpret_cast<const uint4*>(v);
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (c + i < k) dst[i] = v[i];
+                for (int i = 0; i < N; ++i)
+                    if (c + i < k) out[row * ld + c + i] = v[i];
             }
         }
-    } else {
-        const int place = 4 * ((lane & 1) * 4 + (lane >> 1 & 3));         // of element lane % 8 in its word
-#pragma unroll 2
-        for (int i = 0; i < 8; ++i) {
-            const long row = tile * MX_ROWS + mx_row_of(u, i);
-            const uint32_t sc = __shfl_sync(0xffffffffu, scales, 4 * i);
+    }
+    if (VEC) return;
+    __syncwarp();
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const uint32_t code = __shfl_sync(0xffffffffu, word[b], 4 * i + (lane >> 3)) >> place;
-                const int c = chunk * 128 + b * 32 + lane;
-                if (row < m && c < k) out[row * ld + c] = from_f32<T>(mx_value(code, 0) * mx_scale((int)(sc >> (8 * b)) & 255));
-            }
+    for (int i = 0; i < 8; ++i) {
+        const long to = tile * MX_ROWS + mx_row_of(u, i);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int c = chunk * 128 + b * 32 + lane;
+            if (to < m && c < k) out[to * ld + c] = mine[i * MX_PITCH<T> + b * 32 + lane];
         }
     }
 }
@@ -224,16 +237,6 @@ __device__ __forceinline__ void mx_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// 8 elements of a token from element c on, zeros behind k
-__device__ __forceinline__ uint4 mx_tokens8(const bf16* row, int c, int k) {
-    if (c + 8 <= k) return *reinterpret_cast<const uint4*>(row + c);
-    uint32_t v[4] = {};
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (c + i < k) v[i >> 1] |= (uint32_t)__bfloat16_as_ushort(row[c + i]) << (16 * (i & 1));
-    return make_uint4(v[0], v[1], v[2], v[3]);
-}
-
 template <typename TO, int WARPS, bool GATED, int LB>
 __global__ void __launch_bounds__(WARPS * 32, LB / WARPS)
 mx_few_kernel(const bf16* __restrict__ x, long ldx, const uint8_t* __restrict__ w, TO* __restrict__ out, long ldo, int m, int n, int k,
