@@ -412,7 +412,7 @@ static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ld
     int bn = 0, ranks = 1;
     long time = 0, rounds;
     for (int most = MXT_BN; most >= 64; most -= 32) {
-        const int even = (m + most - 1) / most, tokens = ((m + even - 1) / even + 15) / 16 * 16;
+        const int even = (m + most - 1) / most, tokens = (int)(((long)m + even - 1) / even + 15) / 16 * 16;
         if (tokens == bn) continue;
         long t;
         const MxtTimes times = {300, tokens <= 64 ? 560 + tokens * 3 / 2 : 580 + tokens * 2, 3800, 24, 22};
