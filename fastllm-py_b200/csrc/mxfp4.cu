@@ -138,8 +138,9 @@ FL_API int fl_mx_quantize(const void* x, int code, long ld, void* data, int m, i
     return (int)cudaErrorInvalidValue;
 }
 
-// Back: the same division of the work, and the same way for rows that do not begin on 16 bytes.  [2048, 11008] to bfloat16 11.4 us (5.0
-// TB/s), [5503, 4096] to float 18.0 (5.7 TB/s).
+// Back: the same division of the work; rows that do not begin on 16 bytes are written an element a lane, the words of a row handed round
+// by shuffles.  (Through shared memory they took as long, and twice that after a kernel without any: the SMs' memory is then divided
+// anew.)  [2048, 11008] to bfloat16 11.4 us (5.0 TB/s), [5503, 4096] to float 18.0 (5.7 TB/s), [5503, 4097] 23.3.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __restrict__ data, T* __restrict__ out, long ld, int m,
                                                             int k, int chunks) {
@@ -153,59 +154,60 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __res
     const uint8_t* src = data + (tile * chunks + chunk) * MX_CHUNK;
     const uint32_t scales = *reinterpret_cast<const uint32_t*>(src + mx_scale_at(r));
     // 16 bytes of output a lane and store, side by side: 8 bfloat16 of a word, or 4 floats of each of two words
-    constexpr int WORDS = sizeof(T) / 2, N = 16 / sizeof(T);
+    constexpr int WORDS = VEC ? sizeof(T) / 2 : 1, N = 16 / sizeof(T);
     uint32_t word[4][WORDS];
 #pragma unroll
     for (int b = 0; b < 4; ++b)
 #pragma unroll
         for (int j = 0; j < WORDS; ++j)
             word[b][j] = *reinterpret_cast<const uint32_t*>(src + b * 2048 + r * 16 + (WORDS == 1 ? t : 2 * j + (t >> 1)) * 4);
-    __shared__ __align__(16) T staged[VEC ? 1 : 8][VEC ? 8 : 8 * MX_PITCH<T>];
-    T* mine = staged[VEC ? 0 : threadIdx.x >> 5];
-    const long row = tile * MX_ROWS + r;
-    const bool large = __any_sync(0xffffffffu, (scales & 0x80808080u & ((scales & 0x7F7F7F7Fu) + 0x7F7F7F7Fu)) != 0);
-    if (VEC && row >= m) return;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        const uint32_t s = scales >> (8 * b) & 255u;
-#pragma unroll
-        for (int j = 0; j < WORDS; ++j) {
-            uint32_t w[4];                                            // in bfloat16, which has all that float has of these values
-            mx_pairs(WORDS == 1 ? word[b][j] : word[b][j] >> (8 * (t & 1)), large ? mx_factor_large(s) : mx_factor(s), w);
-            if (large)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = mx_mul(w[i], mx_factor_rest(s));
-            __align__(16) T v[N];
-#pragma unroll
-            for (int i = 0; i < N / 2; ++i) {
-                if (sizeof(T) == 2) {
-                    reinterpret_cast<uint32_t*>(v)[i] = w[i];
-                } else {
-                    reinterpret_cast<uint32_t*>(v)[2 * i] = w[i] << 16;
-                    reinterpret_cast<uint32_t*>(v)[2 * i + 1] = w[i] & 0xFFFF0000u;
-                }
-            }
-            const int at = b * 32 + (j * 4 + t) * N, c = chunk * 128 + at;
-            if (!VEC) {
-                *reinterpret_cast<uint4*>(mine + (lane >> 2) * MX_PITCH<T> + at) = *reinterpret_cast<const uint4*>(v);
-            } else if (c + N <= k) {
-                *reinterpret_cast<uint4*>(out + row * ld + c) = *reinterpret_cast<const uint4*>(v);
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (c + i < k) out[row * ld + c + i] = v[i];
-            }
-        }
-    }
-    if (VEC) return;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const long to = tile * MX_ROWS + mx_row_of(u, i);
+    if constexpr (VEC) {
+        const long row = tile * MX_ROWS + r;
+        const bool large = __any_sync(0xffffffffu, (scales & 0x80808080u & ((scales & 0x7F7F7F7Fu) + 0x7F7F7F7Fu)) != 0);
+        if (row >= m) return;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            const int c = chunk * 128 + b * 32 + lane;
-            if (to < m && c < k) out[to * ld + c] = mine[i * MX_PITCH<T> + b * 32 + lane];
+            const uint32_t s = scales >> (8 * b) & 255u;
+#pragma unroll
+            for (int j = 0; j < WORDS; ++j) {
+                uint32_t w[4];                                        // in bfloat16, which has all that float has of these values
+                mx_pairs(WORDS == 1 ? word[b][j] : word[b][j] >> (8 * (t & 1)), large ? mx_factor_large(s) : mx_factor(s), w);
+                if (large)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = mx_mul(w[i], mx_factor_rest(s));
+                __align__(16) T v[N];
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i) {
+                    if (sizeof(T) == 2) {
+                        reinterpret_cast<uint32_t*>(v)[i] = w[i];
+                    } else {
+                        reinterpret_cast<uint32_t*>(v)[2 * i] = w[i] << 16;
+                        reinterpret_cast<uint32_t*>(v)[2 * i + 1] = w[i] & 0xFFFF0000u;
+                    }
+                }
+                const int c = chunk * 128 + b * 32 + (j * 4 + t) * N;
+                T* dst = out + row * ld + c;
+                if (c + N <= k) {
+                    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        if (c + i < k) dst[i] = v[i];
+                }
+            }
+        }
+    } else {
+        const int place = 4 * ((lane & 1) * 4 + (lane >> 1 & 3));         // of element lane % 8 in its word
+#pragma unroll 2
+        for (int i = 0; i < 8; ++i) {
+            const long row = tile * MX_ROWS + mx_row_of(u, i);
+            const uint32_t sc = __shfl_sync(0xffffffffu, scales, 4 * i);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint32_t code = __shfl_sync(0xffffffffu, word[b][0], 4 * i + (lane >> 3)) >> place;
+                const int c = chunk * 128 + b * 32 + lane;
+                if (row < m && c < k) out[row * ld + c] = from_f32<T>(mx_value(code) * mx_scale((int)(sc >> (8 * b)) & 255));
+            }
         }
     }
 }

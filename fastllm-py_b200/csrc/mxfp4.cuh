@@ -25,6 +25,14 @@ static inline int mx_device() {
 }
 
 __device__ __forceinline__ long mx_scale_at(int r) { return MX_CODES + (r & 31) * 16 + (r >> 5) * 4; }
+__device__ __forceinline__ float mx_scale(int s) {          // 2^(s - 127)
+    return s == 255 ? CUDART_NAN_F : (s == 0 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t)s << 23));
+}
+// A code in float, without its block's scale: sign and magnitude put where a float of exponent 2^-126 has them, a subnormal for the
+// magnitudes 0 and 0.5, and multiplied by 2^126, exactly.
+__device__ __forceinline__ float mx_value(uint32_t code) {
+    return __uint_as_float(((code & 8u) << 28) | ((code & 7u) << 22)) * 8.507059173023462e37f;
+}
 __device__ __forceinline__ uint32_t mx_mul(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
