@@ -7,14 +7,15 @@
 // next tile's MMAs run while the epilogue's warps empty the last one's accumulator, 32 tokens a round through shared memory.  (With 256
 // tokens there is room for one accumulator.)  Persistent: a pair walks over its tiles.
 //
-// Warps 0-15 convert, four of them half of a chunk of 128 along K, a thread one row; warps 16-19 are the epilogue; warps 20 and 22 send
-// for the tokens and the codes, warp 21 of the pair's even CTA (the leader) issues the MMAs.
+// Warps 0-15 convert, four of them half of a chunk of 128 along K, a thread one row; warps 16-23 are the epilogue, in two
+// groups; warps 24 and 26 send for the tokens and the codes, warp 25 of the pair's even CTA (the leader) issues the MMAs.
 //
 // What bounds it: a chunk's way through wait, conversion, store to tensor memory and arrival, 1850 clocks of a warp for every other one;
 // MMAs alone take 660 a chunk with 128 tokens, 770 with 192.  The issuing warp has few instructions to spare: with a barrier for each
 // half of a chunk and one for its tokens a chunk took 1070 clocks, however small; it now waits for one, at which a converting
-// warp arrives when it has seen the tokens too.  256 tokens 22016 -> 8192: 100 us, 86 so; 2048 tokens 11008 -> 4096: 172 and 146 (1.26
-// PFLOP/s), 4096 -> the gated 2 x 11008 270 (1.37 PFLOP/s, what the power limit leaves of the rate).
+// warp arrives when it has seen the tokens too.  256 tokens 22016 -> 8192: 100 us, 86 so (81 now); 2048 tokens 11008 ->
+// 4096 141 (1.31 PFLOP/s), 4096 -> the gated 2 x 11008 249 (1.48 PFLOP/s; launched on end 300, what the power limit leaves).  With one
+// group of epilogue warps that 271, 517 tokens 2048 -> 5503 21.2 in place of 18.7: a tile's sums take about 5 us to leave.
 #pragma once
 
 #include "mxfp4_tc.cuh"
@@ -28,7 +29,7 @@
 #define MXP_W_STAGE (MX_CODES + 1536)                    // 128 rows' codes, scales of up to 3 packed tiles
 #define MXP_ROUND (32 * 128 * 4)                         // 32 tokens' sums
 #define MXP_SMEM (MXP_X_RING + MXP_W_STAGES * MXP_W_STAGE + 2 * MXP_ROUND + 1024 + 512)
-#define MXP_THREADS (23 * 32)
+#define MXP_THREADS (27 * 32)
 
 // ------------------------------------------------------------------ what a pair needs
 // (What the leader's MMA reads of the other CTA is in tensor memory, which tcgen05's own fences order.  An arrival with a release at
@@ -61,48 +62,52 @@ __device__ __forceinline__ void mxp_copy_codes(void* dst, const CUtensorMap* map
         "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(row * 2), "r"(0), "r"(chunk)
         : "memory");
 }
-// A barrier of the four epilogue warps, and whether any thread came with `flag`: they leave together or not at all.
-__device__ __forceinline__ bool mxp_vote(bool flag) {
+// A barrier of the epilogue's group `group`, and whether any of its threads came with `flag`: they leave together or not at all.
+__device__ __forceinline__ bool mxp_vote(bool flag, int group) {
     uint32_t any;
     __syncwarp();
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.u32 p, %1, 0;\n\t"
-        "bar.red.or.pred q, 2, 128, p;\n\t"
+        "bar.red.or.pred q, %2, 128, p;\n\t"
         "selp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(any)
-        : "r"((uint32_t)flag)
+        : "r"((uint32_t)flag), "r"(2 + group)
         : "memory");
     return any != 0;
 }
 
-// The accumulator of a tile, emptied by the epilogue's four warps in rounds of 32 tokens: this CTA's 128 rows, FEAT features of them on
-// their way out.  `rounds`: how many this CTA has done, which picks the half of `staged`.  False: given up.
+// The accumulator of a tile, emptied by a group of the epilogue's warps, which takes every other 32 tokens: this CTA's 128 rows, FEAT
+// features of them on their way out.  `staged`: the group's.  False: given up.
 template <typename TO, bool GATED>
-__device__ __forceinline__ bool mxp_epilogue(uint32_t tmem_acc, float* staged, uint32_t& rounds, int tokens, TO* __restrict__ out, long ldo, int n,
+__device__ __forceinline__ bool mxp_epilogue(uint32_t tmem_acc, float* staged, int group, int tokens, TO* __restrict__ out, long ldo, int n,
                                              const FlGate act, volatile int* abort_flag, uint64_t* acc_empty) {
     constexpr int FEAT = GATED ? 64 : 128, V = GATED ? 2 : 4;
     const int quarter = mxt_warp() & 3, r = quarter * 32 + (threadIdx.x & 31);
     const bool vec = (((uintptr_t)out | (uintptr_t)(ldo * (long)sizeof(TO))) & (V * sizeof(TO) - 1)) == 0 && (n & (V - 1)) == 0;
-    for (int t = 0; t < tokens; t += 32, ++rounds) {
-        float* half = staged + (rounds & 1) * (32 * 128);
+    bool read = false;                                    // the group's part of the accumulator has been
+    for (int t = 32 * group; t < tokens; t += 64) {
         uint32_t v[32];
         tmem_ld16(tmem_acc + ((uint32_t)(quarter * 32) << 16) + (uint32_t)t, v);
         tmem_ld16(tmem_acc + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(t + 16), v + 16);
         tmem_ld_wait();
-        if (t + 32 >= tokens) {                           // the accumulator has been read
+        if (t + 64 >= tokens) {
             tc_fence_before();
             __syncwarp();
             if ((threadIdx.x & 31) == 0) mbar_arrive_leader(acc_empty);
+            read = true;
         }
+        if (mxp_vote(false, group)) return false;         // the last round's rows have left
 #pragma unroll
-        for (int j = 0; j < 32; ++j) half[j * 128 + r] = __uint_as_float(v[j]);
-        if (mxp_vote(*abort_flag != 0)) return false;     // (a half's readers have all come here before it is written again)
+        for (int j = 0; j < 32; ++j) staged[j * 128 + r] = __uint_as_float(v[j]);
+        if (mxp_vote(*abort_flag != 0, group)) return false;
         if (n <= 0) continue;
         const int last = min(32, tokens - t);
-        if (vec) mxt_rows<TO, GATED, FEAT, 128, V, 4>(MxtSums{half, half, 1, 0, 0, 0}, quarter, last, out + (long)t * ldo, ldo, n, act);
-        else mxt_rows<TO, GATED, FEAT, 128, 1, 4>(MxtSums{half, half, 1, 0, 0, 0}, quarter, last, out + (long)t * ldo, ldo, n, act);
+        if (vec) mxt_rows<TO, GATED, FEAT, 128, V, 4>(MxtSums{staged, staged, 1, 0, 0, 0}, quarter, last, out + (long)t * ldo, ldo, n, act);
+        else mxt_rows<TO, GATED, FEAT, 128, 1, 4>(MxtSums{staged, staged, 1, 0, 0, 0}, quarter, last, out + (long)t * ldo, ldo, n, act);
     }
+    __syncwarp();
+    if (!read && (threadIdx.x & 31) == 0) mbar_arrive_leader(acc_empty);
     return true;
 }
 
@@ -146,13 +151,13 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], 8);
+            mbar_init(&acc_empty[b], 16);                    // eight warps in each CTA
         }
         *abort_flag = (*(volatile int*)status != 0) ? 1 : 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 21) {
+    if (warp == 25) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
@@ -224,9 +229,9 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
                 if (++s == MXP_W_STAGES) { s = 0; ph ^= 1u; }
             }
         }
-    } else if (warp < 20) {
+    } else if (warp < 24) {
         // ---- epilogue
-        uint32_t rounds = 0;
+        const int group = warp >> 2 & 1;
         int i = 0;
         for (int tile = pair; tile < tiles; tile += pairs, ++i) {
             const int b = i & 1;
@@ -234,14 +239,14 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
                 if (lane == 0) mxt_give_up(abort_flag, status);
                 ok = false;
             }
-            if (mxp_vote(!ok)) break;
+            if (mxp_vote(!ok, group)) break;
             tc_fence_after();
             const int t0 = tile % token_tiles * bn, f0 = tile / token_tiles * (2 * FEAT) + rank * FEAT;
-            if (!mxp_epilogue<TO, GATED>(tmem + (uint32_t)(b * 192), staged, rounds, min(bn, m - t0), out + (long)t0 * ldo + f0, ldo, n - f0, act,
-                                         abort_flag, &acc_empty[b]))
+            if (!mxp_epilogue<TO, GATED>(tmem + (uint32_t)(b * 192), staged + group * (MXP_ROUND / 4), group, min(bn, m - t0),
+                                         out + (long)t0 * ldo + f0, ldo, n - f0, act, abort_flag, &acc_empty[b]))
                 break;
         }
-    } else if (warp == 20) {
+    } else if (warp == 24) {
         // ---- this CTA's half of the tokens, signalled to the leader
         int s = 0;
         uint32_t ph = 0;
@@ -264,7 +269,7 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
                 if (++s == x_stages) { s = 0; ph ^= 1u; }
             }
         }
-    } else if (warp == 22) {
+    } else if (warp == 26) {
         // ---- this CTA's rows of W
         const long tile_bytes = (long)chunks * MX_CHUNK;
         int s = 0;
@@ -351,11 +356,11 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 20 && lane == 0 && *abort_flag) tma_drain(x_full, rank == 0 ? x_stages : 0, issued);
-    if (warp == 22 && lane == 0 && *abort_flag) tma_drain(w_full, MXP_W_STAGES, issued);
+    if (warp == 24 && lane == 0 && *abort_flag) tma_drain(x_full, rank == 0 ? x_stages : 0, issued);
+    if (warp == 26 && lane == 0 && *abort_flag) tma_drain(w_full, MXP_W_STAGES, issued);
     __syncthreads();
     cluster_sync_all();                                      // neither leaves while the other's MMAs or copies may reach it
-    if (warp == 21) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if (warp == 25) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 // What a chunk takes, in ns: the conversion and its hand-overs up to 160 tokens, with 192 the MMAs (K 22016: 86 us with 64 and with 128
@@ -441,21 +446,6 @@ __device__ __forceinline__ void mxqp_umma(uint32_t tmem_d, uint64_t adesc, uint6
 __device__ __forceinline__ void mxqp_st4(uint32_t taddr, const uint4 v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-// A barrier of the epilogue's group `group`, and whether any of its threads came with `flag`.
-__device__ __forceinline__ bool mxqp_vote(bool flag, int group) {
-    uint32_t any;
-    __syncwarp();
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.u32 p, %1, 0;\n\t"
-        "bar.red.or.pred q, %2, 128, p;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(any)
-        : "r"((uint32_t)flag), "r"(2 + group)
-        : "memory");
-    return any != 0;
-}
-
 // tiles: row pairs x token pairs (two packed tiles each).
 template <typename TO>
 __global__ void __launch_bounds__(MXQP_THREADS, 1)
@@ -543,7 +533,7 @@ mxqp_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __
                 if (lane == 0) mxt_give_up(abort_flag, status);
                 ok = false;
             }
-            if (mxqp_vote(!ok, group)) break;
+            if (mxp_vote(!ok, group)) break;
             tc_fence_after();
             const int t0 = tile % token_pairs * 256, f0 = tile / token_pairs * 256 + rank * 128, tokens = min(256, m - t0), left = n - f0;
             TO* dst = out + (long)t0 * ldo + f0;
@@ -560,10 +550,10 @@ mxqp_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __
                     if (lane == 0) mbar_arrive_leader(acc_empty);
                 }
                 if (t >= tokens || left <= 0) continue;          // (the same in the whole group)
-                if (mxqp_vote(false, group)) going = false;      // the last round's rows have left
+                if (mxp_vote(false, group)) going = false;      // the last round's rows have left
 #pragma unroll
                 for (int j = 0; j < 32; ++j) mine[j * 128 + r] = __uint_as_float(v[j]);
-                if (mxqp_vote(*abort_flag != 0, group)) going = false;
+                if (mxp_vote(*abort_flag != 0, group)) going = false;
                 if (!going) break;
                 const int last = min(32, tokens - t);
                 if (vec) mxt_rows<TO, false, 128, 128, 4, 4>(MxtSums{mine, mine, 1, 0, 0, 0}, quarter, last, dst + (long)t * ldo, ldo, left, FlGate{FL_ACT_NONE, 0.0f, 0.0f});
