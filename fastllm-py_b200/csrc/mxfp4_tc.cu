@@ -423,11 +423,11 @@ static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ld
     // The kernel for few rows takes 0.19 ns for 1000 elements of W: one token 22016 -> 8192: 35.7 us, 29.7 here; 4096 -> the gated 2 x
     // 11008: 16.5, 22 here.
     if (which == 0 && m <= MXT_FEW_ROWS && 1500 + (long)n * (GATED ? 2 : 1) * k / 1000 * 19 / 100 < time) return MXT_FEW;
-    // On pairs of CTAs: the chunks, and the last tile's epilogue.  517 tokens 4096 -> 4096: 24.4 us, 27 here; 192 tokens 4096 -> 12288: 32
-    // and 27; 2048 tokens 4096 -> 12288: 141 and 224.
+    // On pairs of CTAs: the way in and out, which no neighbour in the stream overlaps, the chunks, and the last tile's epilogue.  517 tokens
+    // 4096 -> 4096: 24.4 us, 26.4 here; 192 tokens 4096 -> 12288: 25.4 and 26.9; 2048 tokens 4096 -> 12288: 141 and 224.
     const int pair_bn = mxp_tokens(m, row_tiles, num_sms / 2, &rounds);
     const bool fits = tokens_y <= 65535 && row_tiles <= 65535;       // a grid's y and z; pairs walk over any number of tiles
-    if (which == 2 || (which == 0 && (!fits || 5000 + mxp_chunk(pair_bn) * rounds * chunks + 30 * pair_bn < time)))
+    if (which == 2 || (which == 0 && (!fits || 6000 + mxp_chunk(pair_bn) * rounds * chunks + 30 * pair_bn < time)))
         return mxp_launch<TO, GATED>(x, ldx, w, out, ldo, m, n, k, act, num_sms, status, stream);
     if (!fits) return (int)cudaErrorInvalidValue;
     const int per_rank = (chunks + ranks - 1) / ranks;
