@@ -55,6 +55,37 @@ __device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, int acc
         ok = false;
     }
     __syncwarp();
+    // 16 bytes or 8 of a lane's features at a time, where rows are aligned
+    const bool vec = (((uintptr_t)(out + f0) | (uintptr_t)(ldo * (long)sizeof(TO))) & (V * sizeof(TO) - 1)) == 0 && (n & (V - 1)) == 0;
+    if (ranks == 1 && (GATED || !vec)) {
+        // Nothing to add up: a warp's 32 features side by side, a token a store.  Through shared memory as below 128 tokens, 4096 -> the
+        // gated 2 x 11008, took 30.7 us, and 28.8 so; 517 tokens 2048 -> 5503 19.6 and 18.4; but with features by fours 256 x 1536 x
+        // 1024 in 4 bits takes 7.2 that way, and 7.7 so.
+        if (warp < MXT_WARPS && ok && !*abort_flag) {
+            tc_fence_after();
+            constexpr int TILES = GATED ? 1 : 2;                      // that warps share
+            const int tile = GATED ? 0 : warp >> 2 & 1, f = f0 + tile * 128 + (threadIdx.x & 127);
+            const uint32_t src = tmem_d + (uint32_t)(tile * acc_cols) + ((uint32_t)((warp & 3) * 32) << 16);
+            for (int c = warp / (4 * TILES) * 16; c < rows; c += MXT_WARPS / (4 * TILES) * 16) {
+                uint32_t v[16], w[16];
+                tmem_ld16(src + (uint32_t)c, v);
+                if (GATED) tmem_ld16(src + (uint32_t)(acc_cols + c), w);
+                tmem_ld_wait();
+                float g[16], u[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) g[j] = __uint_as_float(v[j]), u[j] = GATED ? __uint_as_float(w[j]) : 1.0f;
+                if (act.act != FL_ACT_NONE) gated_act(g, u, act);
+                TO* dst = out + (long)c * ldo + f;
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (c + j < rows && f < n) dst[(long)j * ldo] = from_f32<TO>(g[j]);
+            }
+        }
+        __syncwarp();
+        tc_fence_before();
+        __syncthreads();
+        return;
+    }
     if (ranks > 1) mxt_cluster_arrive();
     if (warp < MXT_WARPS && ok) {
         tc_fence_after();
@@ -92,7 +123,7 @@ __device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, int acc
         const MxtSums from = {sums, parts, ranks, rank, first, (last - first) * MXT_PITCH};
         out += f0;
         // a warp takes a token: V features a lane and 32 V a step, or single ones side by side where rows are not aligned
-        if ((((uintptr_t)out | (uintptr_t)(ldo * (long)sizeof(TO))) & (V * sizeof(TO) - 1)) == 0 && (n & (V - 1)) == 0)
+        if (vec)
             mxt_rows<TO, GATED, FEAT, MXT_PITCH, V, MXT_WARPS>(from, first + warp, last, out, ldo, n - f0, act);
         else
             mxt_rows<TO, GATED, FEAT, MXT_PITCH, 1, MXT_WARPS>(from, first + warp, last, out, ldo, n - f0, act);
@@ -462,7 +493,7 @@ FL_API int fl_mxt_product(const void* x, long ldx, const void* w, void* out, int
 // side in the packed form, of two tiles of W's rows and of one of A's: three copies.
 //
 // What bounds it: few rows the bytes (64 x 8192 x 22016 21.2 us, 4.5 TB/s), small products the way in and out (16 x 256 x 128 takes
-// 2.8 us, 261 x 1537 x 1000 8.4, 4.5 of them after its last stage).  A stage takes 0.56 us, its MMAs 0.27: the rest is the
+// 2.8 us, 261 x 1537 x 1000 7.8, about 4 of them after its last stage).  A stage takes 0.56 us, its MMAs 0.27: the rest is the
 // issuing warp's, which has three instructions for the scales of each chunk.  (Stages of one chunk: 0.33 us, and 128 x 4096 x 11008
 // 15.5 us in place of 14.1.)
 #define MXQ_STAGE (6 * MX_CHUNK)
