@@ -180,7 +180,10 @@ def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, consta
     from_x, to = x.data_ptr(), out.data_ptr()
     if from_x == to and m > 0:
         raise KernelError(f"mxfp4.{name}: out lies on x, which the kernels read while they write")
-    act = -1 if activation is None else ops.activation_code(activation)
+    if activation is None and not gated:
+        act = -1
+    else:
+        act = ops.activation_code(activation)                    # (a gated product without a unit would leave its up half out)
     code, stream = ops.dtype_code(out), _stream_of(x, data, out)
     if m == 0:
         return
