@@ -317,7 +317,8 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
         issued = mxt_produce(map_x, w, ring, full_bar, empty_bar, stages, stage_bytes, bn, t0, n, chunks, f0, row1, tiles, c_begin, c_end, constant_w,
                              ok, abort_flag, status);
     } else {
-        // ---- MMA issuer
+        // ---- MMA issuer.  (No chunk comes before the preceding kernel is over, and the limit of a wait is not for that kernel's time.)
+        pdl_wait();
         const uint32_t idesc = instr_desc_bf16(128, bn), ring_at = smem_u32(ring);
         int s = 0;
         uint32_t place = 0, pa = 0;

@@ -1,9 +1,14 @@
 """Calls of the 4-bit operators that are refused on the host, and rules of their kernels that are checked on the sources."""
+import re
+from pathlib import Path
+
 import pytest
 import torch
 
 from fastllm_py_b200.native import mxfp4
 from fastllm_py_b200.native.ops import KernelError
+
+CSRC = Path(__file__).resolve().parent.parent / "fastllm-py_b200" / "csrc"
 
 
 def bf(*shape):
@@ -20,3 +25,28 @@ def test_a_gated_product_has_a_unit(kernel):
         mxfp4.linear_gated(bf(0, 96), w, bf(0, 32), None)
     with pytest.raises(KernelError, match="CUDA device only"):
         mxfp4.linear(bf(5, 96), w, bf(5, 64), activation=None, kernel=kernel)
+
+
+def body_of(file, name):
+    """From a function's name to the brace that closes it."""
+    text = (CSRC / file).read_text()
+    body = text[re.search(rf"\n(?:\S[^\n]*[ *])?{name}\(", text).start():]
+    return body[:body.index("\n}\n")]
+
+
+@pytest.mark.parametrize("file, function, roles", [
+    ("mxfp4_tc.cu", "mxt_produce", []), ("mxfp4_tc.cu", "mxt_kernel", ["// ---- codes to bfloat16", "// ---- MMA issuer."]),
+    ("mxfp4_tc.cu", "mxq_kernel", [])])
+def test_time_limits_begin_when_the_preceding_kernel_is_over(file, function, roles):
+    """A kernel launched programmatically may wait for its predecessor as long as that takes.  A role whose barrier comes after that wait of
+    another role waits for the predecessor first itself: the limit after which it gives up is for what its own kernel does."""
+    body = body_of(file, function)
+    cuts = [0] + [body.rindex("{", 0, body.index(mark)) for mark in roles] + [len(body)]
+    parts = [body[a:b] for a, b in zip(cuts, cuts[1:])]
+    waits = 0
+    for part in parts:
+        wait = re.search(r"mxt_wait\(|mbar_wait\(", part)
+        if wait:
+            waits += 1
+            assert "pdl_wait();" in part[:wait.start()], part[:200]
+    assert waits == max(1, len(roles))
