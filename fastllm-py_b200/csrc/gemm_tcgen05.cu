@@ -146,7 +146,9 @@ __global__ void __launch_bounds__(TC_THREADS) gemm_tc_kernel(
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            // ---- MMA issuer
+            // ---- MMA issuer.  (No stage comes before the preceding kernel is over, and the limit of a wait is not for that
+            // kernel's time.)
+            pdl_wait();
             constexpr uint32_t idesc = instr_desc_bf16(TC_BM, BN);
             bool ok = !*abort_flag;
             int s = 0;

@@ -36,7 +36,7 @@ def body_of(file, name):
 
 @pytest.mark.parametrize("file, function, roles", [
     ("mxfp4_tc.cu", "mxt_produce", []), ("mxfp4_tc.cu", "mxt_kernel", ["// ---- codes to bfloat16", "// ---- MMA issuer."]),
-    ("mxfp4_tc.cu", "mxq_kernel", [])])
+    ("mxfp4_tc.cu", "mxq_kernel", []), ("gemm_tcgen05.cu", "gemm_tc_kernel", ["// ---- producer", "// ---- MMA issuer", "// ---- epilogue"])])
 def test_time_limits_begin_when_the_preceding_kernel_is_over(file, function, roles):
     """A kernel launched programmatically may wait for its predecessor as long as that takes.  A role whose barrier comes after that wait of
     another role waits for the predecessor first itself: the limit after which it gives up is for what its own kernel does."""
