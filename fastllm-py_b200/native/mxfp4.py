@@ -12,8 +12,13 @@ points, its scales are exact, and the tensor cores of sm_100a multiply it as it 
     mxfp4.linear(x, q, out)                   # out = x q^T, x bfloat16 as it is
     mxfp4.linear_gated(x, q, out)             # out = act(x gate^T) * (x up^T), q = [gate; up]
     mxfp4.product(a, q, out)                  # out = a q^T, both in 4 bits
+    mxfp4.check(device)                       # raises if a product gave up
 
 Everything launches on the current stream of the current device and allocates nothing.  No output may overlap an operand.
+
+A tensor-core kernel whose wait gives up records that in the device's status word, which the engine's other tensor-core kernels share; its
+output is not valid, and those of the products after it are not written until the word has been looked at: by `check`, or between an
+engine's steps by the engine itself.
 """
 from __future__ import annotations
 
@@ -138,6 +143,23 @@ def _known(t: torch.Tensor):
 def reserve(device) -> None:
     """Make what products on `device` share, once, before one is captured into a graph."""
     _known(torch.empty(0, device=device))
+
+
+def check(device) -> None:
+    """Wait for `device` and raise KernelError if a kernel has recorded a fault since the last look: what products have written
+    since then is not valid, and may not have been written at all.  The record is cleared, so that products run again."""
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise KernelError(f"the engine's kernels run on a CUDA device only; got {device}")
+    if torch.cuda.is_current_stream_capturing():
+        raise KernelError("mxfp4.check waits for the device, which a stream that is being captured cannot")
+    from . import gemm_tc
+    torch.cuda.synchronize(device)
+    word = gemm_tc.status_word(device)
+    code = int(word.item())
+    if code:
+        word.zero_()
+        raise KernelError(f"mxfp4: a kernel reported error code {code} (a wait that gave up): products since the last check are not valid")
 
 
 def quantize(x: torch.Tensor, out: Matrix) -> None:

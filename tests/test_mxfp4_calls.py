@@ -27,6 +27,27 @@ def test_a_gated_product_has_a_unit(kernel):
         mxfp4.linear(bf(5, 96), w, bf(5, 64), activation=None, kernel=kernel)
 
 
+def test_a_recorded_fault_is_raised_once(monkeypatch):
+    """The status word's code is raised and cleared; no word, no error; the host has none."""
+    from fastllm_py_b200.native import gemm_tc
+
+    word, waited = torch.zeros(1, dtype=torch.int32), []
+    monkeypatch.setattr(gemm_tc, "status_word", lambda device: word)
+    monkeypatch.setattr(torch.cuda, "synchronize", waited.append)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    mxfp4.check("cuda:0")
+    word.fill_(121)
+    with pytest.raises(KernelError, match="121"):
+        mxfp4.check("cuda:0")
+    mxfp4.check(torch.device("cuda:0"))
+    assert waited == [torch.device("cuda:0")] * 3 and int(word) == 0
+    with pytest.raises(KernelError, match="CUDA device only"):
+        mxfp4.check("cpu")
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(KernelError, match="captured"):
+        mxfp4.check("cuda:0")
+
+
 def body_of(file, name):
     """From a function's name to the brace that closes it."""
     text = (CSRC / file).read_text()
