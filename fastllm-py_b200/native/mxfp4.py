@@ -170,8 +170,7 @@ def quantize(x: torch.Tensor, out: Matrix) -> None:
         raise KernelError(f"mxfp4.quantize: {tuple(x.shape)} into {out.shape}")
     code, stream = ops.dtype_code(x), _stream_of(x, data)
     rc = (_fns.get("fl_mx_quantize") or _fn(_QUANTIZE))(x.data_ptr(), code, pitch, data.data_ptr(), out.rows, out.k, stream)
-    if rc:
-        ops._check(rc, "mxfp4.quantize")
+    ops._check(rc, "mxfp4.quantize")
 
 
 def dequantize(q: Matrix, out: torch.Tensor) -> None:
@@ -181,8 +180,7 @@ def dequantize(q: Matrix, out: torch.Tensor) -> None:
         raise KernelError(f"mxfp4.dequantize: {q.shape} into {tuple(out.shape)}")
     code, stream = ops.dtype_code(out), _stream_of(data, out)
     rc = (_fns.get("fl_mx_dequantize") or _fn(_DEQUANTIZE))(data.data_ptr(), out.data_ptr(), code, pitch, q.rows, q.k, stream)
-    if rc:
-        ops._check(rc, "mxfp4.dequantize")
+    ops._check(rc, "mxfp4.dequantize")
 
 
 # The kernel for few rows takes up to 8 of them, and no more time than those on the tensor cores with matrices of up to 2^26 values
@@ -216,8 +214,7 @@ def _times_weights(name, x, w: Matrix, out, gated, n, activation, params, consta
                         sms, status, stream)
     if rc == LESS:
         rc = _fn(_FEW)(from_x, pitch, data.data_ptr(), to, code, out_pitch, m, n, k, gated, act, params[0], params[1], constant_w, sms, stream)
-    if rc:
-        ops._check(rc, name)
+    ops._check(rc, name)
 
 
 def linear(x: torch.Tensor, w: Matrix, out: torch.Tensor, activation: str | None = None, params=(0.0, 0.0),

@@ -48,6 +48,36 @@ def test_a_recorded_fault_is_raised_once(monkeypatch):
         mxfp4.check("cuda:0")
 
 
+def test_every_launch_is_counted(monkeypatch):
+    """One kernel a call, whichever launcher takes it; a refused or an empty call counts none."""
+    from fastllm_py_b200.native import ops
+
+    rc = {"fl_mxt_product": 0}
+    monkeypatch.setattr(mxfp4, "_stream_of", lambda *tensors: 0)
+    monkeypatch.setattr(mxfp4, "_known", lambda t: (0, 148))
+    monkeypatch.setattr(mxfp4, "_fns", {name: (lambda *args, name=name: rc.get(name, 0)) for name in
+                                        ("fl_mx_quantize", "fl_mx_dequantize", "fl_mx_few", "fl_mxt_product", "fl_mxq_product")})
+    w, a = mxfp4.Matrix.empty(64, 96, "cpu"), mxfp4.Matrix.empty(20, 96, "cpu")
+    calls = [lambda: mxfp4.quantize(bf(20, 96), a), lambda: mxfp4.dequantize(a, bf(20, 96)), lambda: mxfp4.linear(bf(3, 96), w, bf(3, 64)),
+             lambda: mxfp4.linear(bf(20, 96), w, bf(20, 64)), lambda: mxfp4.linear_gated(bf(20, 96), w, bf(20, 32)),
+             lambda: mxfp4.linear_gated(bf(2, 96), w, bf(2, 32)), lambda: mxfp4.product(a, w, bf(20, 64)), lambda: mxfp4.Matrix.of(bf(20, 96))]
+    for call in calls:
+        before = ops.counter.launches
+        call()
+        assert ops.counter.launches == before + 1
+    before = ops.counter.launches
+    mxfp4.linear(bf(0, 96), w, bf(0, 64))
+    rc["fl_mxt_product"] = 1
+    with pytest.raises(KernelError, match="CUDA error 1"):
+        mxfp4.linear(bf(20, 96), w, bf(20, 64))
+    assert ops.counter.launches == before
+    # a launcher that has left the call to the one for few rows has launched nothing
+    rc["fl_mxt_product"] = mxfp4.LESS
+    monkeypatch.setattr(mxfp4, "FEW_VALUES", 0)
+    mxfp4.linear(bf(3, 96), w, bf(3, 64))
+    assert ops.counter.launches == before + 1
+
+
 def body_of(file, name):
     """From a function's name to the brace that closes it."""
     text = (CSRC / file).read_text()
