@@ -50,6 +50,12 @@ class Model:
         self.engine = None
         self.sampler = None
 
+    @property
+    def matrices_in_four_bits(self) -> int:
+        """How many matrices `weights="mxfp4"` has rounded, stacked ones (q, k and v; gate and up) counted once: 0 for a model that has
+        neither dense attention nor a dense feed-forward, whose matrices all stay as they are stored."""
+        return sum(getattr(value, "_q4", None) is not None for part in self.decoder.all_parts() for value in vars(part).values())
+
     # --------------------------------------------------------------- loading
     @classmethod
     def _build(cls, arch, config, store, engine_config: EngineConfig, where: str):

@@ -83,7 +83,7 @@ def main(argv=None) -> int:
                        max_model_len=longest, cuda_graph=not args.no_graph, max_requests=4)
     cfg = model.cfg
     print(f"[load {time.time() - t0:.1f}s] {cfg.summary()} dtype={model.engine_config.dtype}"
-          + ("" if args.weights == "stored" else f" weights={args.weights}"))
+          + ("" if args.weights == "stored" else f" weights={args.weights} ({model.matrices_in_four_bits} matrices in 4 bits)"))
     if ids is None:
         import numpy as np
 

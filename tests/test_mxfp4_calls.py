@@ -78,6 +78,26 @@ def test_every_launch_is_counted(monkeypatch):
     assert ops.counter.launches == before + 1
 
 
+def test_a_model_counts_its_matrices_in_four_bits():
+    """What `weights="mxfp4"` has come to: the stacked matrices of a Linear are one, those held as stored are none."""
+    from types import SimpleNamespace as Thing
+
+    from fastllm_py_b200 import Model
+    from fastllm_py_b200.parts.linear import Linear
+
+    def linear(q4):
+        lin = Linear([bf(8, 16)])
+        lin._q4 = q4
+        return lin
+
+    q = mxfp4.Matrix.empty(8, 16, "cpu")
+    parts = [Thing(qkv=linear(q), o=linear(q)), Thing(router=linear(None), size=3), Thing(gate_up=linear(q), down=linear(None))]
+    model = Model(None, None, Thing(all_parts=lambda: iter(parts)), None)
+    assert model.matrices_in_four_bits == 3
+    parts[:] = [Thing(head=linear(None))]
+    assert model.matrices_in_four_bits == 0
+
+
 def body_of(file, name):
     """From a function's name to the brace that closes it."""
     text = (CSRC / file).read_text()

@@ -71,3 +71,13 @@ def test_models_of_other_families_in_four_bits(family, name, graph, tmp_path):
     assert np.median(errs) <= 0.08 and np.quantile(errs, 0.9) <= 0.3, (np.median(errs), np.quantile(errs, 0.9))
     assert np.median(off(stored)) > np.median(errs), "the test's model does not tell rounded matrices from stored ones"
     model.engine.check_status()
+
+
+@pytest.mark.parametrize("family, mlp, count", [("kerirax", "dense", 2), ("kerirax", None, 0)])
+def test_the_load_line_says_how_many_matrices_are_in_four_bits(family, mlp, count, tmp_path, capsys):
+    from fastllm_py_b200.cli import main
+
+    raw = kerirax_tiny.config([(kerirax_tiny.latent(2, 8, 4, 12, 10, 14), kerirax_tiny.dense(32) if mlp else None)], width=24, vocab=50)
+    folder = kerirax_tiny.write(raw, kerirax_tiny.weights(raw, seed=1), tmp_path / "model")
+    assert main([str(folder), "", "3", "--weights", "mxfp4", "--prompt-ids", "3,14,15", "--page-size", "16", "--max-model-len", "64"]) == 0
+    assert f"weights=mxfp4 ({count} matrices in 4 bits)" in capsys.readouterr().out
