@@ -121,3 +121,22 @@ def test_time_limits_begin_when_the_preceding_kernel_is_over(file, function, rol
             waits += 1
             assert "pdl_wait();" in part[:wait.start()], part[:200]
     assert waits == max(1, len(roles))
+
+
+WAITS = {
+    "mxt_produce": ["empty_bar[s], ph ^ 1u"],
+    "mxt_kernel": ["full_bar[s], ph", "a_empty[place], pa ^ 1u", "a_full[place], pa"],
+    "mxq_kernel": ["empty_bar[s], ph ^ 1u", "full_bar[s], ph"],
+    "mxp_kernel": ["w_full[s], ph", "x_full[x], xph", "a_empty[turn], pa ^ 1u", "acc_full[b], (uint32_t)(i >> 1) & 1u", "x_empty[s], ph ^ 1u",
+                   "w_empty[s], ph ^ 1u", "acc_empty[b], ((uint32_t)(i >> 1) & 1u) ^ 1u", "a_full[turn], pa"],
+    "mxqp_kernel": ["empty_bar[s], ph ^ 1u", "full_bar[s], ph", "acc_full, (uint32_t)i & 1u", "empty_bar[s], ph ^ 1u",
+                    "acc_empty, ((uint32_t)i & 1u) ^ 1u", "scales_bar[s], ph"],
+}
+
+
+@pytest.mark.parametrize("function", list(WAITS))
+def test_the_kernels_wait_as_their_model_does(function):
+    """The hand-overs that tests/test_mxfp4_barriers.py runs on the host, in the sources: every wait of each kernel, in its order.  One
+    that changes is changed in the model too, which then says whether a phase can be taken for another."""
+    body = body_of("mxfp4_pair.cuh" if function in ("mxp_kernel", "mxqp_kernel") else "mxfp4_tc.cu", function)
+    assert re.findall(r"mxt_wait\(&?(.*?), abort_flag\)", body) == WAITS[function]
