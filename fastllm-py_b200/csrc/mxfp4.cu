@@ -138,9 +138,11 @@ FL_API int fl_mx_quantize(const void* x, int code, long ld, void* data, int m, i
     return (int)cudaErrorInvalidValue;
 }
 
-// Back: the same division of the work; rows that do not begin on 16 bytes are written an element a lane, the words of a row handed round
-// by shuffles.  (Through shared memory they took as long, and twice that after a kernel without any: the SMs' memory is then divided
-// anew.)  [2048, 11008] to bfloat16 11.4 us (5.0 TB/s), [5503, 4096] to float 18.0 (5.7 TB/s), [5503, 4097] 23.3.
+// Back: the same division of the work, bound by memory; rows that do not begin on 16 bytes are written an element a lane, the words of
+// a row handed round by shuffles, and are bound by issue: 19.9 million instructions where the same rows aligned take 7.1, 85% of the
+// issue slots, and as many sectors written.  (Through shared memory they took as long, and twice that after a kernel without any:
+// the SMs' memory is then divided anew.)  [2048, 11008] to bfloat16 11.4 us (5.0 TB/s), [5503, 4096] to float 18.0 (5.7 TB/s),
+// [5503, 4097] 23.3.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __restrict__ data, T* __restrict__ out, long ld, int m,
                                                             int k, int chunks) {
@@ -225,8 +227,9 @@ FL_API int fl_mx_dequantize(const void* data, void* out, int code, long ld, int 
 }
 
 // ---------------------------------------------------------------- products of few rows
-// out[t, f] = sum_k x[t, k] W[f, k] for up to 8 tokens, or of a gated unit act(gate, up) of features f and n + f.  A CTA takes 2 x 16 rows of W (of a gated unit 16 gate rows and the 16 up
-// rows of the same features), a warp of it every WARPS-th chunk of K.  The rows are the 16 of m16n8k16 and the tokens its 8 columns.
+// out[t, f] = sum_k x[t, k] W[f, k] for up to 8 tokens, or of a gated unit act(gate, up) of features f and n + f.  A CTA takes 2 x 16
+// rows of W (of a gated unit 16 gate rows and the 16 up rows of the same features), a warp of it every WARPS-th chunk of K.  The rows
+// are the 16 of m16n8k16 and the tokens its 8 columns.
 // Lane 4 g + q reads the 16 bytes of rows g and g + 8 of block q, so a lane has one scale for 32 codes; which elements of K meet in
 // one instruction does not matter as long as both operands agree, and a lane's 8 consecutive elements of a token are the partners of
 // one word of codes.  The warps' sums meet in shared memory and are added in order.
@@ -234,10 +237,11 @@ FL_API int fl_mx_dequantize(const void* data, void* out, int code, long ld, int 
 // LB warps fit an SM.  With 20 and more a warp has registers for one chunk: its rows are loaded anew for the next one as soon as
 // their codes have been read, and its tokens at the end.  With 16 the next codes are on their way during the whole chunk.
 //
-// What bounds it: the matrix instructions.  One takes 32 clocks of a quarter of the SM for 256 values of W, and the conversion of as
-// many 18 of its integer units: 5.5 us of the 10.1 that one token 4096 -> 12288 takes (2.6 TB/s), 10 of the 16.6 for 4096 -> the gated 2 x
-// 11008 (2.9 TB/s); the rest is the way in, the join of the warps' sums and CTAs that do not fill the SMs evenly.  2 to 8 tokens take 1 to 5%
-// more.
+// What bounds it: the wait for the codes, and then issue.  One token 4096 -> 12288 takes 10.1 us (2.6 TB/s), 4096 -> the gated 2 x 11008
+// 16.6 (2.9 TB/s).  With 20 and 17 warps an SM a warp issues every 9.5 and 7.5 clocks, of which it waits 4.0 and 3.3 for memory; the
+// issue slots are 53% and 59% taken while an SM has work, and SMs have it for 86% and 90% of the busiest one's time.  The conversion of 256 values takes 18 clocks of a quarter's integer units: 3 us and 5.5 at the least.  The matrix instructions
+// bound nothing: 8 clocks of a quarter each, 21 for a link of a chain on one accumulator, which three warps a quarter hide; their pipe
+// is 0.16 and 0.19 busy.  2 to 8 tokens take 1 to 5% more.
 __device__ __forceinline__ void mx_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])

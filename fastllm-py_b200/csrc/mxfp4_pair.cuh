@@ -114,8 +114,9 @@ __device__ __forceinline__ bool mxp_epilogue(uint32_t tmem_acc, float* staged, i
 // row_tiles x token_tiles tiles; bn: tokens of a tile, a multiple of 32.
 template <typename TO, bool GATED>
 __global__ void __launch_bounds__(MXP_THREADS, 1)
-mxp_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const uint8_t* __restrict__ w, TO* __restrict__ out, long ldo, int m, int n, int k,
-           int bn, int x_stages, int token_tiles, int tiles, FlGate act, int* __restrict__ status) {
+mxp_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const uint8_t* __restrict__ w,
+           TO* __restrict__ out, long ldo, int m, int n, int k, int bn, int x_stages, int token_tiles, int tiles, FlGate act,
+           int* __restrict__ status) {
     constexpr int FEAT = GATED ? 64 : 128;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* ring = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -339,8 +340,8 @@ mxp_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CU
                     const uint64_t bdesc = smem_desc_sw128(ring_at + (uint32_t)(s * x_bytes));
 #pragma unroll
                     for (int kk = 0; kk < 8; ++kk)
-                        mxp_umma_ts(acc, tmem + 384u + turn * 64u + (uint32_t)(kk * 8), bdesc + (uint64_t)(2 * (kk & 3)) + (kk >= 4 ? half : 0), idesc,
-                                    (c > 0 || kk > 0) ? 1u : 0u);
+                        mxp_umma_ts(acc, tmem + 384u + turn * 64u + (uint32_t)(kk * 8), bdesc + (uint64_t)(2 * (kk & 3)) + (kk >= 4 ? half : 0),
+                                    idesc, (c > 0 || kk > 0) ? 1u : 0u);
                     umma_commit_pair(&a_empty[turn]);
                     umma_commit_pair(&x_empty[s]);
                     if (c == chunks - 1) umma_commit_pair(&acc_full[b]);
@@ -556,8 +557,10 @@ mxqp_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ w, TO* __
                 if (mxp_vote(*abort_flag != 0, group)) going = false;
                 if (!going) break;
                 const int last = min(32, tokens - t);
-                if (vec) mxt_rows<TO, false, 128, 128, 4, 4>(MxtSums{mine, mine, 1, 0, 0, 0}, quarter, last, dst + (long)t * ldo, ldo, left, FlGate{FL_ACT_NONE, 0.0f, 0.0f});
-                else mxt_rows<TO, false, 128, 128, 1, 4>(MxtSums{mine, mine, 1, 0, 0, 0}, quarter, last, dst + (long)t * ldo, ldo, left, FlGate{FL_ACT_NONE, 0.0f, 0.0f});
+                const MxtSums from = {mine, mine, 1, 0, 0, 0};
+                const FlGate none = {FL_ACT_NONE, 0.0f, 0.0f};
+                if (vec) mxt_rows<TO, false, 128, 128, 4, 4>(from, quarter, last, dst + (long)t * ldo, ldo, left, none);
+                else mxt_rows<TO, false, 128, 128, 1, 4>(from, quarter, last, dst + (long)t * ldo, ldo, left, none);
             }
             if (!going) break;
         }

@@ -43,9 +43,9 @@
 // sums fetched from the other CTAs by loads, 64 tokens 4096 -> 4096 took 11.6 us, 5.5 of them here.)  A CTA that gave up sends
 // what it has: the status word tells that the results are not valid.
 template <typename TO, bool GATED>
-__device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, int acc_cols, uint64_t* acc_bar, uint64_t* sent_bar, volatile int* abort_flag, int* status,
-                                           bool ok, bool any, int rows, int ranks, int rank, TO* __restrict__ out, long ldo, int f0, int n,
-                                           const FlGate act) {
+__device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, int acc_cols, uint64_t* acc_bar, uint64_t* sent_bar,
+                                           volatile int* abort_flag, int* status, bool ok, bool any, int rows, int ranks, int rank,
+                                           TO* __restrict__ out, long ldo, int f0, int n, const FlGate act) {
     constexpr int FEAT = GATED ? 128 : 256, V = 4;
     const int warp = mxt_warp(), lane = threadIdx.x & 31;
     const int share = (rows + ranks - 1) / ranks, first = min(rows, rank * share), last = min(rows, first + share);
@@ -111,7 +111,8 @@ __device__ __forceinline__ void mxt_finish(float* sums, uint32_t tmem_d, int acc
             for (int i = 1; i < ranks; ++i) {
                 const int to = rank + i < ranks ? rank + i : rank + i - ranks, t0 = to * share, tokens = min(share, rows - t0);
                 if (tokens > 0)
-                    mxt_push(parts + (rank - (rank > to)) * tokens * MXT_PITCH, sums + t0 * MXT_PITCH, (uint32_t)(tokens * MXT_PITCH * 4), sent_bar, to);
+                    mxt_push(parts + (rank - (rank > to)) * tokens * MXT_PITCH, sums + t0 * MXT_PITCH,
+                             (uint32_t)(tokens * MXT_PITCH * 4), sent_bar, to);
             }
         }
         // (a CTA that gave up waits for what is on its way to it all the same)
@@ -351,8 +352,8 @@ mxt_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict_
         }
         if (ok && mxt_elect()) umma_commit(acc_bar);
     }
-    mxt_finish<TO, GATED>(reinterpret_cast<float*>(ring), tmem_d, acc_cols, acc_bar, sent_bar, abort_flag, status, ok, c_end > c_begin, min(bn, m - t0), ranks, rank,
-                          out + (long)t0 * ldo, ldo, f0, n, act);
+    mxt_finish<TO, GATED>(reinterpret_cast<float*>(ring), tmem_d, acc_cols, acc_bar, sent_bar, abort_flag, status, ok, c_end > c_begin,
+                          min(bn, m - t0), ranks, rank, out + (long)t0 * ldo, ldo, f0, n, act);
     if (warp == MXT_WARPS && lane == 0 && *abort_flag) tma_drain(full_bar, stages, issued);
     __syncthreads();
     if (warp == MXT_WARPS + 1) tmem_dealloc(tmem_d, 512);
@@ -469,8 +470,8 @@ static int mxt_launch(const void* x, long ldx, const void* w, void* out, long ld
     CUtensorMap map;
     int rc = make_map(&map, x, m, k, ldx, bn);
     if (rc) return rc;
-    return mxt_launch_cluster(mxt_kernel<TO, GATED>, MXT_THREADS, MXT_SMEM, dim3(ranks, tokens_y, row_tiles), stream, map, (const uint8_t*)w, (TO*)out, ldo, m,
-                              n, k, bn, stages, ranks, per_rank, constant_w, act, status);
+    return mxt_launch_cluster(mxt_kernel<TO, GATED>, MXT_THREADS, MXT_SMEM, dim3(ranks, tokens_y, row_tiles), stream, map, (const uint8_t*)w,
+                              (TO*)out, ldo, m, n, k, bn, stages, ranks, per_rank, constant_w, act, status);
 }
 
 // x: bfloat16 rows, 16-byte aligned, `ldx` elements apart (a multiple of 8).  n: output features (gated: half of w's rows).

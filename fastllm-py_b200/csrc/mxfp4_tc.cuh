@@ -1,4 +1,4 @@
-// Shared by the products with matrices in 4 bits on the tensor cores (mxfp4_tc.cu, mxfp4_pair.cu): how their warps wait, issue and
+// Shared by the products with matrices in 4 bits on the tensor cores (mxfp4_tc.cu, mxfp4_pair.cuh): how their warps wait, issue and
 // give up, and how sums of tokens leave shared memory.
 #pragma once
 
@@ -145,7 +145,8 @@ __device__ __forceinline__ void mxt_cluster_arrive() { asm volatile("barrier.clu
 __device__ __forceinline__ void mxt_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // ------------------------------------------------------------------ both operands in 4 bits
-// A tile's codes as an operand of the block-scaled matrix instruction: no swizzle: `lead` bytes between core matrices along K, 128 between those of neighbouring groups of 8 rows
+// A tile's codes as an operand of the block-scaled matrix instruction, no swizzle: `lead` bytes between core matrices along K, 128
+// between those of neighbouring groups of 8 rows
 __device__ __forceinline__ uint64_t mxq_desc(uint32_t saddr, uint32_t lead) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
 }

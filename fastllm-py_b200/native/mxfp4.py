@@ -29,13 +29,13 @@ import torch
 from . import ops
 from .ops import KernelError
 
-ROWS, CHUNK_K, CHUNK_BYTES = 128, 128, 8704      # a tile's rows, a chunk's elements along K and its bytes (csrc/mxfp4.cu)
+ROWS, CHUNK_K, CHUNK_BYTES = 128, 128, 8704      # a tile's rows, a chunk's elements along K and its bytes (csrc/mxfp4.cuh)
 MOST_ROWS, MOST_K = 2**31 - 1024, 2**26 - 1024   # rows are counted in 32 bits, to the end of their tile; a grid holds 65535 x 8 chunks
 LIBRARIES = ["mxfp4", "mxfp4_tc", "gemm_tcgen05"]
 
 
 class Matrix:
-    """A matrix [rows, k] in the packed form: uint8 [ceil(rows / 128), ceil(k / 128), 8704] (csrc/mxfp4.cu says how a chunk
+    """A matrix [rows, k] in the packed form: uint8 [ceil(rows / 128), ceil(k / 128), 8704] (csrc/mxfp4.cuh says how a chunk
     lies).  Codes behind k are zero, and so are the scales of whole blocks there; rows behind the last are not read for any
     result."""
 
